@@ -14,7 +14,11 @@
 #include "gqa_cache.cuh"
 #include "gqa_combine.cuh"
 #include "gqa_prefill.cuh"
+#include "gqa_ragged.cuh"
+#include "gqa_rope.cuh"
+#include "gqa_step.cuh"
 #include "gqa_stream.cuh"
+#include "gqa_verify.cuh"
 
 namespace gqa {
 namespace {
@@ -49,6 +53,8 @@ template <typename K>
 cudaError_t set_smem(K kernel, int bytes) {
   return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
 }
+
+cudaError_t prepare_ragged();  // gqa_serving.cuh
 
 int init_device(int dev) {
   cudaDeviceProp prop;
@@ -106,6 +112,7 @@ int init_device(int dev) {
   chk(set_smem(gqa_stream_kernel<128, false, 1, false, true>, StreamCfg<128>::kSmemBytes));
   chk(set_smem(gqa_stream_kernel<64, true, 1, false, true>, StreamCfg<64>::kSmemBytes));
   chk(set_smem(gqa_stream_kernel<64, false, 1, false, true>, StreamCfg<64>::kSmemBytes));
+  chk(prepare_ragged());
   if (e != cudaSuccess) return GQA_ERR_CUDA;
   return GQA_OK;
 }
@@ -1215,3 +1222,5 @@ int gqa_device_error(int* code, int* site, int clear) {
 }
 
 }  // extern "C"
+
+#include "gqa_serving.cuh"

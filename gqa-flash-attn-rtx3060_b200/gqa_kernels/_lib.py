@@ -20,6 +20,7 @@ LIB_PATH = (os.path.join(_HERE, "libgqa_sm100_debug.so") if _SEL == "debug"
 
 GQA_DTYPE_F16 = 0
 GQA_DTYPE_BF16 = 1
+GQA_DTYPE_F32 = 2
 
 _P = ctypes.c_void_p
 _I64P = ctypes.POINTER(ctypes.c_int64)
@@ -72,6 +73,20 @@ SIGNATURES = {
     "gqa_lse_combine_peer": (_I, [_P, _P, _P, _I, ctypes.c_int64, ctypes.c_int64, _I, _P, _I64P, _I, _I, _I, _I, _I,
                                   _P]),
 }
+
+_I64 = ctypes.c_int64
+SIGNATURES.update({
+    "gqa_step_plan": (_I, [_P, _P, _P, _I64, _P, _P, _I, _P, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P, _P]),
+    "gqa_qk_norm_rope": (_I, [_P, _P, _P, _I64P, _I64P, _I64P, _P, _P, _P, _I64, _I, _P, _P, _I, _I, _I, _P, _P, _P, _P,
+                              _I, _I, _I, _I, _I, _I, _I, _I, _F, _F, _F, _P]),
+    "gqa_ragged_fwd_workspace_bytes": (_SZ, [_I, _I, _I, _I, _I, _I, _I, _I]),
+    "gqa_ragged_fwd": (_I, [_P, _P, _P, _P, _P, _I64P, _I64P, _I64P, _I64P, _P, _I, _P, _P, _P, _P, _P,
+                            _I, _I, _I, _I, _I, _I, _I, _I, _I, _F, _F, _I, _I, _I, _I, _F, _F, _P, _SZ, _P]),
+    "gqa_verify_workspace_bytes": (_SZ, [_I, _I, _I, _I]),
+    "gqa_verify_drafts": (_I, [_P, _I64, _P, _I64, _P, _I64P, _P, _I64, _P, _I64, _P, _P, _P, _I, _I, _I, _I, _I, _P, _SZ,
+                               _P]),
+    "gqa_verify_greedy": (_I, [_P, _I64, _P, _I64, _P, _P, _P, _I, _I, _I, _I, _I, _P, _SZ, _P]),
+})
 
 _lib = None
 _lock = threading.Lock()
@@ -229,6 +244,9 @@ class WorkspaceCache:
 
 
 WORKSPACES = WorkspaceCache()
+# The ragged serving step's: its counters have one place for every shape, so one
+# signature serves all calls and nothing is zeroed after the allocation.
+SERVING_WORKSPACES = WorkspaceCache()
 
 
 def device_error(clear=True):
@@ -242,5 +260,6 @@ def device_error(clear=True):
     site = ctypes.c_int(0)
     check(load().gqa_device_error(ctypes.byref(code), ctypes.byref(site), 1 if clear else 0), "gqa_device_error")
     if code.value != 0:
-        WORKSPACES.drop(torch.device("cuda", torch.cuda.current_device()))
+        for cache in (WORKSPACES, SERVING_WORKSPACES):
+            cache.drop(torch.device("cuda", torch.cuda.current_device()))
     return code.value, site.value

@@ -1,0 +1,192 @@
+"""Attention of a ragged step over the paged cache.
+
+`paged_ragged_attention` attends every request's own number of new tokens in one call:
+decodes, drafted tokens and chunks of prompts side by side, which paged_decode and
+paged_prefill (one chunk length per call) cannot. The lengths stay on the GPU. Scores can
+be capped by a tanh or biased by distance, and each token's visible keys are an interval
+that combines the causal rule, a window, a prefix that every token sees, and documents
+packed into one request.
+
+`RaggedPagedAttention` ties the step's operators together as one attention layer.
+"""
+import torch
+
+from . import _lib
+from .qk_rope import qk_norm_rope_append
+
+__all__ = ["paged_ragged_attention", "RaggedPagedAttention"]
+
+
+def _optional(t, name, dtype, shape, query):
+    if t is None:
+        return None
+    if t.dtype != dtype or t.shape != shape:
+        raise ValueError(f"{name} must be {dtype} {tuple(shape)}")
+    if t.device != query.device:
+        raise ValueError("tensors must be on one device")
+    return (t if t.is_contiguous() else t.contiguous())
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def paged_ragged_attention(query, key_cache, value_cache, block_tables, cu_query_lens, seq_lens, max_query_len=None,
+                           max_seq_len=None, scale=None, causal=True, softcap=0.0, alibi_slopes=None, window=None,
+                           prefix_lens=None, key_starts=None, k_scale=1.0, v_scale=1.0, return_lse=False, out=None):
+    """Attention of each request's new tokens over its cached keys.
+
+    Args:
+        query: (num_tokens, num_heads, head_dim), bf16 or fp16, the requests' tokens one
+            after the other; head_dim 64 or 128, d stride 1.
+        key_cache, value_cache: (num_blocks, block_size, num_kv_heads, head_dim), d stride 1,
+            block_size a power of two >= 16; query's dtype, or float8_e4m3fn (head_dim 128)
+            with key = stored key * k_scale and value = stored value * v_scale. num_heads
+            is any multiple (up to 64) of num_kv_heads.
+        block_tables: int32 (num_seqs, max_blocks); request b's key k is in block
+            block_tables[b, k // block_size] at position k % block_size.
+        cu_query_lens: int32 (num_seqs + 1,); request b's tokens are rows
+            cu_query_lens[b] .. cu_query_lens[b + 1] - 1 of query. Rows past the last
+            request's (padding) are not written.
+        seq_lens: int32 (num_seqs,), cached keys of each request, its new tokens' included:
+            token i of q new ones is at position seq_lens[b] - q + i.
+        max_query_len, max_seq_len: upper bounds of the query lengths and of seq_lens, which
+            size the launch; they must hold (keys past max_seq_len are not seen). Defaults:
+            num_tokens and the tables' capacity.
+        scale: softmax scale; defaults to head_dim ** -0.5.
+        causal: a token sees the keys up to its own position; False: all of the request's.
+        softcap: scores become softcap * tanh(score / softcap); 0: not.
+        alibi_slopes: float32 (num_heads,): slope * |distance| is taken off the (capped) score.
+        window: a token sees at most this many keys back, its own included.
+        prefix_lens: int32 (num_seqs,): the first prefix_lens[b] keys are seen by every token
+            of request b (within its window).
+        key_starts: int32 (num_tokens,): the first key that each token sees, e.g. where its
+            document begins.
+        return_lse: also return the log-sum-exp of each row's scores.
+        out: optional output of query's shape and dtype, d stride 1.
+
+    Returns:
+        (num_tokens, num_heads, head_dim) in query's dtype, and with return_lse float32
+        (num_tokens, num_heads). A token that sees no key gives zeros and -inf (where
+        gqa_flash_attn and paged_prefill give NaN, the reference's rule: here masks that
+        leave a row empty are ordinary). Asynchronous on the current stream.
+    """
+    if query.dim() != 3 or key_cache.dim() != 4:
+        raise ValueError("query must be (num_tokens, num_heads, head_dim) and the caches "
+                         "(num_blocks, block_size, num_kv_heads, head_dim)")
+    num_tokens, num_heads, head_dim = query.shape
+    num_blocks, block_size, num_kv_heads, hd = key_cache.shape
+    num_seqs = seq_lens.shape[0]
+    if hd != head_dim or value_cache.shape != key_cache.shape:
+        raise ValueError("key_cache and value_cache must be (num_blocks, block_size, num_kv_heads, head_dim)")
+    if num_heads % num_kv_heads:
+        raise ValueError("num_heads must be divisible by num_kv_heads")
+    dtype = _lib.dtype_code(query)
+    fp8 = key_cache.dtype == torch.float8_e4m3fn
+    if key_cache.dtype != value_cache.dtype or not (fp8 or key_cache.dtype == query.dtype):
+        raise TypeError("the caches must share query's dtype, or both be float8_e4m3fn")
+    if block_tables.dtype != torch.int32 or seq_lens.dtype != torch.int32 or cu_query_lens.dtype != torch.int32:
+        raise TypeError("block_tables, cu_query_lens and seq_lens must be int32")
+    if block_tables.dim() != 2 or block_tables.shape[0] != num_seqs or seq_lens.dim() != 1 \
+            or cu_query_lens.shape != (num_seqs + 1,):
+        raise ValueError("block_tables must be (num_seqs, max_blocks), seq_lens (num_seqs,) and cu_query_lens (num_seqs + 1,)")
+    if window is not None and window < 1:
+        raise ValueError("window must be at least 1")
+    if softcap < 0:
+        raise ValueError("softcap must not be negative")
+    if not causal and (window is not None or prefix_lens is not None):
+        raise ValueError("window and prefix_lens need causal")
+    if fp8 and not (k_scale > 0 and v_scale > 0):
+        raise ValueError("fp8 caches need positive k_scale and v_scale")
+    _lib.check_one_device(query, key_cache, value_cache, block_tables, cu_query_lens, seq_lens)
+    alibi_slopes = _optional(alibi_slopes, "alibi_slopes", torch.float32, (num_heads,), query)
+    prefix_lens = _optional(prefix_lens, "prefix_lens", torch.int32, (num_seqs,), query)
+    key_starts = _optional(key_starts, "key_starts", torch.int32, (num_tokens,), query)
+    if not block_tables.is_contiguous():
+        block_tables = block_tables.contiguous()
+    if not seq_lens.is_contiguous():
+        seq_lens = seq_lens.contiguous()
+    if not cu_query_lens.is_contiguous():
+        cu_query_lens = cu_query_lens.contiguous()
+    if not _lib.tma_compatible(query):
+        query = query.contiguous()
+    capacity = block_tables.shape[1] * block_size
+    max_seq_len = capacity if max_seq_len is None else min(int(max_seq_len), capacity)
+    max_query_len = num_tokens if max_query_len is None else int(max_query_len)
+    if out is None:
+        out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
+    else:
+        if out.shape != query.shape or out.dtype != query.dtype:
+            raise ValueError("out must have query's shape and dtype")
+        _lib.check_one_device(query, out)
+    dev = query.device
+    lse = torch.empty((num_tokens, num_heads), dtype=torch.float32, device=dev) if return_lse else None
+    with _lib.on_device(dev):
+        nbytes = _lib.workspace_bytes("gqa_ragged_fwd_workspace_bytes", num_seqs, num_tokens, num_heads, num_kv_heads,
+                                      max_query_len, max_seq_len, head_dim,
+                                      0 if window is None or prefix_lens is not None else window)
+        ws = _lib.SERVING_WORKSPACES.get(dev, nbytes, None).data_ptr() if nbytes else None
+        rc = _lib.load().gqa_ragged_fwd(
+            query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), out.data_ptr(), _ptr(lse),
+            _lib.strides(query, 3), _lib.strides(key_cache), _lib.strides(value_cache), _lib.strides(out, 3),
+            block_tables.data_ptr(), block_tables.stride(0), cu_query_lens.data_ptr(), seq_lens.data_ptr(),
+            _ptr(alibi_slopes), _ptr(prefix_lens), _ptr(key_starts), num_seqs, num_tokens, num_heads, num_kv_heads, head_dim,
+            block_size, num_blocks, max_query_len, max_seq_len, head_dim ** -0.5 if scale is None else scale, softcap,
+            0 if window is None else window, 1 if causal else 0, dtype, 1 if fp8 else 0, k_scale, v_scale, ws, nbytes,
+            _lib.stream_ptr(dev))
+        if rc != 0:
+            _lib.SERVING_WORKSPACES.drop(dev)
+    _lib.check(rc, "gqa_ragged_fwd")
+    return (out, lse) if return_lse else out
+
+
+class RaggedPagedAttention:
+    """The attention layer of a ragged step: forward(qkv, plan, ...) normalises and rotates
+    the heads, writes K and V into the layer's cache and attends.
+
+    Args:
+        num_heads, num_kv_heads, head_dim: the layer's heads.
+        cos_sin: the rotation table (qk_rope.rope_table).
+        q_weight, k_weight, eps: the heads' RMS norm (None: no norm).
+        sections, interleaved: see qk_norm_rope_append.
+        scale, softcap, window, alibi_slopes: see paged_ragged_attention.
+        kv_cache_dtype, k_scale, v_scale: "auto" (the model's dtype) or "fp8_e4m3".
+    """
+
+    def __init__(self, num_heads, num_kv_heads, head_dim, cos_sin, q_weight=None, k_weight=None, eps=1e-6, sections=None,
+                 interleaved=False, scale=None, softcap=0.0, window=None, alibi_slopes=None, kv_cache_dtype="auto",
+                 k_scale=1.0, v_scale=1.0):
+        if num_heads % num_kv_heads:
+            raise ValueError("num_heads must be a multiple of num_kv_heads")
+        if kv_cache_dtype not in ("auto", "fp8_e4m3"):
+            raise ValueError("kv_cache_dtype must be 'auto' or 'fp8_e4m3'")
+        self.num_heads, self.num_kv_heads, self.head_dim = num_heads, num_kv_heads, head_dim
+        self.cos_sin, self.q_weight, self.k_weight, self.eps = cos_sin, q_weight, k_weight, eps
+        self.sections, self.interleaved = sections, interleaved
+        self.scale, self.softcap, self.window, self.alibi_slopes = scale, softcap, window, alibi_slopes
+        self.kv_cache_dtype, self.k_scale, self.v_scale = kv_cache_dtype, k_scale, v_scale
+
+    def allocate_kv_cache(self, num_blocks, block_size, dtype, device):
+        """A zeroed (2, num_blocks, block_size, num_kv_heads, head_dim) cache: [0] keys, [1] values."""
+        dt = torch.float8_e4m3fn if self.kv_cache_dtype == "fp8_e4m3" else dtype
+        return torch.zeros(2, num_blocks, block_size, self.num_kv_heads, self.head_dim, dtype=dt, device=device)
+
+    def forward(self, qkv, kv_cache, plan, block_tables, max_query_len, max_seq_len=None, positions=None, prefix_lens=None,
+                key_starts=None):
+        """qkv (num_tokens, (num_heads + 2 num_kv_heads) * head_dim), the fused projection of the
+        packed tokens; plan a StepPlan of at least num_tokens. positions defaults to the
+        plan's (pass (axes, num_tokens) for several axes). Returns (num_tokens, num_heads *
+        head_dim); rows of padding tokens are undefined."""
+        t = qkv.shape[0]
+        x = qkv.view(t, self.num_heads + 2 * self.num_kv_heads, self.head_dim)
+        q = x[:, :self.num_heads]
+        k = x[:, self.num_heads:self.num_heads + self.num_kv_heads]
+        v = x[:, self.num_heads + self.num_kv_heads:]
+        positions = plan.positions[:t] if positions is None else positions
+        q = qk_norm_rope_append(q, k, v, positions, self.cos_sin, kv_cache[0], kv_cache[1], plan.slot_mapping[:t],
+                                self.q_weight, self.k_weight, self.eps, self.sections, self.interleaved,
+                                k_scale=self.k_scale, v_scale=self.v_scale)
+        o = paged_ragged_attention(q, kv_cache[0], kv_cache[1], block_tables, plan.cu_query_lens, plan.seq_lens,
+                                   max_query_len, max_seq_len, self.scale, True, self.softcap, self.alibi_slopes, self.window,
+                                   prefix_lens, key_starts, self.k_scale, self.v_scale)
+        return o.view(t, self.num_heads * self.head_dim)

@@ -44,6 +44,7 @@ extern "C" {
 
 #define GQA_DTYPE_F16 0
 #define GQA_DTYPE_BF16 1
+#define GQA_DTYPE_F32 2 /* gqa_verify_* only */
 
 /* Text for a status code (static storage). */
 const char* gqa_strerror(int code);
@@ -307,6 +308,120 @@ int gqa_paged_kv_append(const void* key, const void* value, const int64_t* k_str
                         void* k_cache, void* v_cache, const int64_t* slot_mapping, int num_tokens, int num_kv_heads,
                         int head_dim, int block_size, int num_blocks, int dtype, int cache_fp8, float k_scale,
                         float v_scale, void* stream);
+
+/*
+ * The ragged serving step: requests of any number of new tokens each (one for a
+ * decode, a few drafted ones, a prompt or a chunk of one) planned, rotated, cached,
+ * attended and verified without the host reading a length. No reference counterpart
+ * (the roadmap's vLLM-shaped interface, README.md:144); the attention's definition is
+ * gqa_kernels/gqa_fwd.py's with more masks.
+ *
+ * gqa_step_plan: from query_lens[b] new and context_lens[b] cached tokens of each
+ * request, the blocks it gains, and its tokens' positions and cache slots. Request b
+ * holds blocks_held[b] entries of its row of block_tables (row stride bt_stride >=
+ * max_blocks); it needs ceil((context + query) / block_size) in all. Requests are granted
+ * in order while the pool's free_count[0] ids on top of the stack free_blocks
+ * (num_free long) last; the j-th block handed out is free_blocks[free_count - 1 - j]. A
+ * request that the pool or the table's width refuses gets granted 0, slots of -1 and
+ * seq_lens[b] = context_lens[b]. Outputs: cu_query_lens (num_seqs + 1), seq_lens,
+ * granted and blocks_held_out (num_seqs), free_count_out (1), and per token, packed by
+ * request, positions, slot_mapping and token_seqs (max_tokens; -1 past the step's
+ * tokens). New table entries are written into block_tables. The inputs blocks_held,
+ * free_count and context_lens must not be the outputs of the same name. More tokens than
+ * max_tokens are dropped and reported (GQA_ERR_INVALID_ARG, site 211). block_size: a
+ * power of two.
+ */
+int gqa_step_plan(const int* query_lens, const int* context_lens, int* block_tables, int64_t bt_stride,
+                  const int* blocks_held, const int* free_blocks, int num_free, const int* free_count, int num_seqs,
+                  int max_blocks, int block_size, int max_tokens, int* cu_query_lens, int* seq_lens, int* positions,
+                  int64_t* slot_mapping, int* token_seqs, unsigned char* granted, int* blocks_held_out,
+                  int* free_count_out, void* stream);
+
+/*
+ * gqa_qk_norm_rope: RMS norm of every query and key head (weights of head_dim values in
+ * the tensors' dtype, or NULL: no norm), the position rotation, and the cache write.
+ * q (num_tokens, num_heads, head_dim), k and v (num_tokens, num_kv_heads, head_dim), element
+ * strides of three dimensions (d stride 1, the others multiples of 8). Positions: axis
+ * a of token t at positions[a * pos_stride + t]; the rotary_dim / 2 frequencies belong to
+ * the axes (1 to 4) in consecutive sections[a] (NULL with one axis). cos_sin is float32
+ * (max_positions, rotary_dim), cosines then sines; rotary_dim a multiple of 16 up to
+ * head_dim. Pairs are (f, f + rotary_dim / 2), interleaved: (2f, 2f + 1). q_out is
+ * (num_tokens, num_heads, head_dim), contiguous. With slot_mapping, k and v go to the
+ * contiguous caches k_dst / v_dst (num_blocks, block_size, num_kv_heads, head_dim) as
+ * gqa_paged_kv_append writes them (negative slots skipped; slots past the cache skipped
+ * and reported at site 213; e4m3 with cache_fp8); without, k goes to k_dst
+ * (num_tokens, num_kv_heads, head_dim) and v is not read. A token with a negative
+ * position (padding) gives zero rows and caches nothing; one with a position past the
+ * table too, and is reported (site 212). Arithmetic is fp32 with one rounding.
+ */
+int gqa_qk_norm_rope(const void* q, const void* k, const void* v, const int64_t* q_strides3, const int64_t* k_strides3,
+                     const int64_t* v_strides3, const void* q_weight, const void* k_weight, const int* positions,
+                     int64_t pos_stride, int axes, const int* sections, const float* cos_sin, int max_positions,
+                     int rotary_dim, int interleaved, void* q_out, void* k_dst, void* v_dst, const int64_t* slot_mapping,
+                     int num_tokens, int num_heads, int num_kv_heads, int head_dim, int block_size, int num_blocks,
+                     int dtype, int cache_fp8, float eps, float k_scale, float v_scale, void* stream);
+
+/*
+ * gqa_ragged_fwd: attention of request b's new tokens, rows cu_query_lens[b] ..
+ * cu_query_lens[b + 1] - 1 of q / o (num_tokens, num_heads, head_dim; element strides of
+ * three dimensions), over its seq_lens[b] cached keys, the new tokens' own being the
+ * last. The caches are (num_blocks, block_size, num_kv_heads, head_dim) with element
+ * strides of four dimensions (d stride 1, the others multiples of 16 bytes), block_size
+ * a power of two >= 16. Token i of request b, at position p = seq_lens[b] - (its query
+ * length) + i, sees keys [max(0, p - window + 1, key_starts[token]),
+ * min(seq_lens[b], max(p + 1, prefix_lens[b]))): window 0, key_starts NULL and
+ * prefix_lens NULL leave those terms out; without `causal` it sees all seq_lens[b] keys
+ * from key_starts on (window and prefix_lens are then errors). Scores are
+ * s = q.k * scale, then softcap * tanh(s / softcap) if softcap > 0, then
+ * - alibi_slopes[head] * |p - key| if given. A token that sees no key gives 0 (unlike
+ * gqa_fwd's NaN, which is the reference's rule) and lse -inf. lse (num_tokens,
+ * num_heads), float32, natural log, may be NULL. Groups of up to 64 heads, any number.
+ * e4m3 caches (cache_fp8, scales as gqa_paged_fwd_kv8) need head_dim 128. max_query_len
+ * and max_seq_len bound the lengths and must hold; longer sequences are clipped.
+ * Workspace: gqa_ragged_fwd_workspace_bytes (window as passed, 0 with prefix_lens or
+ * without causal), zeroed before its first use; every call leaves its counters zero,
+ * whatever its shape, so calls of all shapes on one stream share one workspace. With less
+ * the key axis is not split.
+ */
+size_t gqa_ragged_fwd_workspace_bytes(int num_seqs, int num_tokens, int num_heads, int num_kv_heads, int max_query_len,
+                                      int max_seq_len, int head_dim, int window);
+int gqa_ragged_fwd(const void* q, const void* k_cache, const void* v_cache, void* o, float* lse,
+                   const int64_t* q_strides3, const int64_t* k_strides4, const int64_t* v_strides4,
+                   const int64_t* o_strides3, const int* block_table, int bt_stride, const int* cu_query_lens,
+                   const int* seq_lens, const float* alibi_slopes, const int* prefix_lens, const int* key_starts,
+                   int num_seqs, int num_tokens, int num_heads, int num_kv_heads, int head_dim, int block_size,
+                   int num_blocks, int max_query_len, int max_seq_len, float scale, float softcap, int window, int causal,
+                   int dtype, int cache_fp8, float k_scale, float v_scale, void* workspace, size_t workspace_bytes,
+                   void* stream);
+
+/*
+ * gqa_verify_drafts: request b owns rows cu_query_lens[b] .. of the target's
+ * probabilities (num_rows, vocab); row i is the distribution after its first i drafted
+ * tokens draft_tokens[b][0 ..] (at most max_drafts <= 64, one fewer than its rows). Draft i
+ * is accepted while uniforms[b][i] * draft_probs[b][i][d] < target[i][d] (draft_probs
+ * NULL: 1 * uniforms); the token after the accepted ones is the argmax over j of
+ * max(target[i][j] - draft_probs[b][i][j], 0) / exponentials[b][j] (of target[i][j] /
+ * exponentials[b][j] after the last draft; without draft_probs the refused token's
+ * weight is 0), ties to the lowest index, or, if no weight is positive, the row's first
+ * largest probability. tokens (num_seqs, max_drafts + 1): accepted drafts, then that
+ * token, then -1; num_tokens (num_seqs): how many. A request without rows gives 0
+ * tokens. Probabilities share dtype (GQA_DTYPE_F32, _BF16 or _F16); uniforms and
+ * exponentials are float32. Strides in elements, the vocabulary's is 1. A draft outside
+ * [0, vocab) is refused. gqa_verify_greedy: draft i is accepted while it is row i's
+ * first largest entry, and the next token is that of the row after; `target` may hold
+ * logits. At most 16384 requests.
+ * The workspace (gqa_verify_workspace_bytes) may be gqa_ragged_fwd's: its counters
+ * have the same place and are left zero too.
+ */
+size_t gqa_verify_workspace_bytes(int num_seqs, int max_drafts, int vocab, int greedy);
+int gqa_verify_drafts(const int* draft_tokens, int64_t draft_token_stride, const void* target_probs, int64_t target_stride,
+                      const void* draft_probs, const int64_t* draft_strides2, const float* uniforms,
+                      int64_t uniform_stride, const float* exponentials, int64_t exponential_stride,
+                      const int* cu_query_lens, int* tokens, int* num_tokens, int num_seqs, int num_rows, int max_drafts,
+                      int vocab, int dtype, void* workspace, size_t workspace_bytes, void* stream);
+int gqa_verify_greedy(const int* draft_tokens, int64_t draft_token_stride, const void* target, int64_t target_stride,
+                      const int* cu_query_lens, int* tokens, int* num_tokens, int num_seqs, int num_rows, int max_drafts,
+                      int vocab, int dtype, void* workspace, size_t workspace_bytes, void* stream);
 
 /*
  * The tcgen05 prefill path's launch plan for a shape on `sm_count` SMs, without
