@@ -93,14 +93,14 @@ struct RaggedWork {
   int k_base, n_chunks;    // k_lo down to a box, chunks that hold keys (at least 1)
 };
 
-// The union over the tile's rows, by one warp. False: no such tile, or not this kernel's.
-__device__ __forceinline__ bool ragged_work(const RaggedParams& p, int slot, int lane, RaggedWork& w) {
-  w.b = p.one_tile ? slot : ragged_slot(p, slot, lane);
-  if (w.b < 0) return false;
-  const int first = p.cu[w.b];
-  const int qn = min(p.cu[w.b + 1], p.num_tokens) - first;
-  w.m0 = p.one_tile ? 0 : (slot - (first / p.block_m + w.b)) * p.block_m;
-  if (first < 0 || w.m0 < 0 || w.m0 >= qn) return false;
+// The tile of request b that starts at its token m0: the union over its rows, by one warp.
+// False: no such tile, or not this kernel's.
+__device__ __forceinline__ bool ragged_work_at(const RaggedParams& p, int b, int m0, int lane, RaggedWork& w) {
+  w.b = b;
+  w.m0 = m0;
+  const int first = p.cu[b];
+  const int qn = min(p.cu[b + 1], p.num_tokens) - first;
+  if (first < 0 || m0 < 0 || m0 >= qn) return false;
   const int64_t qrows = (int64_t)qn * p.group;
   if (qrows < p.min_rows || qrows > p.max_rows) return false;
   w.t0 = first + w.m0;
@@ -124,6 +124,11 @@ __device__ __forceinline__ bool ragged_work(const RaggedParams& p, int slot, int
   w.k_base = min(w.k_lo, w.k_hi) & ~(p.box - 1);
   w.n_chunks = w.k_hi > w.k_lo ? (w.k_hi - w.k_base + p.chunk - 1) / p.chunk : 1;
   return true;
+}
+__device__ __forceinline__ bool ragged_work(const RaggedParams& p, int slot, int lane, RaggedWork& w) {
+  const int b = p.one_tile ? slot : ragged_slot(p, slot, lane);
+  if (b < 0) return false;
+  return ragged_work_at(p, b, p.one_tile ? 0 : (slot - (p.cu[b] / p.block_m + b)) * p.block_m, lane, w);
 }
 
 // The interval of the row of token t0 + i.

@@ -1,0 +1,674 @@
+// tcgen05 / TMEM / TMA form of the ragged attention (gqa_ragged.cuh has the masks, the
+// scores and the work of a tile): requests of more than 64 packed rows, i.e. prompts and
+// chunks of them. The pipeline is the dense prefill kernel's (gqa_prefill.cuh): one CTA
+// owns two 128-row query tiles of one (request, kv head), a TMA warp streams 128-key
+// tiles of K and V from the paged cache, one thread issues the UMMAs
+//   S_i = Q_i K_j^T (f32 in TMEM),   O_i += P_i V_j (P from TMEM)
+// and a warpgroup per tile turns S into P with the online softmax, the two tiles taking
+// turns on the tensor core. What differs:
+//  - Rows are packed token-major (row = token x group + head), so a tile's tokens are
+//    consecutive rows of the packed queries and any group up to 64 fits:
+//    bm = 128 / group tokens per tile, 128 - bm x group rows idle.
+//  - The key range is the union of the two tiles' intervals, and every row has its own
+//    [lo, hi) in it. A row's running maximum starts at a finite -3e38, so that tiles
+//    where it sees nothing add exp2(-inf) = 0; rows that saw nothing end with l = 0.
+//  - Scores may be capped or biased (MOD), see below.
+//  - O leaves through shared memory with ordinary 16-byte stores, since a tile may end
+//    where the next request's rows begin.
+//
+// Work is found on the device: every CTA scans the requests' lengths (one load and one
+// block scan per 384 requests) and takes its tile from the end, so that of one prompt the
+// tiles with the most keys start first. The host's grid covers the most tiles that the
+// step can have; CTAs past the real number return before they touch TMEM.
+//
+// Bound by the tensor core and the softmax's exponentials together (gqa_prefill.cuh has
+// the accounting). The cap costs two more MUFU operations per score, exp2 and a reciprocal.
+#pragma once
+
+#include "gqa_prefill.cuh"
+#include "gqa_ragged.cuh"
+
+namespace gqa {
+
+// Score transforms of an instantiation: kRaggedPlain none; kRaggedCap the cap alone
+// (monotone, so the row maximum is taken before it); kRaggedBias a distance bias, capped or not.
+enum : int { kRaggedPlain = 0, kRaggedCap = 1, kRaggedBias = 2 };
+
+template <int HD>
+struct RaggedTileCfg : PrefillCfg<HD> {
+  using Base = PrefillCfg<HD>;
+  // tmem base, abort flag, last-CTA flag, work item, warp sums of the scan
+  static constexpr int kWorkOff = Base::kMiscOff + 16;
+  static constexpr int kSmemBytes = kWorkOff + 64 + 64 + 1024;
+};
+
+template <int HD, bool BF16, int MOD>
+__global__ void __launch_bounds__(384, 1)
+    gqa_ragged_tile_kernel(const RaggedParams p, const __grid_constant__ CUtensorMap qmap,
+                           const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
+  using Cfg = RaggedTileCfg<HD>;
+  constexpr int NSUB = Cfg::kNSub;
+  constexpr int SLOTS = Cfg::kSlots;
+  constexpr int BN = Cfg::kBN;
+
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_base = smem_u32(smem_raw);
+  const uint32_t base = (raw_base + 1023u) & ~1023u;
+  uint8_t* const smem = smem_raw + (base - raw_base);
+
+  const uint32_t q_smem0 = base + Cfg::kQOff;
+  const uint32_t kv_smem0 = base + Cfg::kKVOff;
+  const uint32_t bars = base + Cfg::kBarOff;
+  const uint32_t bar_q_full = bars;                             // [2]
+  const uint32_t bar_kv_full = bars + 16;                       // [SLOTS]
+  const uint32_t bar_kv_empty = bar_kv_full + 8 * SLOTS;        // [SLOTS]
+  const uint32_t bar_s_full = bar_kv_empty + 8 * SLOTS;         // [2]
+  const uint32_t bar_p_full = bar_s_full + 16;                  // [2][kPParts]
+  const uint32_t bar_o_final = bar_p_full + 16 * Cfg::kPParts;  // [2]
+  const uint32_t bar_mma_done = bar_o_final + 16;
+  uint32_t* tmem_base_ptr = reinterpret_cast<uint32_t*>(smem + Cfg::kMiscOff);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + Cfg::kMiscOff + 4);
+
+  // The work item, in shared memory: the softmax warps have no registers to spare, so its
+  // fields are read where they are used.
+  struct Work {
+    int t0, nq, off_m0, len;  // first token's row, tokens, position of the first token, the request's keys
+    int b, k_lo, k_hi;        // request; union of the rows' intervals
+    int key0, nk, n_chunks;   // this CTA's first key, its 128-key tiles; chunks of the tile
+    int unit;
+    int found;                // the scan's answer: request (-1: none) and tile of it
+    int local;
+  };
+  volatile Work* const work = reinterpret_cast<volatile Work*>(smem + Cfg::kWorkOff);
+  int* const scan_sums = reinterpret_cast<int*>(smem + Cfg::kWorkOff + 64);
+
+  const int tid = threadIdx.x;
+  const int warp = tid >> 5;
+  const int lane = tid & 31;
+  const unsigned n_inner = (unsigned)(p.hkv * p.nsplit);
+  const int tile_id = (int)(blockIdx.x / n_inner);
+  const int kvh = (int)((blockIdx.x % n_inner) / (unsigned)p.nsplit);
+  const int split = (int)(blockIdx.x % (unsigned)p.nsplit);
+  const int bm = p.block_m >> 1;  // tokens per query tile
+
+  if (tid == 0) {
+    mbar_init(bar_q_full, 1);
+    mbar_init(bar_q_full + 8, 1);
+    for (int s = 0; s < SLOTS; ++s) {
+      mbar_init(bar_kv_full + 8 * s, 1);
+      mbar_init(bar_kv_empty + 8 * s, 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(bar_s_full + 8 * i, 1);
+      for (int h = 0; h < Cfg::kPParts; ++h) mbar_init(bar_p_full + 8 * (Cfg::kPParts * i + h), 128);
+      mbar_init(bar_o_final + 8 * i, 1);
+    }
+    mbar_init(bar_mma_done, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+    fence_proxy_async_smem();
+    work->found = -1;
+  }
+  pdl_wait();
+  pdl_trigger();
+
+  // ---- which tile: count the tiles of every request that is this kernel's, and take
+  // number (total - 1 - tile_id). The first pass counts, the second finds; with at most
+  // 384 requests the lengths stay in registers in between.
+  {
+    auto tiles_of = [&](int b) -> int {
+      if (b >= p.n) return 0;
+      const int first = p.cu[b];
+      const int qn = min(p.cu[b + 1], p.num_tokens) - first;
+      if (first < 0 || qn <= 0 || (int64_t)qn * p.group < p.min_rows) return 0;
+      return (qn + p.block_m - 1) / p.block_m;
+    };
+    const int rounds = (p.n + 383) / 384;
+    const int mine = tiles_of(tid);
+    int total = 0;
+    for (int r = 0; r < rounds; ++r) {
+      const int s = __reduce_add_sync(0xffffffffu, r ? tiles_of(r * 384 + tid) : mine);
+      __syncthreads();
+      if (lane == 0) scan_sums[warp] = s;
+      __syncthreads();
+      for (int w = 0; w < 12; ++w) total += scan_sums[w];
+    }
+    const int want = total - 1 - tile_id;
+    if (want < 0) return;  // the whole CTA, before TMEM
+    int before = 0;
+    for (int r = 0; r < rounds; ++r) {
+      const int c = r ? tiles_of(r * 384 + tid) : mine;
+      int incl = c;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, incl, d);
+        if (lane >= d) incl += y;
+      }
+      if (rounds > 1) {  // one round: scan_sums still has the warps' sums
+        __syncthreads();
+        if (lane == 31) scan_sums[warp] = incl;
+        __syncthreads();
+      }
+      int at = before;
+      for (int w = 0; w < 12; ++w) {
+        if (w < warp) at += scan_sums[w];
+        before += scan_sums[w];
+      }
+      at += incl - c;
+      if (c > 0 && want >= at && want < at + c) {
+        work->found = r * 384 + tid;
+        work->local = want - at;
+      }
+    }
+    __syncthreads();
+  }
+  if (warp == 0) {
+    RaggedWork w;
+    const bool ok = ragged_work_at(p, work->found, work->local * p.block_m, lane, w);
+    if (lane == 0) {
+      const int k_first = w.k_base + split * p.chunk;
+      work->t0 = w.t0;
+      work->nq = w.nq;
+      work->off_m0 = w.off + w.m0;
+      work->len = w.len;
+      work->b = w.b;
+      work->k_lo = w.k_lo;
+      work->k_hi = w.k_hi;
+      work->key0 = k_first;
+      work->nk = (ok && w.k_hi > w.k_lo) ? max(0, (min(k_first + p.chunk, w.k_hi) - k_first + BN - 1) / BN) : 0;
+      work->n_chunks = ok ? w.n_chunks : 0;
+      work->unit = (int)(blockIdx.x / (unsigned)p.nsplit);
+    }
+  }
+  __syncthreads();
+  if (split >= work->n_chunks) return;  // the whole CTA, before TMEM
+  if (warp == 8) {
+    tmem_alloc(smem_u32(tmem_base_ptr), Cfg::kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_base_ptr;
+
+  // Register split as the dense prefill kernel's: 2 x 128 x 208 + 128 x 88 = 384 x 168.
+  static_assert(Cfg::kSoftmaxRegs == 208 && Cfg::kControlRegs == 88, "keep the asm immediates in sync");
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;" ::: "memory");
+    if (warp == 9) {
+      // ============================================================== producer
+      // Lane i brings box i / NSUB, 64 values of d at i % NSUB, of each K or V tile. Boxes
+      // past the last key get a block outside the cache: TMA fills them with zeros.
+      const int nk = work->nk;
+      if (nk > 0) {
+        if (lane == 0) {
+          tma_prefetch_desc(&qmap);
+          tma_prefetch_desc(&kmap);
+          tma_prefetch_desc(&vmap);
+          const int hq0 = kvh * p.group, t0 = work->t0;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            mbar_arrive_expect_tx(bar_q_full + 8 * i, (uint32_t)(bm * p.group) * 128u * NSUB);
+#pragma unroll
+            for (int s = 0; s < NSUB; ++s)
+              tma_load_4d(q_smem0 + i * Cfg::kTileBytes + s * Cfg::kSubBytes, &qmap, bar_q_full + 8 * i, s * 64, hq0,
+                          t0 + i * bm, 0);
+          }
+        }
+        const int box = p.box, nbox = BN / box;
+        const int my_box = lane / NSUB, my_sub = lane % NSUB;
+        const bool loads = my_box < nbox;
+        const int k_hi = work->k_hi, key_first = work->key0 + my_box * box;
+        const int* row_bt = p.block_table + (int64_t)work->b * p.bt_stride;
+        const int mask = (1 << p.block_shift) - 1;
+        const uint32_t dst0 = kv_smem0 + my_sub * Cfg::kSubBytes + (uint32_t)(my_box * box) * 128u;
+        int t = 0;
+        const int n_loads = 2 * nk;
+        int pb = 0;
+        bool ok = true;
+        for (; t < n_loads; ++t) {
+          const int slot = t % SLOTS;
+          const int use = t / SLOTS;
+          const int key = key_first + (t >> 1) * BN;
+          // Looked up once per tile (K loads; V reuses it), before the slot wait.
+          if ((t & 1) == 0) pb = (loads && key < k_hi) ? row_bt[key >> p.block_shift] : p.num_blocks;
+          if (use > 0) {
+            ok = mbar_wait(bar_kv_empty + 8 * slot, (use - 1) & 1, abort_flag, 121);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+          }
+          if (withheld_load(t)) continue;
+          const uint32_t full = bar_kv_full + 8 * slot;
+          if (lane == 0) mbar_arrive_expect_tx(full, Cfg::kTileBytes);
+          __syncwarp();
+          if (loads) tma_load_4d(dst0 + slot * Cfg::kTileBytes, (t & 1) ? &vmap : &kmap, full, my_sub * 64, kvh, key & mask, pb);
+        }
+        if (t < n_loads && lane == 0) {  // aborted: let in-flight loads land before teardown
+          volatile int dummy = 0;
+          for (int u = max(0, t - SLOTS); u < t; ++u)
+            if (!withheld_load(u)) mbar_wait(bar_kv_full + 8 * (u % SLOTS), (u / SLOTS) & 1, &dummy, 122);
+        }
+      }
+      __syncwarp();
+    } else if (warp == 8) {
+      // ============================================================== MMA issuer
+      const int nk = work->nk;
+      if (lane == 0 && nk > 0) {
+        constexpr uint32_t idesc_qk = make_idesc_f16(128, BN, BF16, false);
+        constexpr uint32_t idesc_pv = make_idesc_f16(128, HD, BF16, true);
+        auto issue_qk = [&](int i, int slot) {
+          const uint32_t tS = tmem_base + (i ? Cfg::kColS1 : Cfg::kColS0);
+          const uint32_t qa = q_smem0 + i * Cfg::kTileBytes;
+          const uint32_t kb = kv_smem0 + slot * Cfg::kTileBytes;
+#pragma unroll
+          for (int k = 0; k < HD / 16; ++k) {
+            const uint32_t o = (k >> 2) * Cfg::kSubBytes + (k & 3) * 32;
+            umma_ss(tS, desc_sw128_kmajor(qa + o), desc_sw128_kmajor(kb + o), idesc_qk, k > 0 ? 1u : 0u);
+          }
+        };
+        auto issue_pv = [&](int i, int slot, int h, bool acc) {
+          const uint32_t tS = tmem_base + (i ? Cfg::kColS1 : Cfg::kColS0);
+          const uint32_t tO = tmem_base + (i ? Cfg::kColO1 : Cfg::kColO0);
+          const uint32_t vb = kv_smem0 + slot * Cfg::kTileBytes;
+          constexpr int kPerPart = BN / 16 / Cfg::kPParts;
+#pragma unroll
+          for (int kk = 0; kk < kPerPart; ++kk) {
+            const int k = h * kPerPart + kk;
+            umma_ts(tO, tS + k * 8, desc_sw128_mnmajor(vb + k * 16 * 128, Cfg::kSubBytes), idesc_pv,
+                    (acc || k > 0) ? 1u : 0u);
+          }
+        };
+        bool ok = mbar_wait(bar_q_full, 0, abort_flag, 130) && mbar_wait(bar_q_full + 8, 0, abort_flag, 131) &&
+                  mbar_wait(bar_kv_full, 0, abort_flag, 132);
+        if (ok) {
+          tc_fence_after();
+          issue_qk(0, 0);
+          umma_commit(bar_s_full);
+          issue_qk(1, 0);
+          umma_commit(bar_s_full + 8);
+          umma_commit(bar_kv_empty);  // K_0 consumed
+          for (int j = 0; j < nk; ++j) {
+            const int tv = 2 * j + 1, sv = tv % SLOTS;
+            const int tk = 2 * j + 2, sk = tk % SLOTS;
+            if (!mbar_wait(bar_kv_full + 8 * sv, (tv / SLOTS) & 1, abort_flag, 133)) break;
+            bool pv_ok = true;
+#pragma unroll
+            for (int h = 0; h < Cfg::kPParts && pv_ok; ++h) {
+              pv_ok = mbar_wait(bar_p_full + 8 * h, j & 1, abort_flag, h ? 138 : 134);
+              if (pv_ok) {
+                tc_fence_after();
+                issue_pv(0, sv, h, h > 0 || j > 0);
+              }
+            }
+            if (!pv_ok) break;
+            const bool more = (j + 1 < nk);
+            if (more) {
+              if (!mbar_wait(bar_kv_full + 8 * sk, (tk / SLOTS) & 1, abort_flag, 135)) break;
+              tc_fence_after();
+              issue_qk(0, sk);
+              umma_commit(bar_s_full);
+            } else {
+              umma_commit(bar_o_final);
+            }
+#pragma unroll
+            for (int h = 0; h < Cfg::kPParts && pv_ok; ++h) {
+              pv_ok = mbar_wait(bar_p_full + 8 * (Cfg::kPParts + h), j & 1, abort_flag, h ? 139 : 136);
+              if (pv_ok) {
+                tc_fence_after();
+                issue_pv(1, sv, h, h > 0 || j > 0);
+              }
+            }
+            if (!pv_ok) break;
+            umma_commit(bar_kv_empty + 8 * sv);  // V_j consumed
+            if (more) {
+              issue_qk(1, sk);
+              umma_commit(bar_s_full + 8);
+              umma_commit(bar_kv_empty + 8 * sk);  // K_{j+1} consumed
+            } else {
+              umma_commit(bar_o_final + 8);
+            }
+          }
+        }
+        // Drain: every MMA issued above completes before TMEM is released.
+        umma_commit(bar_mma_done);
+        volatile int dummy = 0;
+        mbar_wait(bar_mma_done, 0, &dummy, 137);
+      }
+      __syncwarp();
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;" ::: "memory");
+    // ================================================================ softmax warpgroups
+    const int wg = warp >> 2;  // query tile handled by this warpgroup
+    const int row = tid & 127;  // packed row == TMEM lane
+    const int wq = warp & 3;    // TMEM lane quarter of this warp
+    const uint32_t lane_off = (uint32_t)(wq * 32) << 16;
+    const uint32_t tS = tmem_base + lane_off + (wg ? Cfg::kColS1 : Cfg::kColS0);
+    const uint32_t tO = tmem_base + lane_off + (wg ? Cfg::kColO1 : Cfg::kColO0);
+    const uint32_t s_full = bar_s_full + 8 * wg;
+    const uint32_t p_full = bar_p_full + 8 * Cfg::kPParts * wg;
+
+    // The row's interval, counted from this CTA's first key; idle rows and rows past the
+    // tile's tokens see nothing.
+    int lo_rel = 0, hi_rel = 0;
+    float dist0 = 0.f, slope = 0.f;
+    {
+      const int m = row / p.group, i = wg * bm + m;
+      if (m < bm && i < work->nq) {
+        RaggedWork w;
+        w.b = work->b;
+        w.len = work->len;
+        w.off = work->off_m0;
+        w.m0 = 0;
+        w.t0 = work->t0;
+        int pos;
+        ragged_row(p, w, i, pos, lo_rel, hi_rel);
+        if constexpr (MOD == kRaggedBias) {
+          slope = p.alibi[kvh * p.group + row % p.group] * 1.4426950408889634f;
+          dist0 = (float)(pos - work->key0);
+        }
+        lo_rel -= work->key0;
+        hi_rel -= work->key0;
+      }
+    }
+    float m_run = -3.0e38f;
+    float l_run = 0.f;
+    bool ok = true;
+    const int nk = work->nk;
+    for (int j = 0; j < nk; ++j) {
+      ok = mbar_wait(s_full, j & 1, abort_flag, 140 + wg);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      tc_fence_after();
+      {
+        // Keys of the tile that no row sees (past the last, or before the first in its
+        // box) have P = 0, but their stale slots may hold NaN or Inf: each thread zeroes
+        // its row of V, once V has landed and before P is published.
+        const int key = work->key0 + j * BN;
+        if (key + BN > work->k_hi || key < work->k_lo) {
+          const int tv = 2 * j + 1;
+          ok = mbar_wait(bar_kv_full + 8 * (tv % SLOTS), (tv / SLOTS) & 1, abort_flag, 144 + wg);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          if (key + row >= work->k_hi || key + row < work->k_lo) {
+            const uint32_t vrow = kv_smem0 + (tv % SLOTS) * Cfg::kTileBytes + row * 128;
+#pragma unroll
+            for (int c = 0; c < NSUB * 8; ++c)
+              asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(vrow + (c >> 3) * Cfg::kSubBytes +
+                                                                          (c & 7) * 16),
+                           "r"(0u)
+                           : "memory");
+          }
+          fence_proxy_async_smem();
+        }
+      }
+      const int rem = hi_rel - j * BN;   // columns [low, rem) are visible
+      const int low = lo_rel - j * BN;
+      const bool masked = rem < BN || low > 0;
+      uint32_t sr[128];
+      tmem_ld32(tS + 0, sr + 0);
+      tmem_ld32(tS + 32, sr + 32);
+      tmem_wait_ld();
+      reg_fence_n<64>(sr);
+      tmem_ld32(tS + 64, sr + 64);
+      tmem_ld32(tS + 96, sr + 96);
+      float mx;
+      if constexpr (MOD == kRaggedBias) {
+        // Scores to log2 units with cap and bias, in place; then the mask and the maximum.
+        tmem_wait_ld();
+        reg_fence_n<64>(sr + 64);
+        const float d0 = dist0 - (float)(j * BN);
+        if (p.cap_in != 0.f) {
+#pragma unroll
+          for (int c = 0; c < 128; ++c)
+            sr[c] = __float_as_uint(fmaf(-2.f * p.cap_out, fast_rcp(1.f + fast_exp2(__uint_as_float(sr[c]) * p.cap_in)),
+                                         fmaf(-slope, fabsf(d0 - (float)c), p.cap_out)));
+        } else {
+#pragma unroll
+          for (int c = 0; c < 128; ++c)
+            sr[c] = __float_as_uint(fmaf(__uint_as_float(sr[c]), p.scale_log2, -slope * fabsf(d0 - (float)c)));
+        }
+      }
+      if (masked) {
+#pragma unroll
+        for (int c = 0; c < 64; ++c) sr[c] = (c < rem && c >= low) ? sr[c] : __float_as_uint(-INFINITY);
+      }
+      // Row max with three-input maxima, four independent chains.
+      float mx0 = __uint_as_float(sr[0]), mx1 = __uint_as_float(sr[1]);
+      float mx2 = __uint_as_float(sr[2]), mx3 = __uint_as_float(sr[3]);
+#pragma unroll
+      for (int c = 4; c < 60; c += 8) {
+        mx0 = max3(mx0, __uint_as_float(sr[c]), __uint_as_float(sr[c + 1]));
+        mx1 = max3(mx1, __uint_as_float(sr[c + 2]), __uint_as_float(sr[c + 3]));
+        mx2 = max3(mx2, __uint_as_float(sr[c + 4]), __uint_as_float(sr[c + 5]));
+        mx3 = max3(mx3, __uint_as_float(sr[c + 6]), __uint_as_float(sr[c + 7]));
+      }
+      mx0 = max3(mx0, __uint_as_float(sr[60]), __uint_as_float(sr[61]));
+      mx1 = max3(mx1, __uint_as_float(sr[62]), __uint_as_float(sr[63]));
+      if constexpr (MOD != kRaggedBias) {
+        asm volatile("tcgen05.wait::ld.sync.aligned;" ::"f"(mx0), "f"(mx1), "f"(mx2), "f"(mx3) : "memory");
+        reg_fence_n<64>(sr + 64);
+      }
+      if (masked) {
+#pragma unroll
+        for (int c = 64; c < 128; ++c) sr[c] = (c < rem && c >= low) ? sr[c] : __float_as_uint(-INFINITY);
+      }
+#pragma unroll
+      for (int c = 64; c < 128; c += 8) {
+        mx0 = max3(mx0, __uint_as_float(sr[c]), __uint_as_float(sr[c + 1]));
+        mx1 = max3(mx1, __uint_as_float(sr[c + 2]), __uint_as_float(sr[c + 3]));
+        mx2 = max3(mx2, __uint_as_float(sr[c + 4]), __uint_as_float(sr[c + 5]));
+        mx3 = max3(mx3, __uint_as_float(sr[c + 6]), __uint_as_float(sr[c + 7]));
+      }
+      mx = fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3));
+      if constexpr (MOD == kRaggedPlain) mx *= p.scale_log2;
+      if constexpr (MOD == kRaggedCap)
+        mx = mx == -INFINITY ? mx : fmaf(-2.f * p.cap_out, fast_rcp(1.f + fast_exp2(mx * p.cap_in)), p.cap_out);
+      const float m_new = fmaxf(m_run, mx);
+      const bool need = m_new > m_run + 8.0f;
+      if (j > 0 && __any_sync(0xffffffffu, need)) {
+        const float alpha = need ? fast_exp2(m_run - m_new) : 1.0f;
+#pragma unroll
+        for (int c = 0; c < HD / 32; ++c) {
+          uint32_t orr[32];
+          tmem_ld32(tO + c * 32, orr);
+          tmem_wait_ld();
+          reg_fence(orr);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) orr[e] = __float_as_uint(__uint_as_float(orr[e]) * alpha);
+          tmem_st32(tO + c * 32, orr);
+        }
+        tmem_wait_st();
+      }
+      if (need) {
+        l_run *= fast_exp2(m_run - m_new);
+        m_run = m_new;
+      }
+      // P = exp2(x - m), written over S as packed 16-bit pairs in kPParts column parts.
+      const float sc = MOD == kRaggedPlain ? p.scale_log2 : 1.0f;
+      float2 sum2[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+      constexpr int kPairs = 64 / Cfg::kPParts;
+      auto publish = [&](auto shifted) {  // shifted(pair) = x - m of two neighbouring scores
+#pragma unroll
+        for (int h = 0; h < Cfg::kPParts; ++h) {
+          uint32_t pk[kPairs];
+#pragma unroll
+          for (int c = 0; c < kPairs; ++c) {
+            const int col = 2 * kPairs * h + 2 * c;
+            const float2 x = shifted(make_float2(__uint_as_float(sr[col]), __uint_as_float(sr[col + 1])));
+            const float2 pv = make_float2(fast_exp2(x.x), fast_exp2(x.y));
+            sum2[c & 3] = add2(sum2[c & 3], pv);
+            pk[c] = pack2<BF16>(pv.x, pv.y);
+          }
+          tmem_st32(tS + kPairs * h, pk);
+          tmem_wait_st();
+          tc_fence_before();
+          mbar_arrive(p_full + 8 * h);
+        }
+      };
+      static_assert(kPairs == 32, "one 32-column store per part");
+      const float2 nm2 = make_float2(-m_run, -m_run);
+      if constexpr (MOD == kRaggedCap) {
+        const float cin = p.cap_in, cout2 = -2.f * p.cap_out, off = p.cap_out - m_run;
+        publish([&](float2 s) {
+          return make_float2(s.x == -INFINITY ? s.x : fmaf(cout2, fast_rcp(1.f + fast_exp2(s.x * cin)), off),
+                             s.y == -INFINITY ? s.y : fmaf(cout2, fast_rcp(1.f + fast_exp2(s.y * cin)), off));
+        });
+      } else {
+        const float2 sc2 = make_float2(sc, sc);
+        publish([&](float2 s) { return fma2(s, sc2, nm2); });
+      }
+      const float2 s01 = add2(sum2[0], sum2[1]);
+      const float2 s23 = add2(sum2[2], sum2[3]);
+      const float2 st = add2(s01, s23);
+      l_run += st.x + st.y;
+    }
+
+    // ---- epilogue
+    bool have_o = ok && nk > 0;
+    if (have_o) {
+      have_o = mbar_wait(bar_o_final + 8 * wg, 0, abort_flag, 142 + wg);
+      have_o = __all_sync(0xffffffffu, have_o);
+    }
+    if (have_o) tc_fence_after();
+
+    const int n_chunks = work->n_chunks, unit = work->unit;
+    float L = l_run, M = m_run;
+    bool store = true;
+    const int prow = wg * 128 + row;  // row of the pair's 256 packed rows
+    const int64_t pbase = (int64_t)unit * p.nsplit * 256 + prow;
+    if (n_chunks > 1) {
+      // Publish this chunk's partial, m, l [split][256 rows] and acc [split][d][256 rows];
+      // the tile's last CTA (ticket) folds them in chunk order.
+      __stcg(p.ws_m + pbase + (int64_t)split * 256, m_run);
+      __stcg(p.ws_l + pbase + (int64_t)split * 256, l_run);
+      float* acc_own = p.ws_acc + ((int64_t)unit * p.nsplit + split) * HD * 256 + prow;
+#pragma unroll
+      for (int c = 0; c < HD / 32; ++c) {
+        uint32_t orr[32];
+        if (have_o) {
+          tmem_ld32(tO + c * 32, orr);
+          tmem_wait_ld();
+          reg_fence(orr);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) orr[e] = ok ? 0u : 0x7fc00000u;
+        }
+#pragma unroll
+        for (int e = 0; e < 32; ++e) __stcg(acc_own + (c * 32 + e) * 256, __uint_as_float(orr[e]));
+      }
+      asm volatile("bar.sync 3, 256;" ::: "memory");
+      uint32_t* last_slot = tmem_base_ptr + 2;
+      if (tid == 0) {
+        unsigned ticket;
+        asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(ticket) : "l"(p.ws_cnt + unit) : "memory");
+        const bool last = ticket == (unsigned)(n_chunks - 1);
+        *last_slot = last ? 1u : 0u;
+        if (last) p.ws_cnt[unit] = 0u;
+      }
+      asm volatile("bar.sync 3, 256;" ::: "memory");
+      store = *last_slot != 0;
+      if (store) {
+        for (int s0 = 0; s0 < n_chunks; s0 += 4) {
+          float mv[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) mv[i] = __ldcg(p.ws_m + pbase + (int64_t)min(s0 + i, n_chunks - 1) * 256);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) M = fmaxf(M, mv[i]);
+        }
+        L = 0.f;
+        for (int s0 = 0; s0 < n_chunks; s0 += 4) {
+          float mv[4], lv[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int64_t o2 = pbase + (int64_t)min(s0 + i, n_chunks - 1) * 256;
+            mv[i] = __ldcg(p.ws_m + o2);
+            lv[i] = __ldcg(p.ws_l + o2);
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (s0 + i < n_chunks) L += fast_exp2(mv[i] - M) * lv[i];
+        }
+      }
+    }
+    const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);  // no key seen: 0; a NaN sum stays NaN
+    const uint32_t stage = q_smem0 + wg * Cfg::kTileBytes;
+#pragma unroll
+    for (int c = 0; c < HD / 32; ++c) {
+      uint32_t orr[32];
+      if (n_chunks > 1) {
+        // Two chunks per pass: 64 independent loads in flight per thread. An index past
+        // the last chunk reads a valid partial at weight 0.
+#pragma unroll
+        for (int e = 0; e < 32; ++e) orr[e] = 0u;
+        for (int s0 = 0; store && s0 < n_chunks; s0 += 2) {
+          const int sa = s0, sb = min(s0 + 1, n_chunks - 1);
+          const float wa = fast_exp2(__ldcg(p.ws_m + pbase + (int64_t)sa * 256) - M);
+          const float wb = (s0 + 1 >= n_chunks) ? 0.f : fast_exp2(__ldcg(p.ws_m + pbase + (int64_t)sb * 256) - M);
+          const float* xa = p.ws_acc + ((int64_t)unit * p.nsplit + sa) * HD * 256 + prow + c * 32 * 256;
+          const float* xb = p.ws_acc + ((int64_t)unit * p.nsplit + sb) * HD * 256 + prow + c * 32 * 256;
+          float va[32], vb[32];
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            va[e] = __ldcg(xa + e * 256);
+            vb[e] = __ldcg(xb + e * 256);
+          }
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            orr[e] = __float_as_uint(fmaf(wb, vb[e], fmaf(wa, va[e], __uint_as_float(orr[e]))));
+        }
+      } else if (have_o) {
+        tmem_ld32(tO + c * 32, orr);
+        tmem_wait_ld();
+        reg_fence(orr);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 32; ++e) orr[e] = ok ? 0u : 0x7fc00000u;
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int chunk = 4 * c + e;  // 16-byte chunk along d
+#define GQA_OV(i) (__uint_as_float(orr[8 * e + (i)]) * inv)
+        const uint32_t w0 = pack2<BF16>(GQA_OV(0), GQA_OV(1));
+        const uint32_t w1 = pack2<BF16>(GQA_OV(2), GQA_OV(3));
+        const uint32_t w2 = pack2<BF16>(GQA_OV(4), GQA_OV(5));
+        const uint32_t w3 = pack2<BF16>(GQA_OV(6), GQA_OV(7));
+#undef GQA_OV
+        const uint32_t dst = stage + (chunk >> 3) * Cfg::kSubBytes + sw128_off(row, chunk & 7);
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(w0), "r"(w1), "r"(w2), "r"(w3)
+                     : "memory");
+      }
+    }
+    if (wg == 0)
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+    else
+      asm volatile("bar.sync 2, 128;" ::: "memory");
+    if (store) {
+      const int rows = max(0, min(work->nq - wg * bm, bm)) * p.group;  // rows of real tokens
+      const int tok0 = work->t0 + wg * bm;
+      if (p.lse && row < rows)
+        p.lse[(int64_t)(tok0 + row / p.group) * p.hq + kvh * p.group + row % p.group] =
+            L == 0.f ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
+      // 16 bytes per thread, a row's pieces on neighbouring threads.
+      constexpr int kPer = HD / 8;
+      for (int idx = row; idx < rows * kPer; idx += 128) {
+        const int r = idx / kPer, chunk = idx % kPer;
+        uint32_t w0, w1, w2, w3;
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(w0), "=r"(w1), "=r"(w2), "=r"(w3)
+                     : "r"(stage + (chunk >> 3) * Cfg::kSubBytes + sw128_off(r, chunk & 7))
+                     : "memory");
+        const int tok = tok0 + r / p.group, head = kvh * p.group + r % p.group;
+        *reinterpret_cast<uint4*>(p.o + (int64_t)tok * p.o_st + (int64_t)head * p.o_sh + chunk * 8) =
+            make_uint4(w0, w1, w2, w3);
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 8) tmem_dealloc(tmem_base, Cfg::kTmemCols);
+}
+
+}  // namespace gqa

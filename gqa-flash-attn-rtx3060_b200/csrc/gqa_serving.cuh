@@ -39,6 +39,33 @@ cudaError_t prepare_ragged() {
   return e;
 }
 
+template <int HD, bool BF>
+cudaError_t launch_ragged_tile_hd(const RaggedParams& p, unsigned grid, const CUtensorMap& qm, const CUtensorMap& km,
+                                  const CUtensorMap& vm, cudaStream_t st) {
+  using Cfg = RaggedTileCfg<HD>;
+  if (p.alibi)
+    return launch_pdl(gqa_ragged_tile_kernel<HD, BF, kRaggedBias>, grid, Cfg::kThreads, Cfg::kSmemBytes, st, p, qm, km, vm);
+  if (p.cap_in != 0.f)
+    return launch_pdl(gqa_ragged_tile_kernel<HD, BF, kRaggedCap>, grid, Cfg::kThreads, Cfg::kSmemBytes, st, p, qm, km, vm);
+  return launch_pdl(gqa_ragged_tile_kernel<HD, BF, kRaggedPlain>, grid, Cfg::kThreads, Cfg::kSmemBytes, st, p, qm, km, vm);
+}
+
+// Shared memory opt-in, and the setmaxnreg split must fit the registers the launch holds.
+int prepare_ragged_tile() {
+  int rc = GQA_OK;
+  auto prep = [&](auto kernel, int smem) {
+    if (set_smem(kernel, smem) != cudaSuccess) rc = rc ? rc : GQA_ERR_CUDA;
+    if (!rc) rc = check_reg_split(kernel, PrefillCfg<128>::kThreads, PrefillCfg<128>::kRegsNeeded);
+  };
+#define GQA_PREP_RAGGED(HD, BF)                                                           \
+  prep(gqa_ragged_tile_kernel<HD, BF, kRaggedPlain>, RaggedTileCfg<HD>::kSmemBytes);      \
+  prep(gqa_ragged_tile_kernel<HD, BF, kRaggedCap>, RaggedTileCfg<HD>::kSmemBytes);        \
+  prep(gqa_ragged_tile_kernel<HD, BF, kRaggedBias>, RaggedTileCfg<HD>::kSmemBytes)
+  GQA_PREP_RAGGED(128, true); GQA_PREP_RAGGED(128, false); GQA_PREP_RAGGED(64, true); GQA_PREP_RAGGED(64, false);
+#undef GQA_PREP_RAGGED
+  return rc;
+}
+
 struct RaggedShape {
   int n, tokens, hq, hkv, group, max_q, max_len, head_dim, window, causal, prefix;
 };
@@ -73,7 +100,7 @@ RaggedPlan plan_ragged_stream(const RaggedShape& s, int sm_count) {
   const int stages = std::max(1, (span + 127) / 128);
   pl.nsplit = 1;
   pl.chunk = stages * 128;
-  if ((int64_t)pl.slots * s.hkv > kServingCounters) return pl;
+  if ((int64_t)pl.slots * s.hkv > kServingCounters / 2) return pl;
   constexpr double kFixedStages = 2.5;  // a CTA's fixed cost, in 128-key stages (plan_stream's, in 64-key ones, is 5)
   double best = 1e300;
   for (int ns = 1; ns <= std::min(stages, kMaxSplits); ++ns) {
@@ -90,22 +117,70 @@ RaggedPlan plan_ragged_stream(const RaggedShape& s, int sm_count) {
   return pl;
 }
 
-size_t ragged_ws_bytes(const RaggedPlan& pl, const RaggedShape& s) {
-  if (pl.nsplit <= 1) return 0;
-  const size_t n = (size_t)pl.slots * s.hkv * pl.nsplit * pl.rows;
-  return (size_t)kServingCounters * 4 + 2 * align256(n * 4) + align256(n * s.head_dim * 4);
+// Tiles of the tcgen05 kernel (pairs of 128-row query tiles) and its key split. At most
+// tokens / block_m + (requests of more than kStreamMaxRows rows) tiles; when they are
+// fewer than the SMs the keys are split, at least two 128-key tiles per chunk.
+RaggedPlan plan_ragged_tile(const RaggedShape& s, int sm_count) {
+  RaggedPlan pl{};
+  pl.block_m = 2 * (128 / s.group);
+  pl.rows = 256;
+  const int64_t longest = std::min<int64_t>(s.n, (int64_t)s.tokens * s.group / (kStreamMaxRows + 1));
+  pl.slots = (int)std::min<int64_t>((int64_t)s.tokens / pl.block_m + longest, INT_MAX);
+  const int64_t units = (int64_t)pl.slots * s.hkv;
+  int span = s.max_len;
+  if (s.window > 0 && s.causal && !s.prefix)
+    span = (int)std::min<int64_t>(span, (int64_t)s.window + pl.block_m - 1 + 64);
+  const int nk = std::max(1, (span + 127) / 128);
+  pl.nsplit = 1;
+  if (units > 0 && units < sm_count && units <= kServingCounters / 2) {
+    int ns = (int)std::min<int64_t>(sm_count / units, 16);
+    while (ns > 1 && nk < 2 * ns) --ns;
+    pl.nsplit = ns;
+  }
+  pl.chunk = (nk + pl.nsplit - 1) / pl.nsplit * 128;
+  return pl;
 }
 
-void ragged_ws_carve(const RaggedPlan& pl, const RaggedShape& s, void* ws, RaggedParams* p) {
+// The streaming kernel takes the requests of up to kStreamMaxRows packed rows, the
+// tcgen05 kernel the rest; e4m3 caches are the streaming kernel's alone.
+bool ragged_uses_tile(const RaggedShape& s, bool fp8) { return !fp8 && (int64_t)s.max_q * s.group > kStreamMaxRows; }
+
+RaggedShape stream_part(const RaggedShape& s, bool tile) {
+  RaggedShape r = s;
+  if (tile) r.max_q = kStreamMaxRows / s.group;
+  return r;
+}
+
+size_t ragged_partial_bytes(const RaggedPlan& pl, const RaggedShape& s) {
+  if (pl.nsplit <= 1) return 0;
   const size_t n = (size_t)pl.slots * s.hkv * pl.nsplit * pl.rows;
-  uint8_t* c = reinterpret_cast<uint8_t*>(ws);
-  p->ws_cnt = reinterpret_cast<unsigned*>(c);
-  c += (size_t)kServingCounters * 4;
+  return 2 * align256(n * 4) + align256(n * s.head_dim * 4);
+}
+
+// Counters first (half for each kernel), then the streaming kernel's partials, then the
+// tcgen05 kernel's.
+size_t ragged_ws_bytes(const RaggedPlan& stream, const RaggedPlan* tile, const RaggedShape& s) {
+  const size_t n = ragged_partial_bytes(stream, s) + (tile ? ragged_partial_bytes(*tile, s) : 0);
+  return n ? (size_t)kServingCounters * 4 + n : 0;
+}
+
+void ragged_ws_carve(const RaggedPlan& pl, const RaggedShape& s, uint8_t* counters, uint8_t* c, RaggedParams* p) {
+  const size_t n = (size_t)pl.slots * s.hkv * pl.nsplit * pl.rows;
+  p->ws_cnt = reinterpret_cast<unsigned*>(counters);
   p->ws_m = reinterpret_cast<float*>(c);
   c += align256(n * 4);
   p->ws_l = reinterpret_cast<float*>(c);
   c += align256(n * 4);
   p->ws_acc = reinterpret_cast<float*>(c);
+}
+
+void set_plan(RaggedParams& p, const RaggedPlan& pl) {
+  p.block_m = pl.block_m;
+  p.rows = pl.rows;
+  p.one_tile = pl.one_tile;
+  p.slots = pl.slots;
+  p.nsplit = pl.nsplit;
+  p.chunk = pl.chunk;
 }
 
 // 4-D map (d, kv head, position in block, block) of a paged cache with element strides
@@ -255,13 +330,15 @@ int gqa_qk_norm_rope(const void* q, const void* k, const void* v, const int64_t*
 }
 
 size_t gqa_ragged_fwd_workspace_bytes(int num_seqs, int num_tokens, int num_heads, int num_kv_heads, int max_query_len,
-                                      int max_seq_len, int head_dim, int window) {
+                                      int max_seq_len, int head_dim, int window, int cache_fp8) {
   RaggedShape s;
   int sm = 0;
   if (check_ragged_shape(num_seqs, num_tokens, num_heads, num_kv_heads, max_query_len, max_seq_len, head_dim, window, &s) ||
       num_seqs == 0 || num_tokens == 0 || max_query_len == 0 || current_device(&sm))
     return 0;
-  return ragged_ws_bytes(plan_ragged_stream(s, sm), s);
+  const bool tile = ragged_uses_tile(s, cache_fp8 != 0);
+  const RaggedPlan tp = plan_ragged_tile(s, sm);
+  return ragged_ws_bytes(plan_ragged_stream(stream_part(s, tile), sm), tile ? &tp : nullptr, s);
 }
 
 int gqa_ragged_fwd(const void* q, const void* k_cache, const void* v_cache, void* o, float* lse,
@@ -328,32 +405,53 @@ int gqa_ragged_fwd(const void* q, const void* k_cache, const void* v_cache, void
   p.v_scale = cache_fp8 ? v_scale : 1.f;
   p.mods = softcap > 0.f || alibi_slopes;
 
-  RaggedPlan pl = plan_ragged_stream(s, sm);
-  if (pl.nsplit > 1) {
-    if (workspace && aligned16(workspace) && workspace_bytes >= ragged_ws_bytes(pl, s)) {
-      ragged_ws_carve(pl, s, workspace, &p);
-    } else {  // no room for the partials: one CTA per tile
-      pl.nsplit = 1;
-      pl.chunk = std::max(1, (max_seq_len + 127) / 128) * 128;
-    }
+  const bool tile = ragged_uses_tile(s, cache_fp8 != 0);
+  const RaggedShape ss = stream_part(s, tile);
+  RaggedPlan sp = plan_ragged_stream(ss, sm), tp = plan_ragged_tile(s, sm);
+  const bool have_ws = workspace && aligned16(workspace) && workspace_bytes >= ragged_ws_bytes(sp, tile ? &tp : nullptr, s);
+  if (!have_ws) {  // no room for the partials: one CTA per tile
+    sp.nsplit = tp.nsplit = 1;
+    sp.chunk = tp.chunk = std::max(1, (max_seq_len + 127) / 128) * 128;
   }
-  p.block_m = pl.block_m;
-  p.rows = pl.rows;
-  p.one_tile = pl.one_tile;
-  p.slots = pl.slots;
-  p.min_rows = 0;
-  p.max_rows = INT_MAX;
-  p.nsplit = pl.nsplit;
-  p.chunk = pl.chunk;
+  uint8_t* const counters = reinterpret_cast<uint8_t*>(workspace);
+  uint8_t* const partials = counters + (size_t)kServingCounters * 4;
   CUtensorMap km, vm;
   rc = make_cache_map(&km, k_cache, k_strides4, num_blocks, block_size, num_kv_heads, head_dim, p.box, cache_fp8);
   if (!rc) rc = make_cache_map(&vm, v_cache, v_strides4, num_blocks, block_size, num_kv_heads, head_dim, p.box, cache_fp8);
   if (rc) return rc;
-  const int64_t grid = (int64_t)pl.slots * num_kv_heads * pl.nsplit;
-  if (grid > INT_MAX) return GQA_ERR_INVALID_ARG;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const bool bf = dtype == GQA_DTYPE_BF16;
-  cudaError_t e;
+  cudaError_t e = cudaSuccess;
+
+  if (tile) {
+    RaggedParams t = p;
+    set_plan(t, tp);
+    t.min_rows = kStreamMaxRows + 1;
+    t.max_rows = INT_MAX;
+    if (tp.nsplit > 1)
+      ragged_ws_carve(tp, s, counters + (size_t)kServingCounters * 2, partials + ragged_partial_bytes(sp, s), &t);
+    // Queries (d, head, token): a tile is bm tokens of the group's heads, token-major rows.
+    const int64_t bhsd[4] = {q_strides3[0] * num_tokens, q_strides3[0], q_strides3[1], 1};
+    CUtensorMap qm;
+    rc = make_map(&qm, q, bhsd, 1, num_tokens, num_heads, head_dim, s.group, tp.block_m / 2);
+    if (rc) return rc;
+    const int64_t grid = (int64_t)tp.slots * num_kv_heads * tp.nsplit;
+    if (grid > INT_MAX) return GQA_ERR_INVALID_ARG;
+    if (head_dim == 128)
+      e = bf ? launch_ragged_tile_hd<128, true>(t, (unsigned)grid, qm, km, vm, st)
+             : launch_ragged_tile_hd<128, false>(t, (unsigned)grid, qm, km, vm, st);
+    else
+      e = bf ? launch_ragged_tile_hd<64, true>(t, (unsigned)grid, qm, km, vm, st)
+             : launch_ragged_tile_hd<64, false>(t, (unsigned)grid, qm, km, vm, st);
+    if (e != cudaSuccess) return GQA_ERR_CUDA;
+  }
+
+  set_plan(p, sp);
+  p.min_rows = 0;
+  p.max_rows = tile ? kStreamMaxRows : INT_MAX;
+  if (sp.nsplit > 1) ragged_ws_carve(sp, s, counters, partials, &p);
+  const int64_t grid = (int64_t)sp.slots * num_kv_heads * sp.nsplit;
+  if (grid > INT_MAX) return GQA_ERR_INVALID_ARG;
   if (cache_fp8)
     e = bf ? launch_ragged_stream_hd<128, true, true>(p, (unsigned)grid, km, vm, st)
            : launch_ragged_stream_hd<128, false, true>(p, (unsigned)grid, km, vm, st);

@@ -15,6 +15,7 @@
 #include "gqa_combine.cuh"
 #include "gqa_prefill.cuh"
 #include "gqa_ragged.cuh"
+#include "gqa_ragged_tile.cuh"
 #include "gqa_rope.cuh"
 #include "gqa_step.cuh"
 #include "gqa_stream.cuh"
@@ -55,6 +56,7 @@ cudaError_t set_smem(K kernel, int bytes) {
 }
 
 cudaError_t prepare_ragged();  // gqa_serving.cuh
+int prepare_ragged_tile();
 
 int init_device(int dev) {
   cudaDeviceProp prop;
@@ -114,7 +116,7 @@ int init_device(int dev) {
   chk(set_smem(gqa_stream_kernel<64, false, 1, false, true>, StreamCfg<64>::kSmemBytes));
   chk(prepare_ragged());
   if (e != cudaSuccess) return GQA_ERR_CUDA;
-  return GQA_OK;
+  return prepare_ragged_tile();
 }
 
 // Returns GQA_OK and the SM count of the current device, initialising it once.

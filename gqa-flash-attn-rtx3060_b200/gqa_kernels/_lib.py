@@ -79,7 +79,7 @@ SIGNATURES.update({
     "gqa_step_plan": (_I, [_P, _P, _P, _I64, _P, _P, _I, _P, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P, _P]),
     "gqa_qk_norm_rope": (_I, [_P, _P, _P, _I64P, _I64P, _I64P, _P, _P, _P, _I64, _I, _P, _P, _I, _I, _I, _P, _P, _P, _P,
                               _I, _I, _I, _I, _I, _I, _I, _I, _F, _F, _F, _P]),
-    "gqa_ragged_fwd_workspace_bytes": (_SZ, [_I, _I, _I, _I, _I, _I, _I, _I]),
+    "gqa_ragged_fwd_workspace_bytes": (_SZ, [_I, _I, _I, _I, _I, _I, _I, _I, _I]),
     "gqa_ragged_fwd": (_I, [_P, _P, _P, _P, _P, _I64P, _I64P, _I64P, _I64P, _P, _I, _P, _P, _P, _P, _P,
                             _I, _I, _I, _I, _I, _I, _I, _I, _I, _F, _F, _I, _I, _I, _I, _F, _F, _P, _SZ, _P]),
     "gqa_verify_workspace_bytes": (_SZ, [_I, _I, _I, _I]),

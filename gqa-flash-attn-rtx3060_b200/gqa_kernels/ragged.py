@@ -124,7 +124,7 @@ def paged_ragged_attention(query, key_cache, value_cache, block_tables, cu_query
     with _lib.on_device(dev):
         nbytes = _lib.workspace_bytes("gqa_ragged_fwd_workspace_bytes", num_seqs, num_tokens, num_heads, num_kv_heads,
                                       max_query_len, max_seq_len, head_dim,
-                                      0 if window is None or prefix_lens is not None else window)
+                                      0 if window is None or prefix_lens is not None else window, 1 if fp8 else 0)
         ws = _lib.SERVING_WORKSPACES.get(dev, nbytes, None).data_ptr() if nbytes else None
         rc = _lib.load().gqa_ragged_fwd(
             query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), out.data_ptr(), _ptr(lse),

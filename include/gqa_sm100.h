@@ -384,7 +384,7 @@ int gqa_qk_norm_rope(const void* q, const void* k, const void* v, const int64_t*
  * the key axis is not split.
  */
 size_t gqa_ragged_fwd_workspace_bytes(int num_seqs, int num_tokens, int num_heads, int num_kv_heads, int max_query_len,
-                                      int max_seq_len, int head_dim, int window);
+                                      int max_seq_len, int head_dim, int window, int cache_fp8);
 int gqa_ragged_fwd(const void* q, const void* k_cache, const void* v_cache, void* o, float* lse,
                    const int64_t* q_strides3, const int64_t* k_strides4, const int64_t* v_strides4,
                    const int64_t* o_strides3, const int* block_table, int bt_stride, const int* cu_query_lens,
