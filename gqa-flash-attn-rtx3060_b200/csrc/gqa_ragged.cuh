@@ -51,6 +51,8 @@ struct RaggedParams {
   int max_len;            // bound of seq_lens (longer ones are clipped to it)
   float scale_log2;       // scale * log2 e
   float cap_in, cap_out;  // 2 log2 e * scale / cap, cap * log2 e; cap_in 0: no cap
+  float cap_a[4];         // the cap as s (a0 + a1 s^2 + a2 s^4 + a3 s^6), for |s| <= cap_most
+  float cap_most;
   float v_scale;          // e4m3 values
   int mods;               // cap or bias present
   // Tiles: block_m tokens of one request, rows = block_m * group packed rows. With

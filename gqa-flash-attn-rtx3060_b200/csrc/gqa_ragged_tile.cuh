@@ -22,7 +22,14 @@
 // step can have; CTAs past the real number return before they touch TMEM.
 //
 // Bound by the tensor core and the softmax's exponentials together (gqa_prefill.cuh has
-// the accounting). The cap costs two more MUFU operations per score, exp2 and a reciprocal.
+// the accounting). The cap would cost two more MUFU operations per score (exp2 and a
+// reciprocal), three times the exponential's alone. So while every score of a warp's rows
+// in the tile has |y| <= 0.6, y = s scale / cap,
+//   cap log2 e tanh(y) = s (a0 + a1 s^2 + a2 s^4 + a3 s^6),
+// an odd polynomial fitted to tanh (tests/tanh_fit.py, absolute error 6.5e-7 of the cap)
+// whose last product merges with the subtraction of the maximum: four more operations per
+// score on the FMA pipe, which the exponentials leave half idle. Tiles with larger
+// scores, rare in models that cap them, and tiles that a mask cuts take the MUFU form.
 #pragma once
 
 #include "gqa_prefill.cuh"
@@ -33,6 +40,29 @@ namespace gqa {
 // Score transforms of an instantiation: kRaggedPlain none; kRaggedCap the cap alone
 // (monotone, so the row maximum is taken before it); kRaggedBias a distance bias, capped or not.
 enum : int { kRaggedPlain = 0, kRaggedCap = 1, kRaggedBias = 2 };
+
+// tanh(y) ~ y (c0 + c1 y^2 + c2 y^4 + c3 y^6), |y| <= kTanhRange.
+constexpr float kTanhRange = 0.6f;
+constexpr float kTanhC0 = 0.9999909996986389f, kTanhC1 = -0.33298975229263306f;
+constexpr float kTanhC2 = 0.12974554300308228f, kTanhC3 = -0.039611268788576126f;
+
+// The polynomial's coefficients for raw scores s (host side).
+inline void set_cap_polynomial(RaggedParams& p, double scale_over_cap, double cap_log2e) {
+  const double c[4] = {kTanhC0, kTanhC1, kTanhC2, kTanhC3};
+  double k = scale_over_cap;
+  for (int i = 0; i < 4; ++i) {
+    p.cap_a[i] = (float)(cap_log2e * c[i] * k);
+    k *= scale_over_cap * scale_over_cap;
+  }
+  p.cap_most = (float)(kTanhRange / scale_over_cap);
+}
+
+// Three-input maximum of magnitudes.
+__device__ __forceinline__ float max3_abs(float a, float b, float c) {
+  float d;
+  asm("max.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
 
 template <int HD>
 struct RaggedTileCfg : PrefillCfg<HD> {
@@ -509,11 +539,29 @@ __global__ void __launch_bounds__(384, 1)
       static_assert(kPairs == 32, "one 32-column store per part");
       const float2 nm2 = make_float2(-m_run, -m_run);
       if constexpr (MOD == kRaggedCap) {
+        float big = 0.f, big1 = 0.f;
+        const bool any_masked = __any_sync(0xffffffffu, masked);
+        if (!any_masked) {
+#pragma unroll
+          for (int c = 0; c < 128; c += 4) {
+            big = max3_abs(big, __uint_as_float(sr[c]), __uint_as_float(sr[c + 1]));
+            big1 = max3_abs(big1, __uint_as_float(sr[c + 2]), __uint_as_float(sr[c + 3]));
+          }
+        }
+        if (!any_masked && __all_sync(0xffffffffu, fmaxf(big, big1) <= p.cap_most)) {
+          const float2 a0 = make_float2(p.cap_a[0], p.cap_a[0]), a1 = make_float2(p.cap_a[1], p.cap_a[1]);
+          const float2 a2 = make_float2(p.cap_a[2], p.cap_a[2]), a3 = make_float2(p.cap_a[3], p.cap_a[3]);
+          publish([&](float2 s) {
+            const float2 z = make_float2(s.x * s.x, s.y * s.y);
+            return fma2(s, fma2(fma2(fma2(a3, z, a2), z, a1), z, a0), nm2);
+          });
+        } else {
         const float cin = p.cap_in, cout2 = -2.f * p.cap_out, off = p.cap_out - m_run;
         publish([&](float2 s) {
           return make_float2(s.x == -INFINITY ? s.x : fmaf(cout2, fast_rcp(1.f + fast_exp2(s.x * cin)), off),
                              s.y == -INFINITY ? s.y : fmaf(cout2, fast_rcp(1.f + fast_exp2(s.y * cin)), off));
         });
+        }
       } else {
         const float2 sc2 = make_float2(sc, sc);
         publish([&](float2 s) { return fma2(s, sc2, nm2); });

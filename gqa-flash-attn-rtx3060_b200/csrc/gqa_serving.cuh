@@ -402,6 +402,7 @@ int gqa_ragged_fwd(const void* q, const void* k_cache, const void* v_cache, void
   p.scale_log2 = (float)(sc * kLog2e);
   p.cap_in = softcap > 0.f ? (float)(2.0 * kLog2e * sc / softcap) : 0.f;
   p.cap_out = softcap > 0.f ? (float)(softcap * kLog2e) : 0.f;
+  if (softcap > 0.f) set_cap_polynomial(p, sc / softcap, softcap * kLog2e);
   p.v_scale = cache_fp8 ? v_scale : 1.f;
   p.mods = softcap > 0.f || alibi_slopes;
 
