@@ -70,13 +70,16 @@ struct RaggedShape {
   int n, tokens, hq, hkv, group, max_q, max_len, head_dim, window, causal, prefix;
 };
 
-int check_ragged_shape(int n, int tokens, int hq, int hkv, int max_q, int max_len, int head_dim, int window,
-                       RaggedShape* s) {
-  if (n < 0 || tokens < 0 || hq <= 0 || hkv <= 0 || max_q < 0 || max_len < 0 || window < 0) return GQA_ERR_INVALID_ARG;
-  if (hq % hkv != 0) return GQA_ERR_INVALID_ARG;
-  if (head_dim != 64 && head_dim != 128) return GQA_ERR_UNSUPPORTED;
-  if (hq / hkv > kStreamMaxRows) return GQA_ERR_UNSUPPORTED;
-  *s = RaggedShape{n, tokens, hq, hkv, hq / hkv, std::min(max_q, tokens), max_len, head_dim, window, 1, 0};
+int check_ragged_shape(const gqa_ragged_args& a, RaggedShape* s) {
+  if (a.num_seqs < 0 || a.num_tokens < 0 || a.num_heads <= 0 || a.num_kv_heads <= 0 || a.max_query_len < 0 ||
+      a.max_seq_len < 0 || a.window < 0)
+    return GQA_ERR_INVALID_ARG;
+  if (a.num_heads % a.num_kv_heads != 0) return GQA_ERR_INVALID_ARG;
+  if (a.head_dim != 64 && a.head_dim != 128) return GQA_ERR_UNSUPPORTED;
+  if (a.num_heads / a.num_kv_heads > kStreamMaxRows) return GQA_ERR_UNSUPPORTED;
+  *s = RaggedShape{a.num_seqs, a.num_tokens, a.num_heads, a.num_kv_heads, a.num_heads / a.num_kv_heads,
+                   std::min(a.max_query_len, a.num_tokens), a.max_seq_len, a.head_dim, a.window, a.causal ? 1 : 0,
+                   a.prefix_lens != nullptr};
   return GQA_OK;
 }
 
@@ -212,216 +215,203 @@ using namespace gqa;
 
 extern "C" {
 
-int gqa_step_plan(const int* query_lens, const int* context_lens, int* block_tables, int64_t bt_stride,
-                  const int* blocks_held, const int* free_blocks, int num_free, const int* free_count, int num_seqs,
-                  int max_blocks, int block_size, int max_tokens, int* cu_query_lens, int* seq_lens, int* positions,
-                  int64_t* slot_mapping, int* token_seqs, unsigned char* granted, int* blocks_held_out,
-                  int* free_count_out, void* stream) {
-  if (num_seqs < 0 || max_blocks < 0 || max_tokens < 0 || num_free < 0 || bt_stride < max_blocks) return GQA_ERR_INVALID_ARG;
-  if (block_size < 1 || (block_size & (block_size - 1)) != 0) return GQA_ERR_UNSUPPORTED;
-  if (!cu_query_lens || !free_count || !free_count_out || free_count == free_count_out) return GQA_ERR_INVALID_ARG;
-  if (num_seqs > 0 && (!query_lens || !context_lens || !blocks_held || !seq_lens || !granted || !blocks_held_out ||
-                       blocks_held == blocks_held_out || context_lens == seq_lens || (max_blocks > 0 && !block_tables)))
+int gqa_step_plan(const gqa_step_plan_args* args, void* stream) {
+  if (!args) return GQA_ERR_INVALID_ARG;
+  const gqa_step_plan_args& a = *args;
+  if (a.num_seqs < 0 || a.max_blocks < 0 || a.max_tokens < 0 || a.num_free < 0 || a.bt_stride < a.max_blocks)
     return GQA_ERR_INVALID_ARG;
-  if (max_tokens > 0 && (!positions || !slot_mapping || !token_seqs)) return GQA_ERR_INVALID_ARG;
-  if (num_free > 0 && !free_blocks) return GQA_ERR_INVALID_ARG;
+  if (a.block_size < 1 || (a.block_size & (a.block_size - 1)) != 0) return GQA_ERR_UNSUPPORTED;
+  if (!a.cu_query_lens || !a.free_count || !a.free_count_out || a.free_count == a.free_count_out) return GQA_ERR_INVALID_ARG;
+  if (a.num_seqs > 0 && (!a.query_lens || !a.context_lens || !a.blocks_held || !a.seq_lens || !a.granted ||
+                         !a.blocks_held_out || a.blocks_held == a.blocks_held_out || a.context_lens == a.seq_lens ||
+                         (a.max_blocks > 0 && !a.block_tables)))
+    return GQA_ERR_INVALID_ARG;
+  if (a.max_tokens > 0 && (!a.positions || !a.slot_mapping || !a.token_seqs)) return GQA_ERR_INVALID_ARG;
+  if (a.num_free > 0 && !a.free_blocks) return GQA_ERR_INVALID_ARG;
   int sm = 0;
   int rc = current_device(&sm);
   if (rc) return rc;
   StepPlanParams p{};
-  p.query_lens = query_lens;
-  p.context_lens = context_lens;
-  p.blocks_held = blocks_held;
-  p.free_blocks = free_blocks;
-  p.free_count = free_count;
-  p.block_tables = block_tables;
-  p.cu_query_lens = cu_query_lens;
-  p.seq_lens = seq_lens;
-  p.positions = positions;
-  p.slot_mapping = slot_mapping;
-  p.token_seqs = token_seqs;
-  p.granted = granted;
-  p.blocks_held_out = blocks_held_out;
-  p.free_count_out = free_count_out;
-  p.bt_stride = bt_stride;
-  p.n = num_seqs;
-  p.max_blocks = max_blocks;
-  p.num_free = num_free;
-  p.block_shift = pow2_shift(block_size);
-  p.max_tokens = max_tokens;
-  const int threads = num_seqs > 256 ? 1024 : 256;
-  const int grid = std::max(1, std::min(sm, (max_tokens + threads - 1) / threads));
+  p.query_lens = a.query_lens;
+  p.context_lens = a.context_lens;
+  p.blocks_held = a.blocks_held;
+  p.free_blocks = a.free_blocks;
+  p.free_count = a.free_count;
+  p.block_tables = a.block_tables;
+  p.cu_query_lens = a.cu_query_lens;
+  p.seq_lens = a.seq_lens;
+  p.positions = a.positions;
+  p.slot_mapping = a.slot_mapping;
+  p.token_seqs = a.token_seqs;
+  p.granted = a.granted;
+  p.blocks_held_out = a.blocks_held_out;
+  p.free_count_out = a.free_count_out;
+  p.bt_stride = a.bt_stride;
+  p.n = a.num_seqs;
+  p.max_blocks = a.max_blocks;
+  p.num_free = a.num_free;
+  p.block_shift = pow2_shift(a.block_size);
+  p.max_tokens = a.max_tokens;
+  const int threads = a.num_seqs > 256 ? 1024 : 256;
+  const int grid = std::max(1, std::min(sm, (a.max_tokens + threads - 1) / threads));
   const cudaError_t e = launch_pdl(gqa_step_plan_kernel, dim3(grid), threads, 0, reinterpret_cast<cudaStream_t>(stream), p);
   return e == cudaSuccess ? GQA_OK : GQA_ERR_CUDA;
 }
 
-int gqa_qk_norm_rope(const void* q, const void* k, const void* v, const int64_t* q_strides3, const int64_t* k_strides3,
-                     const int64_t* v_strides3, const void* q_weight, const void* k_weight, const int* positions,
-                     int64_t pos_stride, int axes, const int* sections, const float* cos_sin, int max_positions,
-                     int rotary_dim, int interleaved, void* q_out, void* k_dst, void* v_dst, const int64_t* slot_mapping,
-                     int num_tokens, int num_heads, int num_kv_heads, int head_dim, int block_size, int num_blocks,
-                     int dtype, int cache_fp8, float eps, float k_scale, float v_scale, void* stream) {
-  if (num_tokens < 0 || num_heads <= 0 || num_kv_heads <= 0 || max_positions < 0 || !(eps >= 0.f)) return GQA_ERR_INVALID_ARG;
-  if (head_dim != 64 && head_dim != 128) return GQA_ERR_UNSUPPORTED;
-  if (dtype != GQA_DTYPE_BF16 && dtype != GQA_DTYPE_F16) return GQA_ERR_UNSUPPORTED;
-  if (axes < 1 || axes > kMaxAxes) return GQA_ERR_UNSUPPORTED;
-  if (rotary_dim < 0 || rotary_dim > head_dim || rotary_dim % 16 != 0) return GQA_ERR_UNSUPPORTED;
+int gqa_qk_norm_rope(const gqa_qk_norm_rope_args* args, void* stream) {
+  if (!args) return GQA_ERR_INVALID_ARG;
+  const gqa_qk_norm_rope_args& a = *args;
+  if (a.num_tokens < 0 || a.num_heads <= 0 || a.num_kv_heads <= 0 || a.max_positions < 0 || !(a.eps >= 0.f)) return GQA_ERR_INVALID_ARG;
+  if (a.head_dim != 64 && a.head_dim != 128) return GQA_ERR_UNSUPPORTED;
+  if (a.dtype != GQA_DTYPE_BF16 && a.dtype != GQA_DTYPE_F16) return GQA_ERR_UNSUPPORTED;
+  if (a.axes < 1 || a.axes > kMaxAxes) return GQA_ERR_UNSUPPORTED;
+  if (a.rotary_dim < 0 || a.rotary_dim > a.head_dim || a.rotary_dim % 16 != 0) return GQA_ERR_UNSUPPORTED;
   RopeParams p{};
   int end = 0;
-  for (int a = 0; a < axes; ++a) {
-    const int size = sections ? sections[a] : (axes == 1 ? rotary_dim / 2 : -1);
-    if (size < 0) return GQA_ERR_INVALID_ARG;
-    end += size;
-    p.section_end[a] = end;
+  for (int i = 0; i < a.axes; ++i) {
+    if (a.sections[i] < 0) return GQA_ERR_INVALID_ARG;
+    end += a.sections[i];
+    p.section_end[i] = end;
   }
-  if (end != rotary_dim / 2) return GQA_ERR_INVALID_ARG;
-  if (num_tokens == 0) return GQA_OK;
-  const bool cached = slot_mapping != nullptr;
-  if (!positions || !q_out || !k_dst || (rotary_dim > 0 && !cos_sin)) return GQA_ERR_INVALID_ARG;
-  if (cached && (!v_dst || block_size <= 0 || num_blocks < 0)) return GQA_ERR_INVALID_ARG;
-  if (!cached && (v_dst || cache_fp8)) return GQA_ERR_INVALID_ARG;
-  if (cache_fp8 && !(k_scale > 0.f && v_scale > 0.f)) return GQA_ERR_INVALID_ARG;
-  if (!aligned16(q_out) || !aligned16(k_dst) || !aligned16(v_dst) || !aligned16(q_weight) || !aligned16(k_weight))
+  if (end != a.rotary_dim / 2) return GQA_ERR_INVALID_ARG;
+  if (a.num_tokens == 0) return GQA_OK;
+  const bool cached = a.slot_mapping != nullptr;
+  if (!a.positions || !a.q_out || !a.k_dst || (a.rotary_dim > 0 && !a.cos_sin)) return GQA_ERR_INVALID_ARG;
+  if (cached && (!a.v_dst || a.block_size <= 0 || a.num_blocks < 0)) return GQA_ERR_INVALID_ARG;
+  if (!cached && (a.v_dst || a.cache_fp8)) return GQA_ERR_INVALID_ARG;
+  if (a.cache_fp8 && !(a.k_scale > 0.f && a.v_scale > 0.f)) return GQA_ERR_INVALID_ARG;
+  if (!aligned16(a.q_out) || !aligned16(a.k_dst) || !aligned16(a.v_dst) || !aligned16(a.q_weight) || !aligned16(a.k_weight))
     return GQA_ERR_ALIGNMENT;
-  int rc = check_strides3(q, q_strides3, 8);
-  if (!rc) rc = check_strides3(k, k_strides3, 8);
-  if (!rc && cached) rc = check_strides3(v, v_strides3, 8);
+  int rc = check_strides3(a.q, a.q_strides, 8);
+  if (!rc) rc = check_strides3(a.k, a.k_strides, 8);
+  if (!rc && cached) rc = check_strides3(a.v, a.v_strides, 8);
   if (rc) return rc;
   rc = current_device(nullptr);
   if (rc) return rc;
-  p.q = reinterpret_cast<const uint16_t*>(q);
-  p.k = reinterpret_cast<const uint16_t*>(k);
-  p.v = reinterpret_cast<const uint16_t*>(v);
-  p.q_st = q_strides3[0]; p.q_sh = q_strides3[1];
-  p.k_st = k_strides3[0]; p.k_sh = k_strides3[1];
-  if (cached) { p.v_st = v_strides3[0]; p.v_sh = v_strides3[1]; }
-  p.q_weight = reinterpret_cast<const uint16_t*>(q_weight);
-  p.k_weight = reinterpret_cast<const uint16_t*>(k_weight);
-  p.positions = positions;
-  p.pos_stride = pos_stride;
-  p.table = cos_sin;
-  p.q_out = reinterpret_cast<uint16_t*>(q_out);
-  p.k_dst = k_dst;
-  p.v_dst = v_dst;
-  p.slots = slot_mapping;
-  p.num_slots = (int64_t)num_blocks * block_size;
-  p.num_tokens = num_tokens;
-  p.hq = num_heads;
-  p.hkv = num_kv_heads;
-  p.rot = rotary_dim;
-  p.axes = axes;
-  p.max_pos = max_positions;
-  p.interleaved = interleaved ? 1 : 0;
-  p.eps = eps;
-  p.k_scale = k_scale;
-  p.v_scale = v_scale;
+  p.q = reinterpret_cast<const uint16_t*>(a.q);
+  p.k = reinterpret_cast<const uint16_t*>(a.k);
+  p.v = reinterpret_cast<const uint16_t*>(a.v);
+  p.q_st = a.q_strides[0]; p.q_sh = a.q_strides[1];
+  p.k_st = a.k_strides[0]; p.k_sh = a.k_strides[1];
+  if (cached) { p.v_st = a.v_strides[0]; p.v_sh = a.v_strides[1]; }
+  p.q_weight = reinterpret_cast<const uint16_t*>(a.q_weight);
+  p.k_weight = reinterpret_cast<const uint16_t*>(a.k_weight);
+  p.positions = a.positions;
+  p.pos_stride = a.pos_stride;
+  p.table = a.cos_sin;
+  p.q_out = reinterpret_cast<uint16_t*>(a.q_out);
+  p.k_dst = a.k_dst;
+  p.v_dst = a.v_dst;
+  p.slots = a.slot_mapping;
+  p.num_slots = (int64_t)a.num_blocks * a.block_size;
+  p.num_tokens = a.num_tokens;
+  p.hq = a.num_heads;
+  p.hkv = a.num_kv_heads;
+  p.rot = a.rotary_dim;
+  p.axes = a.axes;
+  p.max_pos = a.max_positions;
+  p.interleaved = a.interleaved ? 1 : 0;
+  p.eps = a.eps;
+  p.k_scale = a.k_scale;
+  p.v_scale = a.v_scale;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  const bool bf = dtype == GQA_DTYPE_BF16;
-  const dim3 grid(num_tokens);
+  const bool bf = a.dtype == GQA_DTYPE_BF16;
+  const dim3 grid(a.num_tokens);
   cudaError_t e;
 #define GQA_ROPE(D)                                                                    \
-  e = cache_fp8 ? (bf ? launch_pdl(gqa_rope_kernel<D, true, true>, grid, 256, 0, st, p) \
+  e = a.cache_fp8 ? (bf ? launch_pdl(gqa_rope_kernel<D, true, true>, grid, 256, 0, st, p) \
                       : launch_pdl(gqa_rope_kernel<D, false, true>, grid, 256, 0, st, p)) \
                 : (bf ? launch_pdl(gqa_rope_kernel<D, true, false>, grid, 256, 0, st, p) \
                       : launch_pdl(gqa_rope_kernel<D, false, false>, grid, 256, 0, st, p))
-  if (head_dim == 128) { GQA_ROPE(128); } else { GQA_ROPE(64); }
+  if (a.head_dim == 128) { GQA_ROPE(128); } else { GQA_ROPE(64); }
 #undef GQA_ROPE
   return e == cudaSuccess ? GQA_OK : GQA_ERR_CUDA;
 }
 
-size_t gqa_ragged_fwd_workspace_bytes(int num_seqs, int num_tokens, int num_heads, int num_kv_heads, int max_query_len,
-                                      int max_seq_len, int head_dim, int window, int cache_fp8) {
+size_t gqa_ragged_fwd_workspace_bytes(const gqa_ragged_args* args) {
   RaggedShape s;
   int sm = 0;
-  if (check_ragged_shape(num_seqs, num_tokens, num_heads, num_kv_heads, max_query_len, max_seq_len, head_dim, window, &s) ||
-      num_seqs == 0 || num_tokens == 0 || max_query_len == 0 || current_device(&sm))
-    return 0;
-  const bool tile = ragged_uses_tile(s, cache_fp8 != 0);
+  if (!args || check_ragged_shape(*args, &s) || s.n == 0 || s.tokens == 0 || s.max_q == 0 || current_device(&sm)) return 0;
+  const bool tile = ragged_uses_tile(s, args->cache_fp8 != 0);
   const RaggedPlan tp = plan_ragged_tile(s, sm);
   return ragged_ws_bytes(plan_ragged_stream(stream_part(s, tile), sm), tile ? &tp : nullptr, s);
 }
 
-int gqa_ragged_fwd(const void* q, const void* k_cache, const void* v_cache, void* o, float* lse,
-                   const int64_t* q_strides3, const int64_t* k_strides4, const int64_t* v_strides4,
-                   const int64_t* o_strides3, const int* block_table, int bt_stride, const int* cu_query_lens,
-                   const int* seq_lens, const float* alibi_slopes, const int* prefix_lens, const int* key_starts,
-                   int num_seqs, int num_tokens, int num_heads, int num_kv_heads, int head_dim, int block_size,
-                   int num_blocks, int max_query_len, int max_seq_len, float scale, float softcap, int window, int causal,
-                   int dtype, int cache_fp8, float k_scale, float v_scale, void* workspace, size_t workspace_bytes,
-                   void* stream) {
+int gqa_ragged_fwd(const gqa_ragged_args* args, void* stream) {
   RaggedShape s;
-  int rc = check_ragged_shape(num_seqs, num_tokens, num_heads, num_kv_heads, max_query_len, max_seq_len, head_dim, window,
-                              &s);
+  if (!args) return GQA_ERR_INVALID_ARG;
+  const gqa_ragged_args& a = *args;
+  int rc = check_ragged_shape(a, &s);
   if (rc) return rc;
-  if (dtype != GQA_DTYPE_BF16 && dtype != GQA_DTYPE_F16) return GQA_ERR_UNSUPPORTED;
-  if (block_size < 16 || (block_size & (block_size - 1)) != 0 || num_blocks <= 0) return GQA_ERR_UNSUPPORTED;
-  if (cache_fp8 && head_dim != 128) return GQA_ERR_UNSUPPORTED;
-  if (cache_fp8 && !(k_scale > 0.f && v_scale > 0.f)) return GQA_ERR_INVALID_ARG;
-  if (!(softcap >= 0.f) || !(scale > 0.f)) return GQA_ERR_INVALID_ARG;
-  if (num_seqs == 0 || num_tokens == 0 || max_query_len == 0) return GQA_OK;
-  if (!block_table || !cu_query_lens || !seq_lens || bt_stride <= 0) return GQA_ERR_INVALID_ARG;
-  if (max_seq_len > (int64_t)bt_stride * block_size) return GQA_ERR_INVALID_ARG;
-  if (!causal && (window > 0 || prefix_lens)) return GQA_ERR_INVALID_ARG;
-  rc = check_strides3(q, q_strides3, 8);
-  if (!rc) rc = check_strides3(o, o_strides3, 8);
-  if (!rc) rc = (k_cache && v_cache && k_strides4 && v_strides4) ? GQA_OK : GQA_ERR_INVALID_ARG;
-  if (!rc && (k_strides4[3] != 1 || v_strides4[3] != 1 || !aligned16(k_cache) || !aligned16(v_cache))) rc = GQA_ERR_ALIGNMENT;
+  if (a.dtype != GQA_DTYPE_BF16 && a.dtype != GQA_DTYPE_F16) return GQA_ERR_UNSUPPORTED;
+  if (a.block_size < 16 || (a.block_size & (a.block_size - 1)) != 0 || a.num_blocks <= 0) return GQA_ERR_UNSUPPORTED;
+  if (a.cache_fp8 && a.head_dim != 128) return GQA_ERR_UNSUPPORTED;
+  if (a.cache_fp8 && !(a.k_scale > 0.f && a.v_scale > 0.f)) return GQA_ERR_INVALID_ARG;
+  if (!(a.softcap >= 0.f) || !(a.scale > 0.f)) return GQA_ERR_INVALID_ARG;
+  if (a.num_seqs == 0 || a.num_tokens == 0 || a.max_query_len == 0) return GQA_OK;
+  if (!a.block_table || !a.cu_query_lens || !a.seq_lens || a.bt_stride <= 0) return GQA_ERR_INVALID_ARG;
+  if (a.max_seq_len > (int64_t)a.bt_stride * a.block_size) return GQA_ERR_INVALID_ARG;
+  if (!a.causal && (a.window > 0 || a.prefix_lens)) return GQA_ERR_INVALID_ARG;
+  rc = check_strides3(a.q, a.q_strides, 8);
+  if (!rc) rc = check_strides3(a.o, a.o_strides, 8);
+  if (!rc) rc = (a.k_cache && a.v_cache) ? GQA_OK : GQA_ERR_INVALID_ARG;
+  if (!rc && (a.k_strides[3] != 1 || a.v_strides[3] != 1 || !aligned16(a.k_cache) || !aligned16(a.v_cache))) rc = GQA_ERR_ALIGNMENT;
   if (rc) return rc;
   int sm = 0;
   rc = current_device(&sm);
   if (rc) return rc;
-  s.causal = causal ? 1 : 0;
-  s.prefix = prefix_lens != nullptr;
 
   RaggedParams p{};
-  p.q = reinterpret_cast<const uint16_t*>(q);
-  p.o = reinterpret_cast<uint16_t*>(o);
-  p.lse = lse;
-  p.q_st = q_strides3[0]; p.q_sh = q_strides3[1];
-  p.o_st = o_strides3[0]; p.o_sh = o_strides3[1];
-  p.cu = cu_query_lens;
-  p.seq_lens = seq_lens;
-  p.block_table = block_table;
-  p.bt_stride = bt_stride;
-  p.block_shift = pow2_shift(block_size);
-  p.num_blocks = num_blocks;
-  p.box = std::min(64, block_size);
-  p.alibi = alibi_slopes;
-  p.prefix = prefix_lens;
-  p.key_starts = key_starts;
-  p.window = window;
+  p.q = reinterpret_cast<const uint16_t*>(a.q);
+  p.o = reinterpret_cast<uint16_t*>(a.o);
+  p.lse = a.lse;
+  p.q_st = a.q_strides[0]; p.q_sh = a.q_strides[1];
+  p.o_st = a.o_strides[0]; p.o_sh = a.o_strides[1];
+  p.cu = a.cu_query_lens;
+  p.seq_lens = a.seq_lens;
+  p.block_table = a.block_table;
+  p.bt_stride = a.bt_stride;
+  p.block_shift = pow2_shift(a.block_size);
+  p.num_blocks = a.num_blocks;
+  p.box = std::min(64, a.block_size);
+  p.alibi = a.alibi_slopes;
+  p.prefix = a.prefix_lens;
+  p.key_starts = a.key_starts;
+  p.window = a.window;
   p.causal = s.causal;
-  p.n = num_seqs;
-  p.num_tokens = num_tokens;
-  p.hq = num_heads;
-  p.hkv = num_kv_heads;
+  p.n = a.num_seqs;
+  p.num_tokens = a.num_tokens;
+  p.hq = a.num_heads;
+  p.hkv = a.num_kv_heads;
   p.group = s.group;
-  p.max_len = max_seq_len;
+  p.max_len = a.max_seq_len;
   constexpr double kLog2e = 1.4426950408889634;
-  const double sc = (double)scale * (cache_fp8 ? (double)k_scale : 1.0);
+  const double sc = (double)a.scale * (a.cache_fp8 ? (double)a.k_scale : 1.0);
   p.scale_log2 = (float)(sc * kLog2e);
-  p.cap_in = softcap > 0.f ? (float)(2.0 * kLog2e * sc / softcap) : 0.f;
-  p.cap_out = softcap > 0.f ? (float)(softcap * kLog2e) : 0.f;
-  if (softcap > 0.f) set_cap_polynomial(p, sc / softcap, softcap * kLog2e);
-  p.v_scale = cache_fp8 ? v_scale : 1.f;
-  p.mods = softcap > 0.f || alibi_slopes;
+  p.cap_in = a.softcap > 0.f ? (float)(2.0 * kLog2e * sc / a.softcap) : 0.f;
+  p.cap_out = a.softcap > 0.f ? (float)(a.softcap * kLog2e) : 0.f;
+  if (a.softcap > 0.f) set_cap_polynomial(p, sc / a.softcap, a.softcap * kLog2e);
+  p.v_scale = a.cache_fp8 ? a.v_scale : 1.f;
+  p.mods = a.softcap > 0.f || a.alibi_slopes;
 
-  const bool tile = ragged_uses_tile(s, cache_fp8 != 0);
+  const bool tile = ragged_uses_tile(s, a.cache_fp8 != 0);
   const RaggedShape ss = stream_part(s, tile);
   RaggedPlan sp = plan_ragged_stream(ss, sm), tp = plan_ragged_tile(s, sm);
-  const bool have_ws = workspace && aligned16(workspace) && workspace_bytes >= ragged_ws_bytes(sp, tile ? &tp : nullptr, s);
-  if (!have_ws) {  // no room for the partials: one CTA per tile
+  if (a.workspace) {
+    if (!aligned16(a.workspace)) return GQA_ERR_ALIGNMENT;
+    if (a.workspace_bytes < ragged_ws_bytes(sp, tile ? &tp : nullptr, s)) return GQA_ERR_WORKSPACE;
+  } else {  // nowhere to leave partials: one CTA per tile
     sp.nsplit = tp.nsplit = 1;
-    sp.chunk = tp.chunk = std::max(1, (max_seq_len + 127) / 128) * 128;
+    sp.chunk = tp.chunk = std::max(1, (a.max_seq_len + 127) / 128) * 128;
   }
-  uint8_t* const counters = reinterpret_cast<uint8_t*>(workspace);
+  uint8_t* const counters = reinterpret_cast<uint8_t*>(a.workspace);
   uint8_t* const partials = counters + (size_t)kServingCounters * 4;
   CUtensorMap km, vm;
-  rc = make_cache_map(&km, k_cache, k_strides4, num_blocks, block_size, num_kv_heads, head_dim, p.box, cache_fp8);
-  if (!rc) rc = make_cache_map(&vm, v_cache, v_strides4, num_blocks, block_size, num_kv_heads, head_dim, p.box, cache_fp8);
+  rc = make_cache_map(&km, a.k_cache, a.k_strides, a.num_blocks, a.block_size, a.num_kv_heads, a.head_dim, p.box, a.cache_fp8);
+  if (!rc) rc = make_cache_map(&vm, a.v_cache, a.v_strides, a.num_blocks, a.block_size, a.num_kv_heads, a.head_dim, p.box, a.cache_fp8);
   if (rc) return rc;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  const bool bf = dtype == GQA_DTYPE_BF16;
+  const bool bf = a.dtype == GQA_DTYPE_BF16;
   cudaError_t e = cudaSuccess;
 
   if (tile) {
@@ -432,13 +422,13 @@ int gqa_ragged_fwd(const void* q, const void* k_cache, const void* v_cache, void
     if (tp.nsplit > 1)
       ragged_ws_carve(tp, s, counters + (size_t)kServingCounters * 2, partials + ragged_partial_bytes(sp, s), &t);
     // Queries (d, head, token): a tile is bm tokens of the group's heads, token-major rows.
-    const int64_t bhsd[4] = {q_strides3[0] * num_tokens, q_strides3[0], q_strides3[1], 1};
+    const int64_t bhsd[4] = {a.q_strides[0] * a.num_tokens, a.q_strides[0], a.q_strides[1], 1};
     CUtensorMap qm;
-    rc = make_map(&qm, q, bhsd, 1, num_tokens, num_heads, head_dim, s.group, tp.block_m / 2);
+    rc = make_map(&qm, a.q, bhsd, 1, a.num_tokens, a.num_heads, a.head_dim, s.group, tp.block_m / 2);
     if (rc) return rc;
-    const int64_t grid = (int64_t)tp.slots * num_kv_heads * tp.nsplit;
+    const int64_t grid = (int64_t)tp.slots * a.num_kv_heads * tp.nsplit;
     if (grid > INT_MAX) return GQA_ERR_INVALID_ARG;
-    if (head_dim == 128)
+    if (a.head_dim == 128)
       e = bf ? launch_ragged_tile_hd<128, true>(t, (unsigned)grid, qm, km, vm, st)
              : launch_ragged_tile_hd<128, false>(t, (unsigned)grid, qm, km, vm, st);
     else
@@ -451,12 +441,12 @@ int gqa_ragged_fwd(const void* q, const void* k_cache, const void* v_cache, void
   p.min_rows = 0;
   p.max_rows = tile ? kStreamMaxRows : INT_MAX;
   if (sp.nsplit > 1) ragged_ws_carve(sp, s, counters, partials, &p);
-  const int64_t grid = (int64_t)sp.slots * num_kv_heads * sp.nsplit;
+  const int64_t grid = (int64_t)sp.slots * a.num_kv_heads * sp.nsplit;
   if (grid > INT_MAX) return GQA_ERR_INVALID_ARG;
-  if (cache_fp8)
+  if (a.cache_fp8)
     e = bf ? launch_ragged_stream_hd<128, true, true>(p, (unsigned)grid, km, vm, st)
            : launch_ragged_stream_hd<128, false, true>(p, (unsigned)grid, km, vm, st);
-  else if (head_dim == 128)
+  else if (a.head_dim == 128)
     e = bf ? launch_ragged_stream_hd<128, true, false>(p, (unsigned)grid, km, vm, st)
            : launch_ragged_stream_hd<128, false, false>(p, (unsigned)grid, km, vm, st);
   else
@@ -475,12 +465,13 @@ struct VerifyPlan {
   int nsplit, part;
 };
 
-// CTAs per row: enough for two waves' worth of CTAs over the device, at least 2048
-// entries each.
-VerifyPlan plan_verify(int64_t rows, int vocab, int sm_count) {
+// CTAs per row: about one wave over the device, at least 1024 entries each. Four CTAs of
+// the race fit an SM (registers), five of the greedy scan, of whose rows -- the most that
+// the requests can have -- a good part is usually absent.
+VerifyPlan plan_verify(int64_t rows, int vocab, int sm_count, bool greedy) {
   VerifyPlan pl;
-  const int64_t want = (4 * (int64_t)sm_count + rows - 1) / std::max<int64_t>(rows, 1);
-  const int64_t most = std::max(1, vocab / 2048);
+  const int64_t want = (int64_t)sm_count * (greedy ? 8 : 4) / std::max<int64_t>(rows, 1);
+  const int64_t most = std::max(1, vocab / 1024);
   pl.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>(std::min(want, most), 256));
   pl.part = (((vocab + pl.nsplit - 1) / pl.nsplit) + 7) & ~7;
   return pl;
@@ -490,38 +481,36 @@ size_t verify_ws_bytes(int64_t units, const VerifyPlan& pl) {
   return (size_t)kServingCounters * 4 + 2 * align256((size_t)units * pl.nsplit * 4);
 }
 
-int verify_common(VerifyParams& p, int greedy, const int* draft_tokens, int64_t draft_token_stride, const void* target,
-                  int64_t target_stride, const int* cu_query_lens, int* tokens, int* num_tokens, int num_seqs,
-                  int num_rows, int max_drafts, int vocab, int dtype, void* workspace, size_t workspace_bytes,
-                  int* grid) {
-  if (num_seqs < 0 || num_rows < 0 || max_drafts < 0 || vocab <= 0 || vocab > INT_MAX - 64) return GQA_ERR_INVALID_ARG;
-  if (max_drafts > kVerifyMaxDrafts || num_seqs > kServingCounters) return GQA_ERR_UNSUPPORTED;
-  if (dtype != GQA_DTYPE_BF16 && dtype != GQA_DTYPE_F16 && dtype != GQA_DTYPE_F32) return GQA_ERR_UNSUPPORTED;
-  if (num_seqs == 0) return GQA_OK;
-  if (!cu_query_lens || !tokens || !num_tokens || (max_drafts > 0 && !draft_tokens) || (num_rows > 0 && !target) ||
-      target_stride < 0 || draft_token_stride < 0)
+int verify_common(VerifyParams& p, int greedy, const gqa_verify_args& a, int* grid) {
+  if (a.num_seqs < 0 || a.num_rows < 0 || a.max_drafts < 0 || a.vocab <= 0 || a.vocab > INT_MAX - 64)
+    return GQA_ERR_INVALID_ARG;
+  if (a.max_drafts > kVerifyMaxDrafts || a.num_seqs > kServingCounters) return GQA_ERR_UNSUPPORTED;
+  if (a.dtype != GQA_DTYPE_BF16 && a.dtype != GQA_DTYPE_F16 && a.dtype != GQA_DTYPE_F32) return GQA_ERR_UNSUPPORTED;
+  if (a.num_seqs == 0) return GQA_OK;
+  if (!a.cu_query_lens || !a.tokens || !a.num_tokens || (a.max_drafts > 0 && !a.draft_tokens) ||
+      (a.num_rows > 0 && !a.target) || a.target_stride < 0 || a.draft_token_stride < 0)
     return GQA_ERR_INVALID_ARG;
   int sm = 0;
   const int rc = current_device(&sm);
   if (rc) return rc;
-  const int64_t units = (int64_t)num_seqs * (greedy ? max_drafts + 1 : 1);
-  const VerifyPlan pl = plan_verify(units, vocab, sm);
-  if (!workspace || !aligned16(workspace) || workspace_bytes < verify_ws_bytes(units, pl)) return GQA_ERR_WORKSPACE;
+  const int64_t units = (int64_t)a.num_seqs * (greedy ? a.max_drafts + 1 : 1);
+  const VerifyPlan pl = plan_verify(units, a.vocab, sm, greedy != 0);
+  if (!a.workspace || !aligned16(a.workspace) || a.workspace_bytes < verify_ws_bytes(units, pl)) return GQA_ERR_WORKSPACE;
   if (units * pl.nsplit > INT_MAX) return GQA_ERR_INVALID_ARG;
-  p.draft_tokens = draft_tokens;
-  p.dt_st = draft_token_stride;
-  p.target = target;
-  p.t_st = target_stride;
-  p.cu = cu_query_lens;
-  p.tokens = tokens;
-  p.num_tokens = num_tokens;
-  p.n = num_seqs;
-  p.k = max_drafts;
-  p.vocab = vocab;
-  p.num_rows = num_rows;
+  p.draft_tokens = a.draft_tokens;
+  p.dt_st = a.draft_token_stride;
+  p.target = a.target;
+  p.t_st = a.target_stride;
+  p.cu = a.cu_query_lens;
+  p.tokens = a.tokens;
+  p.num_tokens = a.num_tokens;
+  p.n = a.num_seqs;
+  p.k = a.max_drafts;
+  p.vocab = a.vocab;
+  p.num_rows = a.num_rows;
   p.nsplit = pl.nsplit;
   p.part = pl.part;
-  uint8_t* c = reinterpret_cast<uint8_t*>(workspace);
+  uint8_t* c = reinterpret_cast<uint8_t*>(a.workspace);
   p.ws_cnt = reinterpret_cast<unsigned*>(c);
   c += (size_t)kServingCounters * 4;
   p.ws_score = reinterpret_cast<float*>(c);
@@ -536,53 +525,49 @@ int verify_common(VerifyParams& p, int greedy, const int* draft_tokens, int64_t 
 
 extern "C" {
 
-size_t gqa_verify_workspace_bytes(int num_seqs, int max_drafts, int vocab, int greedy) {
+size_t gqa_verify_workspace_bytes(const gqa_verify_args* args, int greedy) {
   int sm = 0;
-  if (num_seqs <= 0 || max_drafts < 0 || vocab <= 0 || current_device(&sm)) return 0;
-  const int64_t units = (int64_t)num_seqs * (greedy ? max_drafts + 1 : 1);
-  return verify_ws_bytes(units, plan_verify(units, vocab, sm));
+  if (!args || args->num_seqs <= 0 || args->max_drafts < 0 || args->vocab <= 0 || current_device(&sm)) return 0;
+  const int64_t units = (int64_t)args->num_seqs * (greedy ? args->max_drafts + 1 : 1);
+  return verify_ws_bytes(units, plan_verify(units, args->vocab, sm, greedy != 0));
 }
 
-int gqa_verify_drafts(const int* draft_tokens, int64_t draft_token_stride, const void* target_probs, int64_t target_stride,
-                      const void* draft_probs, const int64_t* draft_strides2, const float* uniforms,
-                      int64_t uniform_stride, const float* exponentials, int64_t exponential_stride,
-                      const int* cu_query_lens, int* tokens, int* num_tokens, int num_seqs, int num_rows, int max_drafts,
-                      int vocab, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
+int gqa_verify_drafts(const gqa_verify_args* args, void* stream) {
+  if (!args) return GQA_ERR_INVALID_ARG;
+  const gqa_verify_args& a = *args;
+  if (a.num_seqs > 0 && (!a.exponentials || a.exponential_stride < 0 || (a.max_drafts > 0 && (!a.uniforms || a.uniform_stride < 0)) ||
+                         a.draft_strides[0] < 0 || a.draft_strides[1] < 0))
+    return GQA_ERR_INVALID_ARG;
   VerifyParams p{};
   int grid = 0;
-  int rc = verify_common(p, 0, draft_tokens, draft_token_stride, target_probs, target_stride, cu_query_lens, tokens,
-                         num_tokens, num_seqs, num_rows, max_drafts, vocab, dtype, workspace, workspace_bytes, &grid);
-  if (rc || num_seqs == 0) return rc;
-  if (!exponentials || exponential_stride < 0 || (max_drafts > 0 && (!uniforms || uniform_stride < 0)) ||
-      (draft_probs && (!draft_strides2 || draft_strides2[0] < 0 || draft_strides2[1] < 0)))
-    return GQA_ERR_INVALID_ARG;
-  p.draft = max_drafts > 0 ? draft_probs : nullptr;
-  if (draft_probs) { p.d_sn = draft_strides2[0]; p.d_sk = draft_strides2[1]; }
-  p.uniforms = uniforms;
-  p.u_st = uniform_stride;
-  p.expo = exponentials;
-  p.e_st = exponential_stride;
+  const int rc = verify_common(p, 0, a, &grid);
+  if (rc || a.num_seqs == 0) return rc;
+  p.draft = a.max_drafts > 0 ? a.draft_probs : nullptr;
+  p.d_sn = a.draft_strides[0];
+  p.d_sk = a.draft_strides[1];
+  p.uniforms = a.uniforms;
+  p.u_st = a.uniform_stride;
+  p.expo = a.exponentials;
+  p.e_st = a.exponential_stride;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const cudaError_t e =
-      dtype == GQA_DTYPE_F32 ? launch_pdl(gqa_verify_kernel<kProbF32>, dim3(grid), kVerifyThreads, 0, st, p)
-      : dtype == GQA_DTYPE_BF16 ? launch_pdl(gqa_verify_kernel<kProbBf16>, dim3(grid), kVerifyThreads, 0, st, p)
-                                : launch_pdl(gqa_verify_kernel<kProbF16>, dim3(grid), kVerifyThreads, 0, st, p);
+      a.dtype == GQA_DTYPE_F32    ? launch_pdl(gqa_verify_kernel<kProbF32>, dim3(grid), kVerifyThreads, 0, st, p)
+      : a.dtype == GQA_DTYPE_BF16 ? launch_pdl(gqa_verify_kernel<kProbBf16>, dim3(grid), kVerifyThreads, 0, st, p)
+                                  : launch_pdl(gqa_verify_kernel<kProbF16>, dim3(grid), kVerifyThreads, 0, st, p);
   return e == cudaSuccess ? GQA_OK : GQA_ERR_CUDA;
 }
 
-int gqa_verify_greedy(const int* draft_tokens, int64_t draft_token_stride, const void* target, int64_t target_stride,
-                      const int* cu_query_lens, int* tokens, int* num_tokens, int num_seqs, int num_rows, int max_drafts,
-                      int vocab, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
+int gqa_verify_greedy(const gqa_verify_args* args, void* stream) {
+  if (!args) return GQA_ERR_INVALID_ARG;
   VerifyParams p{};
   int grid = 0;
-  const int rc = verify_common(p, 1, draft_tokens, draft_token_stride, target, target_stride, cu_query_lens, tokens,
-                               num_tokens, num_seqs, num_rows, max_drafts, vocab, dtype, workspace, workspace_bytes, &grid);
-  if (rc || num_seqs == 0) return rc;
+  const int rc = verify_common(p, 1, *args, &grid);
+  if (rc || args->num_seqs == 0) return rc;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const cudaError_t e =
-      dtype == GQA_DTYPE_F32 ? launch_pdl(gqa_verify_greedy_kernel<kProbF32>, dim3(grid), kVerifyThreads, 0, st, p)
-      : dtype == GQA_DTYPE_BF16 ? launch_pdl(gqa_verify_greedy_kernel<kProbBf16>, dim3(grid), kVerifyThreads, 0, st, p)
-                                : launch_pdl(gqa_verify_greedy_kernel<kProbF16>, dim3(grid), kVerifyThreads, 0, st, p);
+      args->dtype == GQA_DTYPE_F32    ? launch_pdl(gqa_verify_greedy_kernel<kProbF32>, dim3(grid), kVerifyThreads, 0, st, p)
+      : args->dtype == GQA_DTYPE_BF16 ? launch_pdl(gqa_verify_greedy_kernel<kProbBf16>, dim3(grid), kVerifyThreads, 0, st, p)
+                                      : launch_pdl(gqa_verify_greedy_kernel<kProbF16>, dim3(grid), kVerifyThreads, 0, st, p);
   return e == cudaSuccess ? GQA_OK : GQA_ERR_CUDA;
 }
 

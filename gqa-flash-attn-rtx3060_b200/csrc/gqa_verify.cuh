@@ -16,8 +16,12 @@
 // the vocabulary is split over `nsplit` CTAs per request. Each walks the request's drafts
 // itself (at most 64 gathers, in parallel) to learn the row, scans its part, and leaves
 // its best in the workspace; the request's last CTA (a ticket, reset for the next call)
-// picks among them.
+// picks among them. The division is only made for entries that can win: w / e > best
+// needs w >= best e (1 - 2^-23) whatever the roundings, one product instead of a
+// division that is slow for the many zero weights.
 #pragma once
+
+#include <climits>
 
 #include "gqa_common.cuh"
 
@@ -39,41 +43,43 @@ struct VerifyParams {
   unsigned* ws_cnt;  // [n], zero between calls
 };
 
-constexpr int kVerifyThreads = 512;
+constexpr int kVerifyThreads = 256;
 constexpr int kVerifyMaxDrafts = 64;
 
 enum : int { kProbF32 = 0, kProbBf16 = 1, kProbF16 = 2 };
 
+// Probabilities or logits of one dtype; Vec = values per 16 bytes.
 template <int DT>
-struct ProbType;
+struct ProbType {
+  using T = uint16_t;
+  static constexpr int Vec = 8;
+  static __device__ __forceinline__ float value(T x) {
+    if constexpr (DT == kProbBf16) return __uint_as_float((uint32_t)x << 16);
+    else return __half2float(__ushort_as_half(x));
+  }
+  static __device__ __forceinline__ float load(const T* p) { return value(__ldg(p)); }
+  static __device__ __forceinline__ void load_vec(const T* p, float (&f)[Vec]) {
+    const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 y = DT == kProbBf16 ? make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u))
+                                       : __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      f[2 * i] = y.x;
+      f[2 * i + 1] = y.y;
+    }
+  }
+};
 template <>
 struct ProbType<kProbF32> {
   using T = float;
-  static constexpr int kVec = 4;
-  static __device__ __forceinline__ float load(const T* p) { return *p; }
-  static __device__ __forceinline__ void load_vec(const T* p, float (&f)[4]) {
-    const float4 v = *reinterpret_cast<const float4*>(p);
+  static constexpr int Vec = 4;
+  static __device__ __forceinline__ float load(const T* p) { return __ldg(p); }
+  static __device__ __forceinline__ void load_vec(const T* p, float (&f)[Vec]) {
+    const float4 v = __ldg(reinterpret_cast<const float4*>(p));
     f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w;
   }
 };
-template <bool BF16>
-struct ProbType16 {
-  using T = uint16_t;
-  static constexpr int kVec = 4;
-  static __device__ __forceinline__ float load(const T* p) {
-    if constexpr (BF16) return __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(p));
-    else return __half2float(*reinterpret_cast<const __half*>(p));
-  }
-  static __device__ __forceinline__ void load_vec(const T* p, float (&f)[4]) {
-    const uint2 v = *reinterpret_cast<const uint2*>(p);
-    f[0] = load(reinterpret_cast<const T*>(&v.x)); f[1] = load(reinterpret_cast<const T*>(&v.x) + 1);
-    f[2] = load(reinterpret_cast<const T*>(&v.y)); f[3] = load(reinterpret_cast<const T*>(&v.y) + 1);
-  }
-};
-template <>
-struct ProbType<kProbBf16> : ProbType16<true> {};
-template <>
-struct ProbType<kProbF16> : ProbType16<false> {};
 
 struct Best {
   float score;
@@ -112,26 +118,108 @@ __device__ __forceinline__ bool verify_rows(const VerifyParams& p, int b, int& r
   return r0 >= 0 && rows > 0;
 }
 
-// Best of entries [j0, j1) of a row by `score(j)` / `score4(j, f)`: each thread takes
-// its entries in rising order, so the first best is kept with a plain comparison.
-template <typename S1, typename S4>
-__device__ __forceinline__ Best scan_part(int j0, int j1, bool vec, S1 score, S4 score4, Best best) {
-  if (vec) {
-    const int jv = j0 + ((j1 - j0) & ~3);
-#pragma unroll 4
-    for (int j = j0 + 4 * (int)threadIdx.x; j < jv; j += 4 * (int)blockDim.x) {
-      float f[4];
-      score4(j, f);
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (f[e] > best.score) best = Best{f[e], j + e};
-    }
-    j0 = jv;
-  }
-#pragma unroll 8
-  for (int j = j0 + (int)threadIdx.x; j < j1; j += (int)blockDim.x) {
-    const float f = score(j);
+// Largest of entries [j0, j1) of a row: each thread takes its entries in rising order, so
+// the first largest is kept with a plain comparison.
+template <typename PT>
+__device__ __forceinline__ Best scan_largest(const typename PT::T* row, int j0, int j1, bool vec) {
+  constexpr int V = PT::Vec, U = 4;
+  Best best{-INFINITY, INT_MAX};
+  auto take = [&](float f, int j) {
     if (f > best.score) best = Best{f, j};
+  };
+  if (vec) {
+    const int step = V * kVerifyThreads;
+    for (int j = j0 + V * (int)threadIdx.x; j < j1; j += U * step) {
+      float f[U][V];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (j + u * step + V <= j1) PT::load_vec(row + j + u * step, f[u]);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int at = j + u * step;
+        if (at + V <= j1) {
+#pragma unroll
+          for (int e = 0; e < V; ++e) take(f[u][e], at + e);
+        } else {
+          for (int e = at; e < j1; ++e) take(PT::load(row + e), e);
+        }
+      }
+    }
+    return best;
+  }
+  constexpr int US = 8;
+  for (int j = j0 + (int)threadIdx.x; j < j1; j += US * kVerifyThreads) {
+    float f[US];
+#pragma unroll
+    for (int u = 0; u < US; ++u) f[u] = j + u * kVerifyThreads < j1 ? PT::load(row + j + u * kVerifyThreads) : -INFINITY;
+#pragma unroll
+    for (int u = 0; u < US; ++u) take(f[u], j + u * kVerifyThreads);
+  }
+  return best;
+}
+
+// First best of max(p - q, 0) / e over entries [j0, j1) (q null: of p / e), entry `hidden` left out.
+template <typename PT>
+__device__ __forceinline__ Best scan_race(const typename PT::T* prow, const typename PT::T* qrow, const float* erow, int hidden,
+                                          int j0, int j1, bool vec) {
+  constexpr int V = 4, U = 2, US = 8;
+  Best best{0.f, INT_MAX};
+  auto take = [&](float pj, float qj, float ej, int j) {
+    const float w = __fsub_rn(pj, qj);
+    if (w > 0.f && w >= best.score * ej * 0.9999995f && j != hidden) {  // 1 - 2^-21
+      const float f = __fdiv_rn(w, ej);
+      if (f > best.score) best = Best{f, j};
+    }
+  };
+  if (vec) {
+    const int step = V * kVerifyThreads;
+    auto load4 = [&](const typename PT::T* p, float (&f)[V]) {
+      if constexpr (sizeof(typename PT::T) == 4) {
+        PT::load_vec(p, f);
+      } else {
+        const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
+        const typename PT::T h[4] = {(uint16_t)v.x, (uint16_t)(v.x >> 16), (uint16_t)v.y, (uint16_t)(v.y >> 16)};
+#pragma unroll
+        for (int e = 0; e < V; ++e) f[e] = PT::value(h[e]);
+      }
+    };
+    for (int j = j0 + V * (int)threadIdx.x; j < j1; j += U * step) {
+      float a[U][V], c[U][V], e4[U][V];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int at = j + u * step;
+        if (at + V <= j1) {
+          load4(prow + at, a[u]);
+          if (qrow) load4(qrow + at, c[u]);
+          const float4 e = __ldg(reinterpret_cast<const float4*>(erow + at));
+          e4[u][0] = e.x; e4[u][1] = e.y; e4[u][2] = e.z; e4[u][3] = e.w;
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int at = j + u * step;
+        if (at + V <= j1) {
+#pragma unroll
+          for (int e = 0; e < V; ++e) take(a[u][e], qrow ? c[u][e] : 0.f, e4[u][e], at + e);
+        } else {
+          for (int e = at; e < j1; ++e) take(PT::load(prow + e), qrow ? PT::load(qrow + e) : 0.f, __ldg(erow + e), e);
+        }
+      }
+    }
+    return best;
+  }
+  for (int j = j0 + (int)threadIdx.x; j < j1; j += US * kVerifyThreads) {
+    float a[US], c[US], e[US];
+#pragma unroll
+    for (int u = 0; u < US; ++u) {
+      const int at = min(j + u * kVerifyThreads, j1 - 1);
+      a[u] = PT::load(prow + at);
+      c[u] = qrow ? PT::load(qrow + at) : 0.f;
+      e[u] = __ldg(erow + at);
+    }
+#pragma unroll
+    for (int u = 0; u < US; ++u)
+      if (j + u * kVerifyThreads < j1) take(a[u], c[u], e[u], j + u * kVerifyThreads);
   }
   return best;
 }
@@ -180,25 +268,9 @@ __global__ void __launch_bounds__(kVerifyThreads) gqa_verify_kernel(const Verify
   const float* erow = p.expo + b * p.e_st;
 
   const int j0 = min(p.vocab, split * p.part), j1 = min(p.vocab, j0 + p.part);
-  auto score_of = [&](float pj, float qj, float ej, int j) {
-    const float w = fmaxf(__fsub_rn(pj, qj), 0.f);
-    return (j == hidden) ? 0.f : __fdiv_rn(w, ej);
-  };
   const bool vec = ((reinterpret_cast<uintptr_t>(prow) | reinterpret_cast<uintptr_t>(drow)) % (4 * sizeof(T))) == 0 &&
                    (reinterpret_cast<uintptr_t>(erow) & 15) == 0;
-  Best best = scan_part(
-      j0, j1, vec, [&](int j) { return score_of(PT::load(prow + j), drow ? PT::load(drow + j) : 0.f, erow[j], j); },
-      [&](int j, float (&f)[4]) {
-        float a[4], c[4] = {0.f, 0.f, 0.f, 0.f};
-        PT::load_vec(prow + j, a);
-        if (drow) PT::load_vec(drow + j, c);
-        const float4 e = *reinterpret_cast<const float4*>(erow + j);
-        f[0] = score_of(a[0], c[0], e.x, j);
-        f[1] = score_of(a[1], c[1], e.y, j + 1);
-        f[2] = score_of(a[2], c[2], e.z, j + 2);
-        f[3] = score_of(a[3], c[3], e.w, j + 3);
-      },
-      Best{0.f, p.vocab});
+  Best best = scan_race<PT>(prow, drow, erow, hidden, j0, j1, vec);
   best = block_best(best);
 
   if (p.nsplit > 1) {
@@ -212,7 +284,7 @@ __global__ void __launch_bounds__(kVerifyThreads) gqa_verify_kernel(const Verify
     }
     __syncthreads();
     if (!s_last) return;
-    best = Best{0.f, p.vocab};
+    best = Best{0.f, INT_MAX};
     for (int i = tid; i < p.nsplit; i += blockDim.x)
       best = better(best, Best{__ldcg(p.ws_score + (int64_t)b * p.nsplit + i),
                                __ldcg(p.ws_index + (int64_t)b * p.nsplit + i)});
@@ -220,9 +292,7 @@ __global__ void __launch_bounds__(kVerifyThreads) gqa_verify_kernel(const Verify
   }
   if (!(best.score > 0.f)) {
     // No weight is left (p and q agree where p is not zero, or the row holds NaN): the row's first largest.
-    best = scan_part(
-        0, p.vocab, false, [&](int j) { return PT::load(prow + j); }, [](int, float (&)[4]) {},
-        Best{-INFINITY, p.vocab});
+    best = scan_largest<PT>(prow, 0, p.vocab, false);
     best = block_best(best);
     if (best.index >= p.vocab) best.index = 0;
   }
@@ -257,10 +327,7 @@ __global__ void __launch_bounds__(kVerifyThreads) gqa_verify_greedy_kernel(const
   if (i > drafts) return;
   const T* row = reinterpret_cast<const T*>(p.target) + (int64_t)(r0 + i) * p.t_st;
   const int j0 = min(p.vocab, split * p.part), j1 = min(p.vocab, j0 + p.part);
-  const bool vec = (reinterpret_cast<uintptr_t>(row) % (4 * sizeof(T))) == 0;
-  Best best = scan_part(
-      j0, j1, vec, [&](int j) { return PT::load(row + j); }, [&](int j, float (&f)[4]) { PT::load_vec(row + j, f); },
-      Best{-INFINITY, p.vocab});
+  Best best = scan_largest<PT>(row, j0, j1, (reinterpret_cast<uintptr_t>(row) & 15) == 0);
   best = block_best(best);
   const int64_t unit = (int64_t)b * (p.k + 1);
   if (tid == 0) {
@@ -274,7 +341,7 @@ __global__ void __launch_bounds__(kVerifyThreads) gqa_verify_greedy_kernel(const
   __syncthreads();
   if (!s_last) return;
   for (int r = warp; r <= drafts; r += blockDim.x >> 5) {
-    Best x{-INFINITY, p.vocab};
+    Best x{-INFINITY, INT_MAX};
     for (int s = lane; s < p.nsplit; s += 32)
       x = better(x, Best{__ldcg(p.ws_score + (unit + r) * p.nsplit + s), __ldcg(p.ws_index + (unit + r) * p.nsplit + s)});
     x = warp_best(x);

@@ -74,18 +74,15 @@ SIGNATURES = {
                                   _P]),
 }
 
-_I64 = ctypes.c_int64
+# The ragged serving step's entry points take a struct (packed by _serving.py) and a stream.
 SIGNATURES.update({
-    "gqa_step_plan": (_I, [_P, _P, _P, _I64, _P, _P, _I, _P, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P, _P]),
-    "gqa_qk_norm_rope": (_I, [_P, _P, _P, _I64P, _I64P, _I64P, _P, _P, _P, _I64, _I, _P, _P, _I, _I, _I, _P, _P, _P, _P,
-                              _I, _I, _I, _I, _I, _I, _I, _I, _F, _F, _F, _P]),
-    "gqa_ragged_fwd_workspace_bytes": (_SZ, [_I, _I, _I, _I, _I, _I, _I, _I, _I]),
-    "gqa_ragged_fwd": (_I, [_P, _P, _P, _P, _P, _I64P, _I64P, _I64P, _I64P, _P, _I, _P, _P, _P, _P, _P,
-                            _I, _I, _I, _I, _I, _I, _I, _I, _I, _F, _F, _I, _I, _I, _I, _F, _F, _P, _SZ, _P]),
-    "gqa_verify_workspace_bytes": (_SZ, [_I, _I, _I, _I]),
-    "gqa_verify_drafts": (_I, [_P, _I64, _P, _I64, _P, _I64P, _P, _I64, _P, _I64, _P, _P, _P, _I, _I, _I, _I, _I, _P, _SZ,
-                               _P]),
-    "gqa_verify_greedy": (_I, [_P, _I64, _P, _I64, _P, _P, _P, _I, _I, _I, _I, _I, _P, _SZ, _P]),
+    "gqa_step_plan": (_I, [_P, _P]),
+    "gqa_qk_norm_rope": (_I, [_P, _P]),
+    "gqa_ragged_fwd_workspace_bytes": (_SZ, [_P]),
+    "gqa_ragged_fwd": (_I, [_P, _P]),
+    "gqa_verify_workspace_bytes": (_SZ, [_P, _I]),
+    "gqa_verify_drafts": (_I, [_P, _P]),
+    "gqa_verify_greedy": (_I, [_P, _P]),
 })
 
 _lib = None
@@ -244,9 +241,7 @@ class WorkspaceCache:
 
 
 WORKSPACES = WorkspaceCache()
-# The ragged serving step's: its counters have one place for every shape, so one
-# signature serves all calls and nothing is zeroed after the allocation.
-SERVING_WORKSPACES = WorkspaceCache()
+ON_DEVICE_ERROR = []  # further drops of cached workspaces, called with the device's index
 
 
 def device_error(clear=True):
@@ -260,6 +255,7 @@ def device_error(clear=True):
     site = ctypes.c_int(0)
     check(load().gqa_device_error(ctypes.byref(code), ctypes.byref(site), 1 if clear else 0), "gqa_device_error")
     if code.value != 0:
-        for cache in (WORKSPACES, SERVING_WORKSPACES):
-            cache.drop(torch.device("cuda", torch.cuda.current_device()))
+        WORKSPACES.drop(torch.device("cuda", torch.cuda.current_device()))
+        for drop in ON_DEVICE_ERROR:
+            drop(torch.cuda.current_device())
     return code.value, site.value

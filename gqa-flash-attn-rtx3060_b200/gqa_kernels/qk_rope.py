@@ -9,11 +9,9 @@ kernel, straight from the projection's output into the paged caches that
 the same without a cache: it returns the rotated keys, for gqa_flash_attn and
 PrefixKVCache.
 """
-import ctypes
-
 import torch
 
-from . import _lib
+from . import _lib, _serving
 
 __all__ = ["rope_table", "qk_norm_rope", "qk_norm_rope_append"]
 
@@ -26,35 +24,12 @@ def rope_table(max_positions, rotary_dim, base=10000.0, device="cuda"):
     return torch.cat([angle.cos(), angle.sin()], dim=1).float().to(device)
 
 
-_SECTIONS = {}
-
-
-def _sections(sections, axes, rotary_dim):
-    """The sections as a ctypes array (one per distinct tuple; the library only reads it during the call)."""
-    if sections is None:
-        if axes != 1:
-            raise ValueError("several position axes need sections")
-        return None
-    key = tuple(sections)
-    arr = _SECTIONS.get(key)
-    if arr is None:
-        if len(_SECTIONS) > 256:
-            _SECTIONS.clear()
-        arr = _SECTIONS[key] = (ctypes.c_int * len(key))(*key)
-    if len(key) != axes or sum(key) * 2 != rotary_dim or min(key) < 0:
-        raise ValueError("sections must give each position axis its share of the rotary_dim / 2 frequencies")
-    return arr
-
-
 def _launch(q, k, v, positions, cos_sin, k_dst, v_dst, slots, block_size, num_blocks, q_weight, k_weight, eps, sections,
             interleaved, out, k_scale, v_scale):
-    if q.dim() != 3 or k.dim() != 3:
-        raise ValueError("q and k must be (num_tokens, heads, head_dim)")
     num_tokens, num_heads, head_dim = q.shape
-    num_kv_heads = k.shape[1]
-    if k.shape[0] != num_tokens or k.shape[2] != head_dim:
-        raise ValueError("q and k must have the same tokens and head_dim")
-    if head_dim not in (64, 128):
+    if k.dim() != 3 or k.shape[0] != num_tokens or k.shape[2] != head_dim:
+        raise ValueError("q and k must be (num_tokens, heads, head_dim) of the same tokens and head_dim")
+    if head_dim != 128 and head_dim != 64:
         raise ValueError(f"unsupported head_dim {head_dim}")
     dt = q.dtype
     dtype = _lib.dtype_code(q)
@@ -63,49 +38,48 @@ def _launch(q, k, v, positions, cos_sin, k_dst, v_dst, slots, block_size, num_bl
     if positions.dtype != torch.int32 or positions.dim() not in (1, 2) or positions.shape[-1] != num_tokens:
         raise ValueError("positions must be int32 (num_tokens,) or (axes, num_tokens)")
     axes = 1 if positions.dim() == 1 else positions.shape[0]
-    if not 1 <= axes <= 4:
-        raise ValueError("1 to 4 position axes are supported")
     if cos_sin.dtype != torch.float32 or cos_sin.dim() != 2 or not cos_sin.is_contiguous():
         raise ValueError("cos_sin must be a contiguous float32 (max_positions, rotary_dim)")
     max_positions, rotary_dim = cos_sin.shape
     if rotary_dim > head_dim or rotary_dim % 16:
         raise ValueError("rotary_dim must be a multiple of 16, at most head_dim")
-    sec = _sections(sections, axes, rotary_dim)
-    others = [k, positions, cos_sin, k_dst]
-    qw = kw = None
-    for w in (q_weight, k_weight):
-        if w is not None:
-            if w.shape != (head_dim,) or w.dtype != dt or w.stride(0) != 1 or w.data_ptr() & 15:
-                raise ValueError("norm weights must be contiguous (head_dim,) tensors of q's dtype, 16-byte aligned")
-            others.append(w)
-    if q_weight is not None:
-        qw = q_weight.data_ptr()
-    if k_weight is not None:
-        kw = k_weight.data_ptr()
-    if out is None:
-        out = torch.empty(q.shape, dtype=dt, device=q.device)
+    if axes == 1:
+        sec = (rotary_dim // 2, 0, 0, 0)
+        if sections is not None and tuple(sections) != sec[:1]:
+            raise ValueError("one position axis has all of the rotary_dim / 2 frequencies")
     else:
-        if out.shape != q.shape or out.dtype != dt or not out.is_contiguous():
-            raise ValueError("out must be a contiguous tensor of q's shape and dtype")
-        others.append(out)
-    if v is not None:
-        others += [v, v_dst, slots]
-    _lib.check_one_device(q, *others)
-    q = q if _lib.tma_compatible(q) else q.contiguous()
-    k = k if _lib.tma_compatible(k) else k.contiguous()
-    if v is not None and not _lib.tma_compatible(v):
-        v = v.contiguous()
-    if positions.stride(-1) != 1:
+        if not 1 < axes <= 4:
+            raise ValueError("1 to 4 position axes are supported")
+        if sections is None or len(sections) != axes or sum(sections) * 2 != rotary_dim or min(sections) < 0:
+            raise ValueError("sections must give each position axis its share of the rotary_dim / 2 frequencies")
+        sec = (*sections, 0, 0)[:4]
+    for w in (q_weight, k_weight):
+        if w is not None and (w.shape != (head_dim,) or w.dtype != dt or w.stride(0) != 1 or w.data_ptr() & 15):
+            raise ValueError("norm weights must be contiguous (head_dim,) tensors of q's dtype, 16-byte aligned")
+    if out is None:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    elif out.shape != q.shape or out.dtype != dt or not out.is_contiguous():
+        raise ValueError("out must be a contiguous tensor of q's shape and dtype")
+    index = _serving.device_index(q, k, v, positions, cos_sin, k_dst, v_dst, slots, q_weight, k_weight, out)
+    if not _lib.tma_compatible(q):
+        q = q.contiguous()
+    if not _lib.tma_compatible(k):
+        k = k.contiguous()
+    if v is None:
+        vp = vd = sp = vs0 = vs1 = vs2 = 0
+    else:
+        if not _lib.tma_compatible(v):
+            v = v.contiguous()
+        vp, vd, sp = v.data_ptr(), v_dst.data_ptr(), slots.data_ptr()
+        vs0, vs1, vs2 = v.stride()
+    if positions.stride(-1) != 1 and num_tokens > 1:
         positions = positions.contiguous()
-    with _lib.on_device(q.device):
-        rc = _lib.load().gqa_qk_norm_rope(
-            q.data_ptr(), k.data_ptr(), None if v is None else v.data_ptr(), _lib.strides(q, 3), _lib.strides(k, 3),
-            None if v is None else _lib.strides(v, 3), qw, kw, positions.data_ptr(), positions.stride(0) if axes > 1 else 0,
-            axes, sec, cos_sin.data_ptr(), max_positions, rotary_dim, 1 if interleaved else 0, out.data_ptr(),
-            k_dst.data_ptr(), None if v is None else v_dst.data_ptr(), None if slots is None else slots.data_ptr(),
-            num_tokens, num_heads, num_kv_heads, head_dim, block_size, num_blocks, dtype,
-            1 if k_dst.dtype == torch.float8_e4m3fn else 0, eps, k_scale, v_scale, _lib.stream_ptr(q.device))
-    _lib.check(rc, "gqa_qk_norm_rope")
+    _serving.call("gqa_qk_norm_rope", _serving.QK_NORM_ROPE(
+        q.data_ptr(), k.data_ptr(), vp, 0 if q_weight is None else q_weight.data_ptr(),
+        0 if k_weight is None else k_weight.data_ptr(), positions.data_ptr(), cos_sin.data_ptr(), out.data_ptr(),
+        k_dst.data_ptr(), vd, sp, *q.stride(), *k.stride(), vs0, vs1, vs2, positions.stride(0) if axes > 1 else 0,
+        *sec, axes, max_positions, rotary_dim, 1 if interleaved else 0, num_tokens, num_heads, k.shape[1], head_dim, block_size,
+        num_blocks, dtype, 1 if k_dst.dtype == torch.float8_e4m3fn else 0, eps, k_scale, v_scale), index)
     return out
 
 
@@ -115,7 +89,7 @@ def qk_norm_rope(q, k, positions, cos_sin, q_weight=None, k_weight=None, eps=1e-
     Returns:
         (q, k) rotated, contiguous, in q's dtype.
     """
-    k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
     return _launch(q, k, None, positions, cos_sin, k_out, None, None, 0, 0, q_weight, k_weight, eps, sections, interleaved,
                    None, 1.0, 1.0), k_out
 
@@ -150,8 +124,8 @@ def qk_norm_rope_append(q, k, v, positions, cos_sin, key_cache, value_cache, slo
         the rotated queries, (num_tokens, num_heads, head_dim). The arithmetic is fp32,
         rounded once. Asynchronous on the current stream.
     """
-    num_blocks, block_size, hkv, hd = key_cache.shape
-    if v.shape != k.shape or v.dtype != k.dtype or value_cache.shape != key_cache.shape or k.shape[1:] != (hkv, hd):
+    num_blocks, block_size, hkv, hd = cache = key_cache.shape
+    if v.shape != k.shape or v.dtype != k.dtype or value_cache.shape != cache or k.shape != (q.shape[0], hkv, hd):
         raise ValueError("k/v must be (num_tokens, num_kv_heads, head_dim) of one dtype and the caches "
                          "(num_blocks, block_size, num_kv_heads, head_dim)")
     fp8 = key_cache.dtype == torch.float8_e4m3fn

@@ -11,24 +11,20 @@ packed into one request.
 """
 import torch
 
-from . import _lib
+from . import _lib, _serving
 from .qk_rope import qk_norm_rope_append
 
 __all__ = ["paged_ragged_attention", "RaggedPagedAttention"]
 
 
-def _optional(t, name, dtype, shape, query):
-    if t is None:
-        return None
+def _optional(t, name, dtype, shape):
     if t.dtype != dtype or t.shape != shape:
         raise ValueError(f"{name} must be {dtype} {tuple(shape)}")
-    if t.device != query.device:
-        raise ValueError("tensors must be on one device")
-    return (t if t.is_contiguous() else t.contiguous())
+    return t if t.is_contiguous() else t.contiguous()
 
 
-def _ptr(t):
-    return None if t is None else t.data_ptr()
+def _workspace_bytes(lib, args):
+    return lib.gqa_ragged_fwd_workspace_bytes(args)
 
 
 def paged_ragged_attention(query, key_cache, value_cache, block_tables, cu_query_lens, seq_lens, max_query_len=None,
@@ -98,10 +94,18 @@ def paged_ragged_attention(query, key_cache, value_cache, block_tables, cu_query
         raise ValueError("window and prefix_lens need causal")
     if fp8 and not (k_scale > 0 and v_scale > 0):
         raise ValueError("fp8 caches need positive k_scale and v_scale")
-    _lib.check_one_device(query, key_cache, value_cache, block_tables, cu_query_lens, seq_lens)
-    alibi_slopes = _optional(alibi_slopes, "alibi_slopes", torch.float32, (num_heads,), query)
-    prefix_lens = _optional(prefix_lens, "prefix_lens", torch.int32, (num_seqs,), query)
-    key_starts = _optional(key_starts, "key_starts", torch.int32, (num_tokens,), query)
+    if alibi_slopes is not None:
+        alibi_slopes = _optional(alibi_slopes, "alibi_slopes", torch.float32, (num_heads,))
+    if prefix_lens is not None:
+        prefix_lens = _optional(prefix_lens, "prefix_lens", torch.int32, (num_seqs,))
+    if key_starts is not None:
+        key_starts = _optional(key_starts, "key_starts", torch.int32, (num_tokens,))
+    if out is None:
+        out = torch.empty_like(query, memory_format=torch.contiguous_format)
+    elif out.shape != query.shape or out.dtype != query.dtype:
+        raise ValueError("out must have query's shape and dtype")
+    index = _serving.device_index(query, key_cache, value_cache, block_tables, cu_query_lens, seq_lens, out, alibi_slopes,
+                                  prefix_lens, key_starts)
     if not block_tables.is_contiguous():
         block_tables = block_tables.contiguous()
     if not seq_lens.is_contiguous():
@@ -110,33 +114,20 @@ def paged_ragged_attention(query, key_cache, value_cache, block_tables, cu_query
         cu_query_lens = cu_query_lens.contiguous()
     if not _lib.tma_compatible(query):
         query = query.contiguous()
-    capacity = block_tables.shape[1] * block_size
-    max_seq_len = capacity if max_seq_len is None else min(int(max_seq_len), capacity)
-    max_query_len = num_tokens if max_query_len is None else int(max_query_len)
-    if out is None:
-        out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
-    else:
-        if out.shape != query.shape or out.dtype != query.dtype:
-            raise ValueError("out must have query's shape and dtype")
-        _lib.check_one_device(query, out)
-    dev = query.device
-    lse = torch.empty((num_tokens, num_heads), dtype=torch.float32, device=dev) if return_lse else None
-    with _lib.on_device(dev):
-        nbytes = _lib.workspace_bytes("gqa_ragged_fwd_workspace_bytes", num_seqs, num_tokens, num_heads, num_kv_heads,
-                                      max_query_len, max_seq_len, head_dim,
-                                      0 if window is None or prefix_lens is not None else window, 1 if fp8 else 0)
-        ws = _lib.SERVING_WORKSPACES.get(dev, nbytes, None).data_ptr() if nbytes else None
-        rc = _lib.load().gqa_ragged_fwd(
-            query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), out.data_ptr(), _ptr(lse),
-            _lib.strides(query, 3), _lib.strides(key_cache), _lib.strides(value_cache), _lib.strides(out, 3),
-            block_tables.data_ptr(), block_tables.stride(0), cu_query_lens.data_ptr(), seq_lens.data_ptr(),
-            _ptr(alibi_slopes), _ptr(prefix_lens), _ptr(key_starts), num_seqs, num_tokens, num_heads, num_kv_heads, head_dim,
-            block_size, num_blocks, max_query_len, max_seq_len, head_dim ** -0.5 if scale is None else scale, softcap,
-            0 if window is None else window, 1 if causal else 0, dtype, 1 if fp8 else 0, k_scale, v_scale, ws, nbytes,
-            _lib.stream_ptr(dev))
-        if rc != 0:
-            _lib.SERVING_WORKSPACES.drop(dev)
-    _lib.check(rc, "gqa_ragged_fwd")
+    max_blocks = block_tables.shape[1]
+    if max_seq_len is None or max_seq_len > max_blocks * block_size:
+        max_seq_len = max_blocks * block_size
+    lse = torch.empty((num_tokens, num_heads), dtype=torch.float32, device=query.device) if return_lse else None
+    _serving.call_with_workspace("gqa_ragged_fwd", _serving.RAGGED(
+        query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(),
+        block_tables.data_ptr(), cu_query_lens.data_ptr(), seq_lens.data_ptr(),
+        0 if alibi_slopes is None else alibi_slopes.data_ptr(), 0 if prefix_lens is None else prefix_lens.data_ptr(),
+        0 if key_starts is None else key_starts.data_ptr(),
+        *query.stride(), *key_cache.stride(), *value_cache.stride(), *out.stride(),
+        max_blocks, num_seqs, num_tokens, num_heads, num_kv_heads, head_dim, block_size, num_blocks,
+        num_tokens if max_query_len is None else max_query_len, max_seq_len, 0 if window is None else window,
+        1 if causal else 0, dtype, 1 if fp8 else 0,
+        head_dim ** -0.5 if scale is None else scale, softcap, k_scale, v_scale), index, _workspace_bytes)
     return (out, lse) if return_lse else out
 
 

@@ -15,7 +15,7 @@ from dataclasses import dataclass
 
 import torch
 
-from . import _lib
+from . import _serving
 
 __all__ = ["StepPlan", "plan_step"]
 
@@ -97,22 +97,19 @@ def plan_step(query_lens, context_lens, block_tables, blocks_held, free_blocks, 
     for t in (query_lens, context_lens, blocks_held, free_blocks):
         if t.shape[0] > 1 and t.stride(0) != 1:
             raise ValueError("lengths and the free list must be contiguous")
-    dev = query_lens.device
-    _lib.check_one_device(query_lens, context_lens, block_tables, blocks_held, free_blocks, free_count)
+    index = _serving.device_index(query_lens, context_lens, block_tables, blocks_held, free_blocks, free_count)
     if out is None:
-        out = StepPlan.empty(n, max_tokens, dev)
+        out = StepPlan.empty(n, max_tokens, query_lens.device)
     else:
-        if out.seq_lens.shape[0] != n or out.positions.shape[0] != max_tokens or out.seq_lens.device != dev:
+        if out.seq_lens.shape[0] != n or out.positions.shape[0] != max_tokens or out.seq_lens.get_device() != index:
             raise ValueError("out must be a StepPlan of this n, max_tokens and device")
         if out.blocks_held.data_ptr() == blocks_held.data_ptr() or out.free_count.data_ptr() == free_count.data_ptr() \
                 or out.seq_lens.data_ptr() == context_lens.data_ptr():
             raise ValueError("out must not hold the tensors that the plan is made from")
-    with _lib.on_device(dev):
-        rc = _lib.load().gqa_step_plan(
-            query_lens.data_ptr(), context_lens.data_ptr(), block_tables.data_ptr(), max(block_tables.stride(0), max_blocks),
-            blocks_held.data_ptr(), free_blocks.data_ptr(), free_blocks.shape[0], free_count.data_ptr(), n, max_blocks,
-            block_size, max_tokens, out.cu_query_lens.data_ptr(), out.seq_lens.data_ptr(), out.positions.data_ptr(),
-            out.slot_mapping.data_ptr(), out.token_seqs.data_ptr(), out.granted.data_ptr(), out.blocks_held.data_ptr(),
-            out.free_count.data_ptr(), _lib.stream_ptr(dev))
-    _lib.check(rc, "gqa_step_plan")
+    _serving.call("gqa_step_plan", _serving.STEP_PLAN(
+        query_lens.data_ptr(), context_lens.data_ptr(), block_tables.data_ptr(), blocks_held.data_ptr(),
+        free_blocks.data_ptr(), free_count.data_ptr(), out.cu_query_lens.data_ptr(), out.seq_lens.data_ptr(),
+        out.positions.data_ptr(), out.slot_mapping.data_ptr(), out.token_seqs.data_ptr(), out.granted.data_ptr(),
+        out.blocks_held.data_ptr(), out.free_count.data_ptr(), max(block_tables.stride(0), max_blocks),
+        n, max_blocks, free_blocks.shape[0], block_size, max_tokens), index)
     return out

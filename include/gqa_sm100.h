@@ -310,7 +310,8 @@ int gqa_paged_kv_append(const void* key, const void* value, const int64_t* k_str
                         float v_scale, void* stream);
 
 /*
- * The ragged serving step: requests of any number of new tokens each (one for a
+ * The ragged serving step (its entry points take their arguments in a struct, which is
+ * only read during the call; strides are in elements): requests of any number of new tokens each (one for a
  * decode, a few drafted ones, a prompt or a chunk of one) planned, rotated, cached,
  * attended and verified without the host reading a length. No reference counterpart
  * (the roadmap's vLLM-shaped interface, README.md:144); the attention's definition is
@@ -331,11 +332,25 @@ int gqa_paged_kv_append(const void* key, const void* value, const int64_t* k_str
  * max_tokens are dropped and reported (GQA_ERR_INVALID_ARG, site 211). block_size: a
  * power of two.
  */
-int gqa_step_plan(const int* query_lens, const int* context_lens, int* block_tables, int64_t bt_stride,
-                  const int* blocks_held, const int* free_blocks, int num_free, const int* free_count, int num_seqs,
-                  int max_blocks, int block_size, int max_tokens, int* cu_query_lens, int* seq_lens, int* positions,
-                  int64_t* slot_mapping, int* token_seqs, unsigned char* granted, int* blocks_held_out,
-                  int* free_count_out, void* stream);
+typedef struct {
+  const int* query_lens;
+  const int* context_lens;
+  int* block_tables;
+  const int* blocks_held;
+  const int* free_blocks;
+  const int* free_count;
+  int* cu_query_lens;
+  int* seq_lens;
+  int* positions;
+  int64_t* slot_mapping;
+  int* token_seqs;
+  unsigned char* granted;
+  int* blocks_held_out;
+  int* free_count_out;
+  int64_t bt_stride;
+  int num_seqs, max_blocks, num_free, block_size, max_tokens;
+} gqa_step_plan_args;
+int gqa_step_plan(const gqa_step_plan_args* args, void* stream);
 
 /*
  * gqa_qk_norm_rope: RMS norm of every query and key head (weights of head_dim values in
@@ -343,7 +358,7 @@ int gqa_step_plan(const int* query_lens, const int* context_lens, int* block_tab
  * q (num_tokens, num_heads, head_dim), k and v (num_tokens, num_kv_heads, head_dim), element
  * strides of three dimensions (d stride 1, the others multiples of 8). Positions: axis
  * a of token t at positions[a * pos_stride + t]; the rotary_dim / 2 frequencies belong to
- * the axes (1 to 4) in consecutive sections[a] (NULL with one axis). cos_sin is float32
+ * the axes (1 to 4) in consecutive sections[a]. cos_sin is float32
  * (max_positions, rotary_dim), cosines then sines; rotary_dim a multiple of 16 up to
  * head_dim. Pairs are (f, f + rotary_dim / 2), interleaved: (2f, 2f + 1). q_out is
  * (num_tokens, num_heads, head_dim), contiguous. With slot_mapping, k and v go to the
@@ -354,12 +369,26 @@ int gqa_step_plan(const int* query_lens, const int* context_lens, int* block_tab
  * position (padding) gives zero rows and caches nothing; one with a position past the
  * table too, and is reported (site 212). Arithmetic is fp32 with one rounding.
  */
-int gqa_qk_norm_rope(const void* q, const void* k, const void* v, const int64_t* q_strides3, const int64_t* k_strides3,
-                     const int64_t* v_strides3, const void* q_weight, const void* k_weight, const int* positions,
-                     int64_t pos_stride, int axes, const int* sections, const float* cos_sin, int max_positions,
-                     int rotary_dim, int interleaved, void* q_out, void* k_dst, void* v_dst, const int64_t* slot_mapping,
-                     int num_tokens, int num_heads, int num_kv_heads, int head_dim, int block_size, int num_blocks,
-                     int dtype, int cache_fp8, float eps, float k_scale, float v_scale, void* stream);
+typedef struct {
+  const void* q;
+  const void* k;
+  const void* v;
+  const void* q_weight;
+  const void* k_weight;
+  const int* positions;
+  const float* cos_sin;
+  void* q_out;
+  void* k_dst;
+  void* v_dst;
+  const int64_t* slot_mapping;
+  int64_t q_strides[3], k_strides[3], v_strides[3];
+  int64_t pos_stride;
+  int sections[4];
+  int axes, max_positions, rotary_dim, interleaved;
+  int num_tokens, num_heads, num_kv_heads, head_dim, block_size, num_blocks, dtype, cache_fp8;
+  float eps, k_scale, v_scale;
+} gqa_qk_norm_rope_args;
+int gqa_qk_norm_rope(const gqa_qk_norm_rope_args* args, void* stream);
 
 /*
  * gqa_ragged_fwd: attention of request b's new tokens, rows cu_query_lens[b] ..
@@ -378,21 +407,32 @@ int gqa_qk_norm_rope(const void* q, const void* k, const void* v, const int64_t*
  * num_heads), float32, natural log, may be NULL. Groups of up to 64 heads, any number.
  * e4m3 caches (cache_fp8, scales as gqa_paged_fwd_kv8) need head_dim 128. max_query_len
  * and max_seq_len bound the lengths and must hold; longer sequences are clipped.
- * Workspace: gqa_ragged_fwd_workspace_bytes (window as passed, 0 with prefix_lens or
- * without causal), zeroed before its first use; every call leaves its counters zero,
- * whatever its shape, so calls of all shapes on one stream share one workspace. With less
- * the key axis is not split.
+ * Workspace: gqa_ragged_fwd_workspace_bytes of the same arguments (workspace and
+ * pointers are not looked at), zeroed before its first use; every call leaves its
+ * counters zero, whatever its shape, so calls of all shapes on one stream share one
+ * workspace. Too little gives GQA_ERR_WORKSPACE; NULL leaves the key axis unsplit.
  */
-size_t gqa_ragged_fwd_workspace_bytes(int num_seqs, int num_tokens, int num_heads, int num_kv_heads, int max_query_len,
-                                      int max_seq_len, int head_dim, int window, int cache_fp8);
-int gqa_ragged_fwd(const void* q, const void* k_cache, const void* v_cache, void* o, float* lse,
-                   const int64_t* q_strides3, const int64_t* k_strides4, const int64_t* v_strides4,
-                   const int64_t* o_strides3, const int* block_table, int bt_stride, const int* cu_query_lens,
-                   const int* seq_lens, const float* alibi_slopes, const int* prefix_lens, const int* key_starts,
-                   int num_seqs, int num_tokens, int num_heads, int num_kv_heads, int head_dim, int block_size,
-                   int num_blocks, int max_query_len, int max_seq_len, float scale, float softcap, int window, int causal,
-                   int dtype, int cache_fp8, float k_scale, float v_scale, void* workspace, size_t workspace_bytes,
-                   void* stream);
+typedef struct {
+  void* workspace;
+  size_t workspace_bytes;
+  const void* q;
+  const void* k_cache;
+  const void* v_cache;
+  void* o;
+  float* lse;
+  const int* block_table;
+  const int* cu_query_lens;
+  const int* seq_lens;
+  const float* alibi_slopes;
+  const int* prefix_lens;
+  const int* key_starts;
+  int64_t q_strides[3], k_strides[4], v_strides[4], o_strides[3];
+  int bt_stride, num_seqs, num_tokens, num_heads, num_kv_heads, head_dim, block_size, num_blocks;
+  int max_query_len, max_seq_len, window, causal, dtype, cache_fp8;
+  float scale, softcap, k_scale, v_scale;
+} gqa_ragged_args;
+size_t gqa_ragged_fwd_workspace_bytes(const gqa_ragged_args* args);
+int gqa_ragged_fwd(const gqa_ragged_args* args, void* stream);
 
 /*
  * gqa_verify_drafts: request b owns rows cu_query_lens[b] .. of the target's
@@ -413,15 +453,23 @@ int gqa_ragged_fwd(const void* q, const void* k_cache, const void* v_cache, void
  * The workspace (gqa_verify_workspace_bytes) may be gqa_ragged_fwd's: its counters
  * have the same place and are left zero too.
  */
-size_t gqa_verify_workspace_bytes(int num_seqs, int max_drafts, int vocab, int greedy);
-int gqa_verify_drafts(const int* draft_tokens, int64_t draft_token_stride, const void* target_probs, int64_t target_stride,
-                      const void* draft_probs, const int64_t* draft_strides2, const float* uniforms,
-                      int64_t uniform_stride, const float* exponentials, int64_t exponential_stride,
-                      const int* cu_query_lens, int* tokens, int* num_tokens, int num_seqs, int num_rows, int max_drafts,
-                      int vocab, int dtype, void* workspace, size_t workspace_bytes, void* stream);
-int gqa_verify_greedy(const int* draft_tokens, int64_t draft_token_stride, const void* target, int64_t target_stride,
-                      const int* cu_query_lens, int* tokens, int* num_tokens, int num_seqs, int num_rows, int max_drafts,
-                      int vocab, int dtype, void* workspace, size_t workspace_bytes, void* stream);
+typedef struct {
+  void* workspace;
+  size_t workspace_bytes;
+  const int* draft_tokens;
+  const void* target;
+  const void* draft_probs;   /* gqa_verify_drafts only, as the next two */
+  const float* uniforms;
+  const float* exponentials;
+  const int* cu_query_lens;
+  int* tokens;
+  int* num_tokens;
+  int64_t draft_token_stride, target_stride, draft_strides[2], uniform_stride, exponential_stride;
+  int num_seqs, num_rows, max_drafts, vocab, dtype;
+} gqa_verify_args;
+size_t gqa_verify_workspace_bytes(const gqa_verify_args* args, int greedy);
+int gqa_verify_drafts(const gqa_verify_args* args, void* stream);
+int gqa_verify_greedy(const gqa_verify_args* args, void* stream);
 
 /*
  * The tcgen05 prefill path's launch plan for a shape on `sm_count` SMs, without

@@ -1,6 +1,8 @@
 """The ragged step's argument checks, which need no GPU, and the restatements that its
 GPU tests compare with, against one another on small cases."""
-import ctypes
+import os
+import shutil
+import subprocess
 
 import pytest
 import torch
@@ -8,6 +10,8 @@ import torch
 from gqa_kernels import (RaggedPagedAttention, paged_ragged_attention, plan_step, qk_norm_rope, qk_norm_rope_append, rope_table,
                          verify_drafts, verify_drafts_greedy)
 from tests._serving import plan64, rope64, verify64
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
 def i32(*shape):
@@ -112,34 +116,55 @@ def test_layer_refuses():
 
 def test_c_entry_points_refuse_before_any_launch(lib_path):
     """The C ABI's own checks answer with a status, on a machine without a GPU."""
-    from gqa_kernels import _lib
+    from gqa_kernels import _lib, _serving
     lib = _lib.load()
-    st3, st4 = (ctypes.c_int64 * 3)(8, 8, 1), (ctypes.c_int64 * 4)(8, 8, 8, 1)
     one = 1 << 20  # a non-null, aligned address that is never read
 
     def ragged(hq=8, hkv=2, d=128, block=64, dtype=1, fp8=0, causal=1, window=0, scale=0.1, cap=0.0, table=one, max_len=64,
-               kstr=st4):
-        return lib.gqa_ragged_fwd(one, one, one, one, None, st3, kstr, kstr, st3, table, 1, one, one, None, None, None, 1, 1,
-                                  hq, hkv, d, block, 4, 1, max_len, scale, cap, window, causal, dtype, fp8, 1.0, 1.0, None, 0, None)
+               dstr=1, n=1):
+        return lib.gqa_ragged_fwd(_serving._WORKSPACE(0, 0) + _serving.RAGGED(
+            one, one, one, one, 0, table, one, one, 0, 0, 0, 8, 8, 1, 8, 8, 8, dstr, 8, 8, 8, 1, 8, 8, 1,
+            1, n, 1, hq, hkv, d, block, 4, 1, max_len, window, causal, dtype, fp8, scale, cap, 1.0, 1.0), None)
     assert ragged(hq=7) == 1 and ragged(d=96) == 2 and ragged(hq=130) == 2 and ragged(block=8) == 2 and ragged(block=48) == 2
     assert ragged(dtype=5) == 2 and ragged(d=64, fp8=1) == 2 and ragged(causal=0, window=3) == 1 and ragged(window=-1) == 1
-    assert ragged(scale=float("nan")) == 1 and ragged(cap=-1.0) == 1 and ragged(table=None) == 1 and ragged(max_len=65) == 1
-    assert ragged(kstr=(ctypes.c_int64 * 4)(8, 8, 8, 2)) == 3
+    assert ragged(scale=float("nan")) == 1 and ragged(cap=-1.0) == 1 and ragged(table=0) == 1 and ragged(max_len=65) == 1
+    assert ragged(dstr=2) == 3 and ragged(n=0) == 0 and lib.gqa_ragged_fwd(None, None) == 1
 
     def plan(held_out=2 * one, block=16, stride=4):
-        return lib.gqa_step_plan(one, one, one, stride, one, one, 4, one, 2, 4, block, 8, one, 3 * one, one, one, one, one, held_out,
-                                 2 * one, None)
-    assert plan(held_out=one) == 1 and plan(block=12) == 2 and plan(stride=3) == 1
+        return lib.gqa_step_plan(_serving.STEP_PLAN(one, one, one, one, one, one, one, 3 * one, one, one, one, one, held_out, 2 * one,
+                                                    stride, 2, 4, 4, block, 8), None)
+    assert plan(held_out=one) == 1 and plan(block=12) == 2 and plan(stride=3) == 1 and lib.gqa_step_plan(None, None) == 1
 
-    def rotate(d=128, rot=128, axes=1, sections=None, slots=one, eps=1e-6, q=one):
-        return lib.gqa_qk_norm_rope(q, one, one, st3, st3, st3, None, None, one, 0, axes, sections, one, 9, rot, 0, one, one, one,
-                                    slots, 3, 8, 2, d, 16, 4, 1, 0, eps, 1.0, 1.0, None)
-    assert rotate(d=80) == 2 and rotate(rot=24) == 2 and rotate(axes=5) == 2 and rotate(axes=2) == 1 and rotate(slots=None) == 1
-    assert rotate(eps=-1.0) == 1 and rotate(q=one + 8) == 3
+    def rotate(d=128, rot=128, axes=1, sections=(64, 0, 0, 0), slots=one, eps=1e-6, q=one):
+        return lib.gqa_qk_norm_rope(_serving.QK_NORM_ROPE(q, one, one, 0, 0, one, one, one, one, one, slots, 8, 8, 1, 8, 8, 1, 8, 8, 1, 0,
+                                                          *sections, axes, 9, rot, 0, 3, 8, 2, d, 16, 4, 1, 0, eps, 1.0, 1.0), None)
+    assert rotate(d=80) == 2 and rotate(rot=24) == 2 and rotate(axes=5) == 2 and rotate(axes=2, sections=(60, 3, 0, 0)) == 1
+    assert rotate(slots=0) == 1 and rotate(eps=-1.0) == 1 and rotate(q=one + 8) == 3 and lib.gqa_qk_norm_rope(None, None) == 1
 
-    def check(k=2, vocab=9, dtype=2, n=1, ws=None):
-        return lib.gqa_verify_drafts(one, 2, one, 9, None, None, one, 2, one, 9, one, one, one, n, 3, k, vocab, dtype, ws, 0, None)
-    assert check(k=65) == 2 and check(vocab=0) == 1 and check(dtype=7) == 2 and check(n=20000) == 2
+    def check(k=2, vocab=9, dtype=2, n=1):
+        return lib.gqa_verify_drafts(_serving._WORKSPACE(0, 0) + _serving.VERIFY(one, one, 0, one, one, one, one, one, 2, 9, 0, 0, 2, 9,
+                                                                                 n, 3, k, vocab, dtype), None)
+    assert check(k=65) == 2 and check(vocab=0) == 1 and check(dtype=7) == 2 and check(n=20000) == 2 and check(n=0) == 0
+    assert lib.gqa_verify_drafts(None, None) == 1 and lib.gqa_verify_greedy(None, None) == 1
+
+
+@pytest.mark.skipif(shutil.which("gcc") is None, reason="no C compiler")
+def test_packed_structs_match_the_header(tmp_path):
+    """The structs as a C compiler lays them out have the packed records' sizes and last fields' places."""
+    from gqa_kernels import _serving
+    ws = len(_serving._WORKSPACE(0, 0))
+    want = {"gqa_step_plan_args": ("max_tokens", _serving.STEP_PLAN(*[0] * 20)),
+            "gqa_qk_norm_rope_args": ("v_scale", _serving.QK_NORM_ROPE(*[0] * 40)),
+            "gqa_ragged_args": ("v_scale", bytes(ws) + _serving.RAGGED(*[0] * 43)),
+            "gqa_verify_args": ("dtype", bytes(ws) + _serving.VERIFY(*[0] * 19))}
+    src = tmp_path / "sizes.c"
+    src.write_text('#include <stdio.h>\n#include "gqa_sm100.h"\nint main(void) {\n' + "".join(
+        f'  printf("%zu %zu\\n", sizeof({t}), offsetof({t}, {f}));\n' for t, (f, _) in want.items()) + "  return 0;\n}\n")
+    exe = tmp_path / "sizes"
+    subprocess.run(["gcc", "-I", os.path.join(ROOT, "include"), str(src), "-o", str(exe)], check=True)
+    got = [tuple(map(int, x.split())) for x in subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout.splitlines()]
+    for (name, (_, packed)), (size, last) in zip(want.items(), got):
+        assert last == len(packed) - 4 and -(-len(packed) // 8) * 8 == size, name
 
 
 # ----------------------------------------------------------------------------- the restatements themselves
