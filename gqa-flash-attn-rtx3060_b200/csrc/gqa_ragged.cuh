@@ -31,6 +31,23 @@
 
 namespace gqa {
 
+// Requests of up to this many packed rows stream, longer ones take the tcgen05 form
+// (16-bit caches). STREAM_FIGURES
+constexpr int kRaggedStreamRows = 16;
+
+// How one of the two forms cuts the step into tiles of block_m tokens of one request.
+struct RaggedTiling {
+  int block_m, rows;      // rows = packed rows of a tile at most (its partials' stride)
+  int one_tile, slots;    // streaming form: every request has at most one tile, and slot b is
+                          // request b's; otherwise slots are found by ragged_slot
+  int min_rows, max_rows;  // packed rows of the requests that the form takes
+  int nsplit, chunk;      // key chunks of a tile at most; keys per chunk (a multiple of 128)
+  float* ws_m;            // partials [unit][nsplit][rows], unit = tile x kv head
+  float* ws_l;
+  float* ws_acc;
+  unsigned* ws_cnt;       // tickets [unit], zero between calls
+};
+
 struct RaggedParams {
   const uint16_t* q;
   uint16_t* o;
@@ -55,29 +72,20 @@ struct RaggedParams {
   float cap_most;
   float v_scale;          // e4m3 values
   int mods;               // cap or bias present
-  // Tiles: block_m tokens of one request, rows = block_m * group packed rows. With
-  // `one_tile` every request has at most one tile and tile slot b is request b; otherwise
-  // slots are found by ragged_slot.
-  int block_m, rows, one_tile, slots;
-  int min_rows;           // requests of fewer packed rows belong to the other kernel (0: none)
-  int max_rows;           // requests of more packed rows belong to the other kernel
-  int nsplit, chunk;      // key chunks of a tile (grid z); keys per chunk
-  float* ws_m;            // [slots * hkv][nsplit][rows]
-  float* ws_l;
-  float* ws_acc;          // [slots * hkv][nsplit][rows][HD]
-  unsigned* ws_cnt;       // [slots * hkv], zero between calls
+  RaggedTiling stream, tile;
+  unsigned tile_ctas;     // CTAs of the tcgen05 form, the grid's first; the rest stream
 };
 
 // Request b's tiles take the slots cu[b] / block_m + b, +1, ...: it has at most
 // cu[b + 1] / block_m - cu[b] / block_m + 1 of them, so the ranges do not overlap, and
 // the last request whose first slot is not above `slot` is its owner, if any. A warp
 // bisects 32 ways. Returns the request, or -1.
-__device__ __forceinline__ int ragged_slot(const RaggedParams& p, int slot, int lane) {
+__device__ __forceinline__ int ragged_slot(const RaggedParams& p, const RaggedTiling& tl, int slot, int lane) {
   int lo = 0, n = p.n;  // the owner is in [lo, lo + n)
   while (n > 1) {
     const int step = (n + 31) >> 5;
     const int i = lo + lane * step;
-    const bool below = lane * step < n && p.cu[i] / p.block_m + i <= slot;
+    const bool below = lane * step < n && p.cu[i] / tl.block_m + i <= slot;
     const unsigned m = __ballot_sync(0xffffffffu, below);
     if (m == 0) return -1;
     const int at = 31 - __clz(m);
@@ -97,16 +105,17 @@ struct RaggedWork {
 
 // The tile of request b that starts at its token m0: the union over its rows, by one warp.
 // False: no such tile, or not this kernel's.
-__device__ __forceinline__ bool ragged_work_at(const RaggedParams& p, int b, int m0, int lane, RaggedWork& w) {
+__device__ __forceinline__ bool ragged_work_at(const RaggedParams& p, const RaggedTiling& tl, int b, int m0, int lane,
+                                               RaggedWork& w) {
   w.b = b;
   w.m0 = m0;
   const int first = p.cu[b];
   const int qn = min(p.cu[b + 1], p.num_tokens) - first;
   if (first < 0 || m0 < 0 || m0 >= qn) return false;
   const int64_t qrows = (int64_t)qn * p.group;
-  if (qrows < p.min_rows || qrows > p.max_rows) return false;
+  if (qrows < tl.min_rows || qrows > tl.max_rows) return false;
   w.t0 = first + w.m0;
-  w.nq = min(p.block_m, qn - w.m0);
+  w.nq = min(tl.block_m, qn - w.m0);
   (void)GQA_CHECK(p.seq_lens[w.b] <= p.max_len, 906);
   w.len = max(0, min(p.seq_lens[w.b], p.max_len));
   w.off = w.len - qn;
@@ -124,13 +133,14 @@ __device__ __forceinline__ bool ragged_work_at(const RaggedParams& p, int b, int
     w.k_lo = max(w.k_lo, __reduce_min_sync(0xffffffffu, s));
   }
   w.k_base = min(w.k_lo, w.k_hi) & ~(p.box - 1);
-  w.n_chunks = w.k_hi > w.k_lo ? (w.k_hi - w.k_base + p.chunk - 1) / p.chunk : 1;
+  w.n_chunks = w.k_hi > w.k_lo ? (w.k_hi - w.k_base + tl.chunk - 1) / tl.chunk : 1;
   return true;
 }
-__device__ __forceinline__ bool ragged_work(const RaggedParams& p, int slot, int lane, RaggedWork& w) {
-  const int b = p.one_tile ? slot : ragged_slot(p, slot, lane);
+__device__ __forceinline__ bool ragged_work(const RaggedParams& p, const RaggedTiling& tl, int slot, int lane,
+                                            RaggedWork& w) {
+  const int b = tl.one_tile ? slot : ragged_slot(p, tl, slot, lane);
   if (b < 0) return false;
-  return ragged_work_at(p, b, p.one_tile ? 0 : (slot - (p.cu[b] / p.block_m + b)) * p.block_m, lane, w);
+  return ragged_work_at(p, tl, b, tl.one_tile ? 0 : (slot - (p.cu[b] / tl.block_m + b)) * tl.block_m, lane, w);
 }
 
 // The interval of the row of token t0 + i.
@@ -161,14 +171,14 @@ __device__ __forceinline__ float ragged_score(const RaggedParams& p, float s, fl
 
 #define GQA_CBAR() asm volatile("bar.sync 1, %0;" ::"n"(CT) : "memory")  // the compute warps
 
-// Template parameters as gqa_stream_kernel's: RG row groups of 16, FP8 = e4m3 caches
-// (HD 128, both MMAs in f16), NT = at most 8 packed rows, MMAs transposed. The scores and
-// the accumulators are fp32; P is rounded to the values' 16-bit type for its MMA, as the
-// dense kernels round it (relative error 2^-9, as large as the output's own rounding).
+// The compute warps of one streaming CTA, for tiles of up to 16 RG packed rows. Template
+// parameters as gqa_stream_kernel's: FP8 = e4m3 caches (HD 128, both MMAs in f16), NT = at
+// most 8 rows, MMAs transposed. The scores and the accumulators are fp32; P is rounded to
+// the values' 16-bit type for its MMA, as the dense kernels round it (relative error
+// 2^-9, as large as the output's own rounding).
 template <int HD, bool BF16, int RG, bool FP8, bool NT>
-__global__ void __launch_bounds__(288, 1)
-    gqa_ragged_stream_kernel(const RaggedParams p, const __grid_constant__ CUtensorMap kmap,
-                             const __grid_constant__ CUtensorMap vmap) {
+__device__ __forceinline__ void ragged_stream_compute(const RaggedParams& p, const RaggedWork& w, uint8_t* smem, uint32_t base,
+                                                      int k_begin, int k_end, int n_stages, int unit, int split, int kvh) {
   static_assert(!FP8 || HD == 128, "fp8 K/V rows are 128 bytes");
   static_assert(!NT || RG == 1, "the transposed form is the one-row-group kernel");
   using Cfg = StreamCfg<FP8 ? 64 : HD>;
@@ -181,92 +191,14 @@ __global__ void __launch_bounds__(288, 1)
   constexpr int NKS = HD / 16;
   constexpr int CT = NW * 32;
   constexpr int NACC = NT ? HD / 16 : NDB;
-
-  extern __shared__ uint8_t smem_raw[];
-  const uint32_t raw_base = smem_u32(smem_raw);
-  const uint32_t base = (raw_base + 1023u) & ~1023u;
-  uint8_t* const smem = smem_raw + (base - raw_base);
   const uint32_t bar_full = base + Cfg::kRingBytes;
   const uint32_t bar_empty = bar_full + Cfg::kStages * 8;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + Cfg::kRingBytes + Cfg::kBarBytes);
   int* last_flag = reinterpret_cast<int*>(smem + Cfg::kRingBytes + Cfg::kBarBytes + 4);
-
+  const RaggedTiling& tl = p.stream;
   const int tid = threadIdx.x;
   const int warp = tid >> 5;
   const int lane = tid & 31;
-  const int split = blockIdx.x % p.nsplit;
-  const int unit = blockIdx.x / p.nsplit;
-  const int kvh = unit % p.hkv;
-  const int slot_id = unit / p.hkv;
-
-  if (tid == CT) {
-    for (int s = 0; s < Cfg::kStages; ++s) {
-      mbar_init(bar_full + 8 * s, 1);
-      mbar_init(bar_empty + 8 * s, NW);
-    }
-    *abort_flag = 0;
-    fence_mbar_init();
-    fence_proxy_async_smem();
-    tma_prefetch_desc(&kmap);
-    tma_prefetch_desc(&vmap);
-  }
-  pdl_wait();
-  pdl_trigger();
-  RaggedWork w;
-  if (!ragged_work(p, slot_id, lane, w)) return;  // the same answer in every warp
-  if (split >= w.n_chunks) return;
-  const int k_begin = w.k_base + split * p.chunk;
-  const int k_end = min(k_begin + p.chunk, w.k_hi);
-  const int n_stages = (w.k_hi > w.k_lo) ? (k_end - k_begin + Cfg::kBN - 1) / Cfg::kBN : 0;
-  __syncthreads();
-
-  if (warp == NW) {
-    // ---------------------------------------------------------------- producer
-    // Lane i brings box i / NSUB, 64 values of d at i % NSUB, of each stage; its block is
-    // looked up before the stage's slot is waited for. A table entry outside the cache
-    // gives zeros (TMA's fill).
-    constexpr int NSUB = Cfg::kNSub;
-    const int box = p.box;
-    const int nbox_full = Cfg::kBN / box;
-    const uint32_t box_bytes = (uint32_t)box * 128u;
-    const int* row_bt = p.block_table + (int64_t)w.b * p.bt_stride;
-    const int mask = (1 << p.block_shift) - 1;
-    const int my_box = lane / NSUB, my_sub = lane % NSUB;
-    bool ok = true;
-    int t = 0;
-    for (; t < n_stages; ++t) {
-      const int slot = t % Cfg::kStages;
-      const uint32_t full = bar_full + 8 * slot;
-      const int key0 = k_begin + t * Cfg::kBN;
-      const int nbox = (min(Cfg::kBN, k_end - key0) + box - 1) / box;
-      const int key = key0 + my_box * box;
-      int pb = 0;
-      if (my_box < nbox) pb = row_bt[key >> p.block_shift];
-      if (t >= Cfg::kStages) {
-        ok = mbar_wait(bar_empty + 8 * slot, (t / Cfg::kStages - 1) & 1, abort_flag, 111);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-      }
-      if (withheld_load(t)) continue;
-      if (lane == 0) mbar_arrive_expect_tx(full, (uint32_t)nbox * 2u * NSUB * box_bytes);
-      __syncwarp();
-      if (my_box < nbox && my_box < nbox_full) {
-        const uint32_t o = base + slot * Cfg::kStageBytes + my_sub * Cfg::kSubBytes + my_box * box_bytes;
-        tma_load_4d(o, &kmap, full, my_sub * 64, kvh, key & mask, pb);
-        tma_load_4d(o + Cfg::kTileBytes, &vmap, full, my_sub * 64, kvh, key & mask, pb);
-      }
-    }
-    // On abort, let the loads already issued land before the CTA exits.
-    if (t < n_stages && lane == 0) {
-      for (int u = max(0, t - Cfg::kStages); u < t; ++u) {
-        volatile int dummy = 0;
-        if (!withheld_load(u)) mbar_wait(bar_full + 8 * (u % Cfg::kStages), (u / Cfg::kStages) & 1, &dummy, 112);
-      }
-    }
-    return;
-  }
-
-  // ------------------------------------------------------------------- compute
   const int rg = warp % RG;
   const int ks = warp / RG;
   const int gr = lane >> 2;
@@ -682,23 +614,23 @@ __global__ void __launch_bounds__(288, 1)
   }
 
   // ---- publish this chunk's partial; the tile's last CTA combines them in chunk order.
-  const int64_t ubase = (int64_t)unit * p.nsplit * p.rows;
-  const int64_t wbase = ubase + (int64_t)split * p.rows;
+  const int64_t ubase = (int64_t)unit * tl.nsplit * tl.rows;
+  const int64_t wbase = ubase + (int64_t)split * tl.rows;
   for (int idx = tid; idx < n_valid * per_row; idx += CT) {
     const int r = idx / per_row, d = (idx - r * per_row) * 4;
     const RowMerge mr = merge_row(r, d);
-    __stcg(reinterpret_cast<float4*>(p.ws_acc + (wbase + r) * HD + d), mr.a);
+    __stcg(reinterpret_cast<float4*>(tl.ws_acc + (wbase + r) * HD + d), mr.a);
     if (d == 0) {
-      __stcg(p.ws_m + wbase + r, mr.M);
-      __stcg(p.ws_l + wbase + r, mr.L);
+      __stcg(tl.ws_m + wbase + r, mr.M);
+      __stcg(tl.ws_l + wbase + r, mr.L);
     }
   }
   GQA_CBAR();
   if (tid == 0) {
     unsigned ticket;
-    asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(ticket) : "l"(p.ws_cnt + unit) : "memory");
+    asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(ticket) : "l"(tl.ws_cnt + unit) : "memory");
     *last_flag = (ticket == (unsigned)(w.n_chunks - 1)) ? 1 : 0;
-    if (*last_flag) p.ws_cnt[unit] = 0u;
+    if (*last_flag) tl.ws_cnt[unit] = 0u;
   }
   GQA_CBAR();
   if (!*last_flag) return;
@@ -707,8 +639,8 @@ __global__ void __launch_bounds__(288, 1)
   float* sm_l = sm_m + nc * n_valid;
   for (int i = tid; i < nc * n_valid; i += CT) {
     const int s2 = i / n_valid, r = i - s2 * n_valid;
-    sm_m[i] = __ldcg(p.ws_m + ubase + (int64_t)s2 * p.rows + r);
-    sm_l[i] = __ldcg(p.ws_l + ubase + (int64_t)s2 * p.rows + r);
+    sm_m[i] = __ldcg(tl.ws_m + ubase + (int64_t)s2 * tl.rows + r);
+    sm_l[i] = __ldcg(tl.ws_l + ubase + (int64_t)s2 * tl.rows + r);
   }
   GQA_CBAR();
   for (int idx = tid; idx < n_valid * per_row; idx += CT) {
@@ -723,7 +655,7 @@ __global__ void __launch_bounds__(288, 1)
       float4 v[kBatch];
 #pragma unroll
       for (int u = 0; u < kBatch; ++u)
-        v[u] = __ldcg(reinterpret_cast<const float4*>(p.ws_acc + (ubase + (int64_t)min(s0 + u, nc - 1) * p.rows + r) * HD + d));
+        v[u] = __ldcg(reinterpret_cast<const float4*>(tl.ws_acc + (ubase + (int64_t)min(s0 + u, nc - 1) * tl.rows + r) * HD + d));
 #pragma unroll
       for (int u = 0; u < kBatch; ++u) {
         if (s0 + u < nc) {
@@ -741,5 +673,117 @@ __global__ void __launch_bounds__(288, 1)
 }
 
 #undef GQA_CBAR
+
+// One CTA of the streaming form: at least 288 threads, warps 0-7 compute, warp 8 loads,
+// any others only keep the barrier company. The tile's rows pick the compute form.
+template <int HD, bool BF16, bool FP8>
+__device__ __forceinline__ void ragged_stream_cta(const RaggedParams& p, const CUtensorMap* kmap, const CUtensorMap* vmap,
+                                                  unsigned cta) {
+  using Cfg = StreamCfg<FP8 ? 64 : HD>;
+  constexpr int NW = Cfg::kWarps;
+  constexpr int CT = NW * 32;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_base = smem_u32(smem_raw);
+  const uint32_t base = (raw_base + 1023u) & ~1023u;
+  uint8_t* const smem = smem_raw + (base - raw_base);
+  const uint32_t bar_full = base + Cfg::kRingBytes;
+  const uint32_t bar_empty = bar_full + Cfg::kStages * 8;
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + Cfg::kRingBytes + Cfg::kBarBytes);
+
+  const RaggedTiling& tl = p.stream;
+  const int tid = threadIdx.x;
+  const int warp = tid >> 5;
+  const int lane = tid & 31;
+  const int split = (int)(cta % (unsigned)tl.nsplit);
+  const int unit = (int)(cta / (unsigned)tl.nsplit);
+  const int kvh = unit % p.hkv;
+  const int slot_id = unit / p.hkv;
+  if (tid == CT) {
+    for (int s = 0; s < Cfg::kStages; ++s) {
+      mbar_init(bar_full + 8 * s, 1);
+      mbar_init(bar_empty + 8 * s, NW);
+    }
+    *abort_flag = 0;
+    fence_mbar_init();
+    fence_proxy_async_smem();
+    tma_prefetch_desc(kmap);
+    tma_prefetch_desc(vmap);
+  }
+  pdl_wait();
+  pdl_trigger();
+  RaggedWork w;
+  if (!ragged_work(p, tl, slot_id, lane, w)) return;  // the same answer in every warp
+  if (split >= w.n_chunks) return;
+  const int k_begin = w.k_base + split * tl.chunk;
+  const int k_end = min(k_begin + tl.chunk, w.k_hi);
+  const int n_stages = (w.k_hi > w.k_lo) ? (k_end - k_begin + Cfg::kBN - 1) / Cfg::kBN : 0;
+  __syncthreads();
+
+  if (warp == NW) {
+    // ---------------------------------------------------------------- producer
+    // Lane i brings box i / NSUB, 64 values of d at i % NSUB, of each stage; its block is
+    // looked up before the stage's slot is waited for. A table entry outside the cache
+    // gives zeros (TMA's fill).
+    constexpr int NSUB = Cfg::kNSub;
+    const int box = p.box;
+    const int nbox_full = Cfg::kBN / box;
+    const uint32_t box_bytes = (uint32_t)box * 128u;
+    const int* row_bt = p.block_table + (int64_t)w.b * p.bt_stride;
+    const int mask = (1 << p.block_shift) - 1;
+    const int my_box = lane / NSUB, my_sub = lane % NSUB;
+    bool ok = true;
+    int t = 0;
+    for (; t < n_stages; ++t) {
+      const int slot = t % Cfg::kStages;
+      const uint32_t full = bar_full + 8 * slot;
+      const int key0 = k_begin + t * Cfg::kBN;
+      const int nbox = (min(Cfg::kBN, k_end - key0) + box - 1) / box;
+      const int key = key0 + my_box * box;
+      int pb = 0;
+      if (my_box < nbox) pb = row_bt[key >> p.block_shift];
+      if (t >= Cfg::kStages) {
+        ok = mbar_wait(bar_empty + 8 * slot, (t / Cfg::kStages - 1) & 1, abort_flag, 111);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+      }
+      if (withheld_load(t)) continue;
+      if (lane == 0) mbar_arrive_expect_tx(full, (uint32_t)nbox * 2u * NSUB * box_bytes);
+      __syncwarp();
+      if (my_box < nbox && my_box < nbox_full) {
+        const uint32_t o = base + slot * Cfg::kStageBytes + my_sub * Cfg::kSubBytes + my_box * box_bytes;
+        tma_load_4d(o, kmap, full, my_sub * 64, kvh, key & mask, pb);
+        tma_load_4d(o + Cfg::kTileBytes, vmap, full, my_sub * 64, kvh, key & mask, pb);
+      }
+    }
+    // On abort, let the loads already issued land before the CTA exits.
+    if (t < n_stages && lane == 0) {
+      for (int u = max(0, t - Cfg::kStages); u < t; ++u) {
+        volatile int dummy = 0;
+        if (!withheld_load(u)) mbar_wait(bar_full + 8 * (u % Cfg::kStages), (u / Cfg::kStages) & 1, &dummy, 112);
+      }
+    }
+    return;
+  }
+  if (warp > NW) return;
+  const int n_valid = w.nq * p.group;
+  if (n_valid <= 8) {
+    ragged_stream_compute<HD, BF16, 1, FP8, true>(p, w, smem, base, k_begin, k_end, n_stages, unit, split, kvh);
+  } else if (n_valid <= 16) {
+    ragged_stream_compute<HD, BF16, 1, FP8, false>(p, w, smem, base, k_begin, k_end, n_stages, unit, split, kvh);
+  } else if constexpr (FP8) {  // 16-bit tiles have at most kRaggedStreamRows rows
+    if (n_valid <= 32)
+      ragged_stream_compute<HD, BF16, 2, FP8, false>(p, w, smem, base, k_begin, k_end, n_stages, unit, split, kvh);
+    else
+      ragged_stream_compute<HD, BF16, 4, FP8, false>(p, w, smem, base, k_begin, k_end, n_stages, unit, split, kvh);
+  }
+}
+
+// Steps whose requests all stream.
+template <int HD, bool BF16, bool FP8>
+__global__ void __launch_bounds__(288, 1)
+    gqa_ragged_stream_kernel(const __grid_constant__ RaggedParams p, const __grid_constant__ CUtensorMap kmap,
+                             const __grid_constant__ CUtensorMap vmap) {
+  ragged_stream_cta<HD, BF16, FP8>(p, &kmap, &vmap, blockIdx.x);
+}
 
 }  // namespace gqa

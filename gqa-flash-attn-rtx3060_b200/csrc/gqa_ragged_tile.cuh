@@ -1,6 +1,6 @@
 // tcgen05 / TMEM / TMA form of the ragged attention (gqa_ragged.cuh has the masks, the
-// scores and the work of a tile): requests of more than 64 packed rows, i.e. prompts and
-// chunks of them. The pipeline is the dense prefill kernel's (gqa_prefill.cuh): one CTA
+// scores and the work of a tile): requests of more than kRaggedStreamRows packed rows, i.e.
+// prompts, chunks of them and most drafts. The pipeline is the dense prefill kernel's (gqa_prefill.cuh): one CTA
 // owns two 128-row query tiles of one (request, kv head), a TMA warp streams 128-key
 // tiles of K and V from the paged cache, one thread issues the UMMAs
 //   S_i = Q_i K_j^T (f32 in TMEM),   O_i += P_i V_j (P from TMEM)
@@ -13,6 +13,10 @@
 //    [lo, hi) in it. A row's running maximum starts at a finite -3e38, so that tiles
 //    where it sees nothing add exp2(-inf) = 0; rows that saw nothing end with l = 0.
 //  - Scores may be capped or biased (MOD), see below.
+//  - A tile whose tokens fit the first query tile runs solo: the two warpgroups take the
+//    even and the odd key tiles of the same 128 rows (own S, O, maximum and sum) and merge
+//    at the end. So a request of few rows keeps the tensor core and both warpgroups busy,
+//    and with 256 keys in flight a CTA streams as fast as HBM delivers.
 //  - O leaves through shared memory with ordinary 16-byte stores, since a tile may end
 //    where the next request's rows begin.
 //
@@ -67,18 +71,30 @@ __device__ __forceinline__ float max3_abs(float a, float b, float c) {
 template <int HD>
 struct RaggedTileCfg : PrefillCfg<HD> {
   using Base = PrefillCfg<HD>;
+  // A solo tile's second Q buffer is one more K/V slot, in front of the ring's first.
+  static constexpr int kMaxSlots = Base::kSlots + 1;
+  static constexpr int kNumBars = 2 + 2 * kMaxSlots + 2 + 2 * Base::kPParts + 2 + 1;
+  static constexpr int kMiscOff = Base::kBarOff + kNumBars * 8;
   // tmem base, abort flag, last-CTA flag, work item, warp sums of the scan
-  static constexpr int kWorkOff = Base::kMiscOff + 16;
-  static constexpr int kSmemBytes = kWorkOff + 64 + 64 + 1024;
+  static constexpr int kWorkOff = kMiscOff + 16;
+  static constexpr int kTileSmem = kWorkOff + 64 + 64 + 1024;
+  static constexpr int kSmemBytes = kTileSmem > StreamCfg<HD>::kSmemBytes ? kTileSmem : StreamCfg<HD>::kSmemBytes;
 };
 
 template <int HD, bool BF16, int MOD>
 __global__ void __launch_bounds__(384, 1)
-    gqa_ragged_tile_kernel(const RaggedParams p, const __grid_constant__ CUtensorMap qmap,
+    gqa_ragged_tile_kernel(const __grid_constant__ RaggedParams p, const __grid_constant__ CUtensorMap qmap,
                            const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
+  // The step's short requests stream in the grid's last CTAs: they fill the SMs as the
+  // tiles run out.
+  if (blockIdx.x >= p.tile_ctas) {
+    ragged_stream_cta<HD, BF16, false>(p, &kmap, &vmap, blockIdx.x - p.tile_ctas);
+    return;
+  }
   using Cfg = RaggedTileCfg<HD>;
+  const RaggedTiling& tl = p.tile;
   constexpr int NSUB = Cfg::kNSub;
-  constexpr int SLOTS = Cfg::kSlots;
+  constexpr int SLOTS = Cfg::kMaxSlots;  // barriers; a pair uses one slot fewer
   constexpr int BN = Cfg::kBN;
 
   extern __shared__ uint8_t smem_raw[];
@@ -115,11 +131,11 @@ __global__ void __launch_bounds__(384, 1)
   const int tid = threadIdx.x;
   const int warp = tid >> 5;
   const int lane = tid & 31;
-  const unsigned n_inner = (unsigned)(p.hkv * p.nsplit);
+  const unsigned n_inner = (unsigned)(p.hkv * tl.nsplit);
   const int tile_id = (int)(blockIdx.x / n_inner);
-  const int kvh = (int)((blockIdx.x % n_inner) / (unsigned)p.nsplit);
-  const int split = (int)(blockIdx.x % (unsigned)p.nsplit);
-  const int bm = p.block_m >> 1;  // tokens per query tile
+  const int kvh = (int)((blockIdx.x % n_inner) / (unsigned)tl.nsplit);
+  const int split = (int)(blockIdx.x % (unsigned)tl.nsplit);
+  const int bm = tl.block_m >> 1;  // tokens per query tile
 
   if (tid == 0) {
     mbar_init(bar_q_full, 1);
@@ -150,8 +166,8 @@ __global__ void __launch_bounds__(384, 1)
       if (b >= p.n) return 0;
       const int first = p.cu[b];
       const int qn = min(p.cu[b + 1], p.num_tokens) - first;
-      if (first < 0 || qn <= 0 || (int64_t)qn * p.group < p.min_rows) return 0;
-      return (qn + p.block_m - 1) / p.block_m;
+      if (first < 0 || qn <= 0 || (int64_t)qn * p.group < tl.min_rows) return 0;
+      return (qn + tl.block_m - 1) / tl.block_m;
     };
     const int rounds = (p.n + 383) / 384;
     const int mine = tiles_of(tid);
@@ -194,9 +210,9 @@ __global__ void __launch_bounds__(384, 1)
   }
   if (warp == 0) {
     RaggedWork w;
-    const bool ok = ragged_work_at(p, work->found, work->local * p.block_m, lane, w);
+    const bool ok = ragged_work_at(p, tl, work->found, work->local * tl.block_m, lane, w);
     if (lane == 0) {
-      const int k_first = w.k_base + split * p.chunk;
+      const int k_first = w.k_base + split * tl.chunk;
       work->t0 = w.t0;
       work->nq = w.nq;
       work->off_m0 = w.off + w.m0;
@@ -205,13 +221,16 @@ __global__ void __launch_bounds__(384, 1)
       work->k_lo = w.k_lo;
       work->k_hi = w.k_hi;
       work->key0 = k_first;
-      work->nk = (ok && w.k_hi > w.k_lo) ? max(0, (min(k_first + p.chunk, w.k_hi) - k_first + BN - 1) / BN) : 0;
+      work->nk = (ok && w.k_hi > w.k_lo) ? max(0, (min(k_first + tl.chunk, w.k_hi) - k_first + BN - 1) / BN) : 0;
       work->n_chunks = ok ? w.n_chunks : 0;
-      work->unit = (int)(blockIdx.x / (unsigned)p.nsplit);
+      work->unit = (int)(blockIdx.x / (unsigned)tl.nsplit);
     }
   }
   __syncthreads();
   if (split >= work->n_chunks) return;  // the whole CTA, before TMEM
+  const bool solo = work->nq <= bm;
+  const int slots = solo ? SLOTS : SLOTS - 1;                          // ring slots in use,
+  const uint32_t kv_base = solo ? kv_smem0 - Cfg::kTileBytes : kv_smem0;  // the first of them
   if (warp == 8) {
     tmem_alloc(smem_u32(tmem_base_ptr), Cfg::kTmemCols);
     tmem_relinquish();
@@ -238,6 +257,7 @@ __global__ void __launch_bounds__(384, 1)
           const int hq0 = kvh * p.group, t0 = work->t0;
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
+            if (i == 1 && solo) break;
             mbar_arrive_expect_tx(bar_q_full + 8 * i, (uint32_t)(bm * p.group) * 128u * NSUB);
 #pragma unroll
             for (int s = 0; s < NSUB; ++s)
@@ -251,14 +271,13 @@ __global__ void __launch_bounds__(384, 1)
         const int k_hi = work->k_hi, key_first = work->key0 + my_box * box;
         const int* row_bt = p.block_table + (int64_t)work->b * p.bt_stride;
         const int mask = (1 << p.block_shift) - 1;
-        const uint32_t dst0 = kv_smem0 + my_sub * Cfg::kSubBytes + (uint32_t)(my_box * box) * 128u;
+        const uint32_t dst0 = kv_base + my_sub * Cfg::kSubBytes + (uint32_t)(my_box * box) * 128u;
         int t = 0;
         const int n_loads = 2 * nk;
         int pb = 0;
         bool ok = true;
+        int slot = 0, use = 0;
         for (; t < n_loads; ++t) {
-          const int slot = t % SLOTS;
-          const int use = t / SLOTS;
           const int key = key_first + (t >> 1) * BN;
           // Looked up once per tile (K loads; V reuses it), before the slot wait.
           if ((t & 1) == 0) pb = (loads && key < k_hi) ? row_bt[key >> p.block_shift] : p.num_blocks;
@@ -267,16 +286,22 @@ __global__ void __launch_bounds__(384, 1)
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
           }
-          if (withheld_load(t)) continue;
-          const uint32_t full = bar_kv_full + 8 * slot;
-          if (lane == 0) mbar_arrive_expect_tx(full, Cfg::kTileBytes);
-          __syncwarp();
-          if (loads) tma_load_4d(dst0 + slot * Cfg::kTileBytes, (t & 1) ? &vmap : &kmap, full, my_sub * 64, kvh, key & mask, pb);
+          if (!withheld_load(t)) {
+            const uint32_t full = bar_kv_full + 8 * slot;
+            if (lane == 0) mbar_arrive_expect_tx(full, Cfg::kTileBytes);
+            __syncwarp();
+            if (loads)
+              tma_load_4d(dst0 + slot * Cfg::kTileBytes, (t & 1) ? &vmap : &kmap, full, my_sub * 64, kvh, key & mask, pb);
+          }
+          if (++slot == slots) {
+            slot = 0;
+            ++use;
+          }
         }
         if (t < n_loads && lane == 0) {  // aborted: let in-flight loads land before teardown
           volatile int dummy = 0;
-          for (int u = max(0, t - SLOTS); u < t; ++u)
-            if (!withheld_load(u)) mbar_wait(bar_kv_full + 8 * (u % SLOTS), (u / SLOTS) & 1, &dummy, 122);
+          for (int u = max(0, t - slots); u < t; ++u)
+            if (!withheld_load(u)) mbar_wait(bar_kv_full + 8 * (u % slots), (u / slots) & 1, &dummy, 122);
         }
       }
       __syncwarp();
@@ -288,8 +313,8 @@ __global__ void __launch_bounds__(384, 1)
         constexpr uint32_t idesc_pv = make_idesc_f16(128, HD, BF16, true);
         auto issue_qk = [&](int i, int slot) {
           const uint32_t tS = tmem_base + (i ? Cfg::kColS1 : Cfg::kColS0);
-          const uint32_t qa = q_smem0 + i * Cfg::kTileBytes;
-          const uint32_t kb = kv_smem0 + slot * Cfg::kTileBytes;
+          const uint32_t qa = q_smem0 + (solo ? 0 : i) * Cfg::kTileBytes;
+          const uint32_t kb = kv_base + slot * Cfg::kTileBytes;
 #pragma unroll
           for (int k = 0; k < HD / 16; ++k) {
             const uint32_t o = (k >> 2) * Cfg::kSubBytes + (k & 3) * 32;
@@ -299,7 +324,7 @@ __global__ void __launch_bounds__(384, 1)
         auto issue_pv = [&](int i, int slot, int h, bool acc) {
           const uint32_t tS = tmem_base + (i ? Cfg::kColS1 : Cfg::kColS0);
           const uint32_t tO = tmem_base + (i ? Cfg::kColO1 : Cfg::kColO0);
-          const uint32_t vb = kv_smem0 + slot * Cfg::kTileBytes;
+          const uint32_t vb = kv_base + slot * Cfg::kTileBytes;
           constexpr int kPerPart = BN / 16 / Cfg::kPParts;
 #pragma unroll
           for (int kk = 0; kk < kPerPart; ++kk) {
@@ -308,9 +333,10 @@ __global__ void __launch_bounds__(384, 1)
                     (acc || k > 0) ? 1u : 0u);
           }
         };
-        bool ok = mbar_wait(bar_q_full, 0, abort_flag, 130) && mbar_wait(bar_q_full + 8, 0, abort_flag, 131) &&
-                  mbar_wait(bar_kv_full, 0, abort_flag, 132);
-        if (ok) {
+        bool ok = mbar_wait(bar_q_full, 0, abort_flag, 130) &&
+                  (solo || mbar_wait(bar_q_full + 8, 0, abort_flag, 131)) && mbar_wait(bar_kv_full, 0, abort_flag, 132);
+        if (ok && !solo) {
+          constexpr int SLOTS = Cfg::kSlots;
           tc_fence_after();
           issue_qk(0, 0);
           umma_commit(bar_s_full);
@@ -359,6 +385,38 @@ __global__ void __launch_bounds__(384, 1)
             }
           }
         }
+        if (ok && solo) {
+          // Key tile j belongs to warpgroup j & 1, which owns S_i and O_i, i = j & 1. Loads
+          // are K_0 V_0 K_1 V_1 ...; QK_0 and QK_1 go first, then PV_j and QK_{j + 2}.
+          auto qk = [&](int j) -> bool {
+            const int t = 2 * j, sl = t % SLOTS;
+            if (!mbar_wait(bar_kv_full + 8 * sl, (t / SLOTS) & 1, abort_flag, 135)) return false;
+            tc_fence_after();
+            issue_qk(j & 1, sl);
+            umma_commit(bar_s_full + 8 * (j & 1));
+            umma_commit(bar_kv_empty + 8 * sl);  // K_j consumed
+            return true;
+          };
+          bool go = qk(0) && (nk < 2 || qk(1));
+          for (int j = 0; j < nk && go; ++j) {
+            const int i = j & 1, t = 2 * j + 1, sl = t % SLOTS;
+            go = mbar_wait(bar_kv_full + 8 * sl, (t / SLOTS) & 1, abort_flag, 133);
+#pragma unroll
+            for (int h = 0; h < Cfg::kPParts && go; ++h) {
+              go = mbar_wait(bar_p_full + 8 * (Cfg::kPParts * i + h), (j >> 1) & 1, abort_flag, h ? 138 : 134);
+              if (go) {
+                tc_fence_after();
+                issue_pv(i, sl, h, h > 0 || j > 1);
+              }
+            }
+            if (!go) break;
+            umma_commit(bar_kv_empty + 8 * sl);  // V_j consumed
+            if (j + 2 < nk)
+              go = qk(j + 2);
+            else
+              umma_commit(bar_o_final + 8 * i);
+          }
+        }
         // Drain: every MMA issued above completes before TMEM is released.
         umma_commit(bar_mma_done);
         volatile int dummy = 0;
@@ -383,7 +441,7 @@ __global__ void __launch_bounds__(384, 1)
     int lo_rel = 0, hi_rel = 0;
     float dist0 = 0.f, slope = 0.f;
     {
-      const int m = row / p.group, i = wg * bm + m;
+      const int m = row / p.group, i = (solo ? 0 : wg * bm) + m;
       if (m < bm && i < work->nq) {
         RaggedWork w;
         w.b = work->b;
@@ -404,9 +462,16 @@ __global__ void __launch_bounds__(384, 1)
     float m_run = -3.0e38f;
     float l_run = 0.f;
     bool ok = true;
+    // This warpgroup's key tiles: all of them, or of a solo tile every other one. Step n
+    // is key tile j.
     const int nk = work->nk;
-    for (int j = 0; j < nk; ++j) {
-      ok = mbar_wait(s_full, j & 1, abort_flag, 140 + wg);
+    const int n_steps = solo ? (nk + 1 - wg) >> 1 : nk;
+    // Rows that see nothing at all (idle rows, rows past the tile's tokens) do no softmax: a warp
+    // of them only keeps the barriers going. What is left in its rows of P reaches its own rows of O alone.
+    const bool idle_warp = __all_sync(0xffffffffu, hi_rel <= lo_rel);
+    for (int n = 0; n < n_steps; ++n) {
+      const int j = solo ? 2 * n + wg : n;
+      ok = mbar_wait(s_full, n & 1, abort_flag, 140 + wg);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc_fence_after();
@@ -417,11 +482,11 @@ __global__ void __launch_bounds__(384, 1)
         const int key = work->key0 + j * BN;
         if (key + BN > work->k_hi || key < work->k_lo) {
           const int tv = 2 * j + 1;
-          ok = mbar_wait(bar_kv_full + 8 * (tv % SLOTS), (tv / SLOTS) & 1, abort_flag, 144 + wg);
+          ok = mbar_wait(bar_kv_full + 8 * (tv % slots), (tv / slots) & 1, abort_flag, 144 + wg);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           if (key + row >= work->k_hi || key + row < work->k_lo) {
-            const uint32_t vrow = kv_smem0 + (tv % SLOTS) * Cfg::kTileBytes + row * 128;
+            const uint32_t vrow = kv_base + (tv % slots) * Cfg::kTileBytes + row * 128;
 #pragma unroll
             for (int c = 0; c < NSUB * 8; ++c)
               asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(vrow + (c >> 3) * Cfg::kSubBytes +
@@ -431,6 +496,11 @@ __global__ void __launch_bounds__(384, 1)
           }
           fence_proxy_async_smem();
         }
+      }
+      if (idle_warp) {
+#pragma unroll
+        for (int h = 0; h < Cfg::kPParts; ++h) mbar_arrive(p_full + 8 * h);
+        continue;
       }
       const int rem = hi_rel - j * BN;   // columns [low, rem) are visible
       const int low = lo_rel - j * BN;
@@ -496,7 +566,7 @@ __global__ void __launch_bounds__(384, 1)
         mx = mx == -INFINITY ? mx : fmaf(-2.f * p.cap_out, fast_rcp(1.f + fast_exp2(mx * p.cap_in)), p.cap_out);
       const float m_new = fmaxf(m_run, mx);
       const bool need = m_new > m_run + 8.0f;
-      if (j > 0 && __any_sync(0xffffffffu, need)) {
+      if (n > 0 && __any_sync(0xffffffffu, need)) {
         const float alpha = need ? fast_exp2(m_run - m_new) : 1.0f;
 #pragma unroll
         for (int c = 0; c < HD / 32; ++c) {
@@ -573,26 +643,76 @@ __global__ void __launch_bounds__(384, 1)
     }
 
     // ---- epilogue
-    bool have_o = ok && nk > 0;
+    bool have_o = ok && n_steps > 0;
     if (have_o) {
       have_o = mbar_wait(bar_o_final + 8 * wg, 0, abort_flag, 142 + wg);
       have_o = __all_sync(0xffffffffu, have_o);
     }
     if (have_o) tc_fence_after();
 
+    if (solo && nk > 0) {
+      // Both warpgroups' MMAs are done after the first barrier, so the ring and Q are free:
+      // the odd key tiles' O, m and l go through shared memory ([d][row] floats, rows
+      // fastest) into the even ones', whose warpgroup goes on alone.
+      float* const o1 = reinterpret_cast<float*>(smem + Cfg::kKVOff) + row;
+      float* const ml1 = reinterpret_cast<float*>(smem + Cfg::kKVOff + HD * 128 * 4) + row;
+      asm volatile("bar.sync 3, 256;" ::: "memory");
+      if (wg == 1) {
+#pragma unroll
+        for (int c = 0; c < HD / 32; ++c) {
+          uint32_t orr[32];
+          if (have_o) {
+            tmem_ld32(tO + c * 32, orr);
+            tmem_wait_ld();
+            reg_fence(orr);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) orr[e] = 0u;
+          }
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o1[(c * 32 + e) * 128] = __uint_as_float(orr[e]);
+        }
+        ml1[0] = m_run;
+        ml1[128] = l_run;
+      }
+      asm volatile("bar.sync 3, 256;" ::: "memory");
+      if (wg == 0 && have_o) {
+        const float M1 = ml1[0], Mx = fmaxf(m_run, M1);
+        const float w0 = fast_exp2(m_run - Mx), w1 = fast_exp2(M1 - Mx);
+        l_run = w0 * l_run + w1 * ml1[128];
+        m_run = Mx;
+#pragma unroll
+        for (int c = 0; c < HD / 32; ++c) {
+          uint32_t orr[32];
+          tmem_ld32(tO + c * 32, orr);
+          tmem_wait_ld();
+          reg_fence(orr);
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            orr[e] = __float_as_uint(w0 * __uint_as_float(orr[e]) + w1 * o1[(c * 32 + e) * 128]);
+          tmem_st32(tO + c * 32, orr);
+        }
+        tmem_wait_st();
+      }
+    }
+    const bool merged_away = solo && wg == 1;  // nothing left to write
+
     const int n_chunks = work->n_chunks, unit = work->unit;
     float L = l_run, M = m_run;
-    bool store = true;
+    bool store = !merged_away;
     const int prow = wg * 128 + row;  // row of the pair's 256 packed rows
-    const int64_t pbase = (int64_t)unit * p.nsplit * 256 + prow;
+    const int64_t pbase = (int64_t)unit * tl.nsplit * 256 + prow;
     if (n_chunks > 1) {
       // Publish this chunk's partial, m, l [split][256 rows] and acc [split][d][256 rows];
       // the tile's last CTA (ticket) folds them in chunk order.
-      __stcg(p.ws_m + pbase + (int64_t)split * 256, m_run);
-      __stcg(p.ws_l + pbase + (int64_t)split * 256, l_run);
-      float* acc_own = p.ws_acc + ((int64_t)unit * p.nsplit + split) * HD * 256 + prow;
+      if (!merged_away) {
+        __stcg(tl.ws_m + pbase + (int64_t)split * 256, m_run);
+        __stcg(tl.ws_l + pbase + (int64_t)split * 256, l_run);
+      }
+      float* acc_own = tl.ws_acc + ((int64_t)unit * tl.nsplit + split) * HD * 256 + prow;
 #pragma unroll
       for (int c = 0; c < HD / 32; ++c) {
+        if (merged_away) break;
         uint32_t orr[32];
         if (have_o) {
           tmem_ld32(tO + c * 32, orr);
@@ -609,18 +729,18 @@ __global__ void __launch_bounds__(384, 1)
       uint32_t* last_slot = tmem_base_ptr + 2;
       if (tid == 0) {
         unsigned ticket;
-        asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(ticket) : "l"(p.ws_cnt + unit) : "memory");
+        asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(ticket) : "l"(tl.ws_cnt + unit) : "memory");
         const bool last = ticket == (unsigned)(n_chunks - 1);
         *last_slot = last ? 1u : 0u;
-        if (last) p.ws_cnt[unit] = 0u;
+        if (last) tl.ws_cnt[unit] = 0u;
       }
       asm volatile("bar.sync 3, 256;" ::: "memory");
-      store = *last_slot != 0;
+      store = *last_slot != 0 && !merged_away;
       if (store) {
         for (int s0 = 0; s0 < n_chunks; s0 += 4) {
           float mv[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) mv[i] = __ldcg(p.ws_m + pbase + (int64_t)min(s0 + i, n_chunks - 1) * 256);
+          for (int i = 0; i < 4; ++i) mv[i] = __ldcg(tl.ws_m + pbase + (int64_t)min(s0 + i, n_chunks - 1) * 256);
 #pragma unroll
           for (int i = 0; i < 4; ++i) M = fmaxf(M, mv[i]);
         }
@@ -630,8 +750,8 @@ __global__ void __launch_bounds__(384, 1)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int64_t o2 = pbase + (int64_t)min(s0 + i, n_chunks - 1) * 256;
-            mv[i] = __ldcg(p.ws_m + o2);
-            lv[i] = __ldcg(p.ws_l + o2);
+            mv[i] = __ldcg(tl.ws_m + o2);
+            lv[i] = __ldcg(tl.ws_l + o2);
           }
 #pragma unroll
           for (int i = 0; i < 4; ++i)
@@ -651,10 +771,10 @@ __global__ void __launch_bounds__(384, 1)
         for (int e = 0; e < 32; ++e) orr[e] = 0u;
         for (int s0 = 0; store && s0 < n_chunks; s0 += 2) {
           const int sa = s0, sb = min(s0 + 1, n_chunks - 1);
-          const float wa = fast_exp2(__ldcg(p.ws_m + pbase + (int64_t)sa * 256) - M);
-          const float wb = (s0 + 1 >= n_chunks) ? 0.f : fast_exp2(__ldcg(p.ws_m + pbase + (int64_t)sb * 256) - M);
-          const float* xa = p.ws_acc + ((int64_t)unit * p.nsplit + sa) * HD * 256 + prow + c * 32 * 256;
-          const float* xb = p.ws_acc + ((int64_t)unit * p.nsplit + sb) * HD * 256 + prow + c * 32 * 256;
+          const float wa = fast_exp2(__ldcg(tl.ws_m + pbase + (int64_t)sa * 256) - M);
+          const float wb = (s0 + 1 >= n_chunks) ? 0.f : fast_exp2(__ldcg(tl.ws_m + pbase + (int64_t)sb * 256) - M);
+          const float* xa = tl.ws_acc + ((int64_t)unit * tl.nsplit + sa) * HD * 256 + prow + c * 32 * 256;
+          const float* xb = tl.ws_acc + ((int64_t)unit * tl.nsplit + sb) * HD * 256 + prow + c * 32 * 256;
           float va[32], vb[32];
 #pragma unroll
           for (int e = 0; e < 32; ++e) {

@@ -12,35 +12,14 @@ namespace {
 constexpr int kServingCounters = 16384;
 
 template <int HD, bool BF, bool F8>
-cudaError_t launch_ragged_stream_hd(const RaggedParams& p, unsigned grid, const CUtensorMap& km, const CUtensorMap& vm,
-                                    cudaStream_t st) {
+cudaError_t launch_ragged_stream(const RaggedParams& p, unsigned grid, const CUtensorMap& km, const CUtensorMap& vm,
+                                 cudaStream_t st) {
   using Cfg = StreamCfg<F8 ? 64 : HD>;
-  if (p.rows <= 8)
-    return launch_pdl(gqa_ragged_stream_kernel<HD, BF, 1, F8, true>, grid, Cfg::kThreads, Cfg::kSmemBytes, st, p, km, vm);
-  if (p.rows <= 16)
-    return launch_pdl(gqa_ragged_stream_kernel<HD, BF, 1, F8, false>, grid, Cfg::kThreads, Cfg::kSmemBytes, st, p, km, vm);
-  if (p.rows <= 32)
-    return launch_pdl(gqa_ragged_stream_kernel<HD, BF, 2, F8, false>, grid, Cfg::kThreads, Cfg::kSmemBytes, st, p, km, vm);
-  return launch_pdl(gqa_ragged_stream_kernel<HD, BF, 4, F8, false>, grid, Cfg::kThreads, Cfg::kSmemBytes, st, p, km, vm);
-}
-
-cudaError_t prepare_ragged() {
-  cudaError_t e = cudaSuccess;
-  auto chk = [&](cudaError_t x) { if (x != cudaSuccess && e == cudaSuccess) e = x; };
-#define GQA_SET_RAGGED(HD, BF, F8)                                                                        \
-  chk(set_smem(gqa_ragged_stream_kernel<HD, BF, 1, F8, true>, StreamCfg<F8 ? 64 : HD>::kSmemBytes));      \
-  chk(set_smem(gqa_ragged_stream_kernel<HD, BF, 1, F8, false>, StreamCfg<F8 ? 64 : HD>::kSmemBytes));     \
-  chk(set_smem(gqa_ragged_stream_kernel<HD, BF, 2, F8, false>, StreamCfg<F8 ? 64 : HD>::kSmemBytes));     \
-  chk(set_smem(gqa_ragged_stream_kernel<HD, BF, 4, F8, false>, StreamCfg<F8 ? 64 : HD>::kSmemBytes))
-  GQA_SET_RAGGED(128, true, false); GQA_SET_RAGGED(128, false, false);
-  GQA_SET_RAGGED(64, true, false); GQA_SET_RAGGED(64, false, false);
-  GQA_SET_RAGGED(128, true, true); GQA_SET_RAGGED(128, false, true);
-#undef GQA_SET_RAGGED
-  return e;
+  return launch_pdl(gqa_ragged_stream_kernel<HD, BF, F8>, grid, Cfg::kThreads, Cfg::kSmemBytes, st, p, km, vm);
 }
 
 template <int HD, bool BF>
-cudaError_t launch_ragged_tile_hd(const RaggedParams& p, unsigned grid, const CUtensorMap& qm, const CUtensorMap& km,
+cudaError_t launch_ragged_tile(const RaggedParams& p, unsigned grid, const CUtensorMap& qm, const CUtensorMap& km,
                                   const CUtensorMap& vm, cudaStream_t st) {
   using Cfg = RaggedTileCfg<HD>;
   if (p.alibi)
@@ -50,19 +29,23 @@ cudaError_t launch_ragged_tile_hd(const RaggedParams& p, unsigned grid, const CU
   return launch_pdl(gqa_ragged_tile_kernel<HD, BF, kRaggedPlain>, grid, Cfg::kThreads, Cfg::kSmemBytes, st, p, qm, km, vm);
 }
 
-// Shared memory opt-in, and the setmaxnreg split must fit the registers the launch holds.
-int prepare_ragged_tile() {
+// Shared memory opt-in, and the tcgen05 form's setmaxnreg split must fit the registers the launch holds.
+int prepare_ragged() {
   int rc = GQA_OK;
-  auto prep = [&](auto kernel, int smem) {
+  auto prep = [&](auto kernel, int smem, int regs) {
     if (set_smem(kernel, smem) != cudaSuccess) rc = rc ? rc : GQA_ERR_CUDA;
-    if (!rc) rc = check_reg_split(kernel, PrefillCfg<128>::kThreads, PrefillCfg<128>::kRegsNeeded);
+    if (!rc && regs) rc = check_reg_split(kernel, PrefillCfg<128>::kThreads, regs);
   };
-#define GQA_PREP_RAGGED(HD, BF)                                                           \
-  prep(gqa_ragged_tile_kernel<HD, BF, kRaggedPlain>, RaggedTileCfg<HD>::kSmemBytes);      \
-  prep(gqa_ragged_tile_kernel<HD, BF, kRaggedCap>, RaggedTileCfg<HD>::kSmemBytes);        \
-  prep(gqa_ragged_tile_kernel<HD, BF, kRaggedBias>, RaggedTileCfg<HD>::kSmemBytes)
+  constexpr int kRegs = PrefillCfg<128>::kRegsNeeded;
+#define GQA_PREP_RAGGED(HD, BF)                                                              \
+  prep(gqa_ragged_tile_kernel<HD, BF, kRaggedPlain>, RaggedTileCfg<HD>::kSmemBytes, kRegs);  \
+  prep(gqa_ragged_tile_kernel<HD, BF, kRaggedCap>, RaggedTileCfg<HD>::kSmemBytes, kRegs);    \
+  prep(gqa_ragged_tile_kernel<HD, BF, kRaggedBias>, RaggedTileCfg<HD>::kSmemBytes, kRegs);   \
+  prep(gqa_ragged_stream_kernel<HD, BF, false>, StreamCfg<HD>::kSmemBytes, 0)
   GQA_PREP_RAGGED(128, true); GQA_PREP_RAGGED(128, false); GQA_PREP_RAGGED(64, true); GQA_PREP_RAGGED(64, false);
 #undef GQA_PREP_RAGGED
+  prep(gqa_ragged_stream_kernel<128, true, true>, StreamCfg<64>::kSmemBytes, 0);
+  prep(gqa_ragged_stream_kernel<128, false, true>, StreamCfg<64>::kSmemBytes, 0);
   return rc;
 }
 
@@ -83,107 +66,115 @@ int check_ragged_shape(const gqa_ragged_args& a, RaggedShape* s) {
   return GQA_OK;
 }
 
+// The launch: the two forms' tilings and their CTAs.
 struct RaggedPlan {
-  int block_m, rows, one_tile, slots, nsplit, chunk;
+  RaggedTiling stream, tile;
+  int64_t stream_ctas, tile_ctas;
 };
 
-// Tiles of the streaming kernel, and its key split. Only bounds are known here, so the
-// chunk is chosen for the longest request; requests with fewer keys use fewer chunks.
-RaggedPlan plan_ragged_stream(const RaggedShape& s, int sm_count) {
-  RaggedPlan pl{};
-  pl.block_m = std::max(1, std::min(s.max_q, kStreamMaxRows / s.group));
-  pl.rows = s.group * pl.block_m;
-  pl.one_tile = s.max_q <= pl.block_m;
-  pl.slots = pl.one_tile ? s.n : s.tokens / pl.block_m + s.n;
-  const int64_t tiles = pl.one_tile ? std::min(s.n, s.tokens) : std::min(pl.slots, s.tokens);
-  const int64_t units = tiles * s.hkv;
-  int span = s.max_len;  // keys of a tile at most
-  if (s.window > 0 && s.causal && !s.prefix)
-    span = (int)std::min<int64_t>(span, (int64_t)s.window + pl.block_m - 1 + 64);
-  const int stages = std::max(1, (span + 127) / 128);
-  pl.nsplit = 1;
-  pl.chunk = stages * 128;
-  if ((int64_t)pl.slots * s.hkv > kServingCounters / 2) return pl;
-  constexpr double kFixedStages = 2.5;  // a CTA's fixed cost, in 128-key stages (plan_stream's, in 64-key ones, is 5)
+int64_t tiling_units(const RaggedTiling& t, int hkv) { return (int64_t)t.slots * hkv; }
+
+// Keys that a tile of block_m tokens sees at most.
+int ragged_span(const RaggedShape& s, int block_m) {
+  int64_t span = s.max_len;
+  if (s.window > 0 && s.causal && !s.prefix) span = std::min<int64_t>(span, (int64_t)s.window + block_m - 1 + 64);
+  return (int)std::max<int64_t>(1, span);
+}
+
+// Key split of `units` tiles that see up to `stages` 128-key stages each; a CTA's fixed
+// cost is `fixed` stages. The lengths are not known here. One request: its length is the
+// bound, and the split that gives the fewest wave-stages is taken. Several: lengths
+// between a quarter of the bound and the bound are assumed, the CTAs dealt to the SMs as
+// they come free, so that the time is the mean load plus half of the last CTA's.
+void split_keys(RaggedTiling& t, int64_t units, int stages, int n, int sm_count, double fixed, int most) {
+  t.nsplit = 1;
+  t.chunk = stages * 128;
   double best = 1e300;
-  for (int ns = 1; ns <= std::min(stages, kMaxSplits); ++ns) {
-    const int chunk_st = (stages + ns - 1) / ns;
-    if ((stages + chunk_st - 1) / chunk_st != ns) continue;
-    const double waves = std::ceil((double)units * ns / sm_count);
-    const double cost = waves * (chunk_st + kFixedStages);
+  for (int ns = 1; ns <= std::min(stages, most); ++ns) {
+    const int chunk = (stages + ns - 1) / ns;
+    if ((stages + chunk - 1) / chunk != ns) continue;
+    double cost;
+    if (n == 1) {
+      cost = std::ceil((double)units * ns / sm_count) * (chunk + fixed);
+    } else {
+      const double load = (double)units * (0.625 * stages + (0.625 * ns + 0.5) * fixed) / sm_count;
+      cost = std::max(chunk + fixed, load + 0.5 * (chunk + fixed));
+    }
     if (cost < best - 1e-9) {
       best = cost;
-      pl.nsplit = ns;
-      pl.chunk = chunk_st * 128;
+      t.nsplit = ns;
+      t.chunk = chunk * 128;
     }
   }
-  return pl;
 }
 
-// Tiles of the tcgen05 kernel (pairs of 128-row query tiles) and its key split. At most
-// tokens / block_m + (requests of more than kStreamMaxRows rows) tiles; when they are
-// fewer than the SMs the keys are split, at least two 128-key tiles per chunk.
-RaggedPlan plan_ragged_tile(const RaggedShape& s, int sm_count) {
+RaggedPlan plan_ragged(const RaggedShape& s, bool fp8, int sm_count) {
   RaggedPlan pl{};
-  pl.block_m = 2 * (128 / s.group);
-  pl.rows = 256;
-  const int64_t longest = std::min<int64_t>(s.n, (int64_t)s.tokens * s.group / (kStreamMaxRows + 1));
-  pl.slots = (int)std::min<int64_t>((int64_t)s.tokens / pl.block_m + longest, INT_MAX);
-  const int64_t units = (int64_t)pl.slots * s.hkv;
-  int span = s.max_len;
-  if (s.window > 0 && s.causal && !s.prefix)
-    span = (int)std::min<int64_t>(span, (int64_t)s.window + pl.block_m - 1 + 64);
-  const int nk = std::max(1, (span + 127) / 128);
-  pl.nsplit = 1;
-  if (units > 0 && units < sm_count && units <= kServingCounters / 2) {
-    int ns = (int)std::min<int64_t>(sm_count / units, 16);
-    while (ns > 1 && nk < 2 * ns) --ns;
-    pl.nsplit = ns;
+  const int stream_rows = fp8 ? kStreamMaxRows : kRaggedStreamRows;
+  const bool tile = !fp8 && (int64_t)s.max_q * s.group > stream_rows;
+  // A single request of which the bounds allow the tcgen05 form takes it, whatever its length.
+  const bool stream = !tile || (s.group <= stream_rows && s.n > 1);
+  if (tile) {
+    // Pairs of 128-row query tiles: at most tokens / block_m + (requests of the form) of them.
+    RaggedTiling& t = pl.tile;
+    t.block_m = 2 * (128 / s.group);
+    t.rows = 256;
+    t.min_rows = stream ? stream_rows + 1 : 0;
+    t.max_rows = INT_MAX;
+    const int64_t longest = std::min<int64_t>(s.n, (int64_t)s.tokens * s.group / std::max(1, t.min_rows));
+    t.slots = (int)std::min<int64_t>((int64_t)s.tokens / t.block_m + longest, INT_MAX);
+    const int64_t units = tiling_units(t, s.hkv);
+    const int stages = (ragged_span(s, t.block_m) + 127) / 128;
+    if (units < sm_count && units <= kServingCounters / 2) {
+      split_keys(t, units, stages, s.n, sm_count, 6.0, std::max(1, std::min(16, stages / 2)));
+    } else {
+      t.nsplit = 1;
+      t.chunk = stages * 128;
+    }
+    pl.tile_ctas = units * t.nsplit;
   }
-  pl.chunk = (nk + pl.nsplit - 1) / pl.nsplit * 128;
+  if (stream) {
+    RaggedTiling& t = pl.stream;
+    const int max_q = tile ? stream_rows / s.group : s.max_q;
+    t.block_m = std::max(1, std::min(max_q, stream_rows / s.group));
+    t.rows = s.group * t.block_m;
+    t.one_tile = max_q <= t.block_m;
+    t.slots = t.one_tile ? s.n : s.tokens / t.block_m + s.n;
+    t.min_rows = 0;
+    t.max_rows = tile ? stream_rows : INT_MAX;
+    const int64_t tiles = t.one_tile ? std::min(s.n, s.tokens) : std::min(t.slots, s.tokens);
+    const int stages = (ragged_span(s, t.block_m) + 127) / 128;
+    if (tiling_units(t, s.hkv) <= kServingCounters / 2) {
+      split_keys(t, tiles * s.hkv, stages, s.n, sm_count, 3.0, kMaxSplits);
+    } else {
+      t.nsplit = 1;
+      t.chunk = stages * 128;
+    }
+    pl.stream_ctas = tiling_units(t, s.hkv) * t.nsplit;
+  }
   return pl;
 }
 
-// The streaming kernel takes the requests of up to kStreamMaxRows packed rows, the
-// tcgen05 kernel the rest; e4m3 caches are the streaming kernel's alone.
-bool ragged_uses_tile(const RaggedShape& s, bool fp8) { return !fp8 && (int64_t)s.max_q * s.group > kStreamMaxRows; }
-
-RaggedShape stream_part(const RaggedShape& s, bool tile) {
-  RaggedShape r = s;
-  if (tile) r.max_q = kStreamMaxRows / s.group;
-  return r;
-}
-
-size_t ragged_partial_bytes(const RaggedPlan& pl, const RaggedShape& s) {
-  if (pl.nsplit <= 1) return 0;
-  const size_t n = (size_t)pl.slots * s.hkv * pl.nsplit * pl.rows;
+size_t ragged_partial_bytes(const RaggedTiling& t, const RaggedShape& s) {
+  if (t.nsplit <= 1) return 0;
+  const size_t n = (size_t)tiling_units(t, s.hkv) * t.nsplit * t.rows;
   return 2 * align256(n * 4) + align256(n * s.head_dim * 4);
 }
 
-// Counters first (half for each kernel), then the streaming kernel's partials, then the
-// tcgen05 kernel's.
-size_t ragged_ws_bytes(const RaggedPlan& stream, const RaggedPlan* tile, const RaggedShape& s) {
-  const size_t n = ragged_partial_bytes(stream, s) + (tile ? ragged_partial_bytes(*tile, s) : 0);
+// Counters first (half for each form), then the streaming form's partials, then the other's.
+size_t ragged_ws_bytes(const RaggedPlan& pl, const RaggedShape& s) {
+  const size_t n = ragged_partial_bytes(pl.stream, s) + ragged_partial_bytes(pl.tile, s);
   return n ? (size_t)kServingCounters * 4 + n : 0;
 }
 
-void ragged_ws_carve(const RaggedPlan& pl, const RaggedShape& s, uint8_t* counters, uint8_t* c, RaggedParams* p) {
-  const size_t n = (size_t)pl.slots * s.hkv * pl.nsplit * pl.rows;
-  p->ws_cnt = reinterpret_cast<unsigned*>(counters);
-  p->ws_m = reinterpret_cast<float*>(c);
+void carve_partials(RaggedTiling& t, const RaggedShape& s, uint8_t* counters, uint8_t* c) {
+  const size_t n = (size_t)tiling_units(t, s.hkv) * t.nsplit * t.rows;
+  t.ws_cnt = reinterpret_cast<unsigned*>(counters);
+  t.ws_m = reinterpret_cast<float*>(c);
   c += align256(n * 4);
-  p->ws_l = reinterpret_cast<float*>(c);
+  t.ws_l = reinterpret_cast<float*>(c);
   c += align256(n * 4);
-  p->ws_acc = reinterpret_cast<float*>(c);
-}
-
-void set_plan(RaggedParams& p, const RaggedPlan& pl) {
-  p.block_m = pl.block_m;
-  p.rows = pl.rows;
-  p.one_tile = pl.one_tile;
-  p.slots = pl.slots;
-  p.nsplit = pl.nsplit;
-  p.chunk = pl.chunk;
+  t.ws_acc = reinterpret_cast<float*>(c);
 }
 
 // 4-D map (d, kv head, position in block, block) of a paged cache with element strides
@@ -332,9 +323,7 @@ size_t gqa_ragged_fwd_workspace_bytes(const gqa_ragged_args* args) {
   RaggedShape s;
   int sm = 0;
   if (!args || check_ragged_shape(*args, &s) || s.n == 0 || s.tokens == 0 || s.max_q == 0 || current_device(&sm)) return 0;
-  const bool tile = ragged_uses_tile(s, args->cache_fp8 != 0);
-  const RaggedPlan tp = plan_ragged_tile(s, sm);
-  return ragged_ws_bytes(plan_ragged_stream(stream_part(s, tile), sm), tile ? &tp : nullptr, s);
+  return ragged_ws_bytes(plan_ragged(s, args->cache_fp8 != 0, sm), s);
 }
 
 int gqa_ragged_fwd(const gqa_ragged_args* args, void* stream) {
@@ -394,18 +383,27 @@ int gqa_ragged_fwd(const gqa_ragged_args* args, void* stream) {
   p.v_scale = a.cache_fp8 ? a.v_scale : 1.f;
   p.mods = a.softcap > 0.f || a.alibi_slopes;
 
-  const bool tile = ragged_uses_tile(s, a.cache_fp8 != 0);
-  const RaggedShape ss = stream_part(s, tile);
-  RaggedPlan sp = plan_ragged_stream(ss, sm), tp = plan_ragged_tile(s, sm);
+  RaggedPlan pl = plan_ragged(s, a.cache_fp8 != 0, sm);
   if (a.workspace) {
     if (!aligned16(a.workspace)) return GQA_ERR_ALIGNMENT;
-    if (a.workspace_bytes < ragged_ws_bytes(sp, tile ? &tp : nullptr, s)) return GQA_ERR_WORKSPACE;
+    if (a.workspace_bytes < ragged_ws_bytes(pl, s)) return GQA_ERR_WORKSPACE;
+    uint8_t* const counters = reinterpret_cast<uint8_t*>(a.workspace);
+    uint8_t* const partials = counters + (size_t)kServingCounters * 4;
+    if (pl.stream.nsplit > 1) carve_partials(pl.stream, s, counters, partials);
+    if (pl.tile.nsplit > 1)
+      carve_partials(pl.tile, s, counters + (size_t)kServingCounters * 2, partials + ragged_partial_bytes(pl.stream, s));
   } else {  // nowhere to leave partials: one CTA per tile
-    sp.nsplit = tp.nsplit = 1;
-    sp.chunk = tp.chunk = std::max(1, (a.max_seq_len + 127) / 128) * 128;
+    pl.stream_ctas /= std::max(1, pl.stream.nsplit);
+    pl.tile_ctas /= std::max(1, pl.tile.nsplit);
+    pl.stream.nsplit = pl.tile.nsplit = 1;
+    pl.stream.chunk = pl.tile.chunk = std::max(1, (a.max_seq_len + 127) / 128) * 128;
   }
-  uint8_t* const counters = reinterpret_cast<uint8_t*>(a.workspace);
-  uint8_t* const partials = counters + (size_t)kServingCounters * 4;
+  if (pl.tile_ctas + pl.stream_ctas > INT_MAX) return GQA_ERR_INVALID_ARG;
+  const unsigned grid = (unsigned)(pl.tile_ctas + pl.stream_ctas);
+  p.stream = pl.stream;
+  p.tile = pl.tile;
+  p.tile_ctas = (unsigned)pl.tile_ctas;
+
   CUtensorMap km, vm;
   rc = make_cache_map(&km, a.k_cache, a.k_strides, a.num_blocks, a.block_size, a.num_kv_heads, a.head_dim, p.box, a.cache_fp8);
   if (!rc) rc = make_cache_map(&vm, a.v_cache, a.v_strides, a.num_blocks, a.block_size, a.num_kv_heads, a.head_dim, p.box, a.cache_fp8);
@@ -413,45 +411,23 @@ int gqa_ragged_fwd(const gqa_ragged_args* args, void* stream) {
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const bool bf = a.dtype == GQA_DTYPE_BF16;
   cudaError_t e = cudaSuccess;
-
-  if (tile) {
-    RaggedParams t = p;
-    set_plan(t, tp);
-    t.min_rows = kStreamMaxRows + 1;
-    t.max_rows = INT_MAX;
-    if (tp.nsplit > 1)
-      ragged_ws_carve(tp, s, counters + (size_t)kServingCounters * 2, partials + ragged_partial_bytes(sp, s), &t);
-    // Queries (d, head, token): a tile is bm tokens of the group's heads, token-major rows.
+  if (pl.tile_ctas > 0) {
+    // Queries (d, head, token): a tile is tokens of the group's heads, token-major rows.
     const int64_t bhsd[4] = {a.q_strides[0] * a.num_tokens, a.q_strides[0], a.q_strides[1], 1};
     CUtensorMap qm;
-    rc = make_map(&qm, a.q, bhsd, 1, a.num_tokens, a.num_heads, a.head_dim, s.group, tp.block_m / 2);
+    rc = make_map(&qm, a.q, bhsd, 1, a.num_tokens, a.num_heads, a.head_dim, s.group, pl.tile.block_m / 2);
     if (rc) return rc;
-    const int64_t grid = (int64_t)tp.slots * a.num_kv_heads * tp.nsplit;
-    if (grid > INT_MAX) return GQA_ERR_INVALID_ARG;
     if (a.head_dim == 128)
-      e = bf ? launch_ragged_tile_hd<128, true>(t, (unsigned)grid, qm, km, vm, st)
-             : launch_ragged_tile_hd<128, false>(t, (unsigned)grid, qm, km, vm, st);
+      e = bf ? launch_ragged_tile<128, true>(p, grid, qm, km, vm, st) : launch_ragged_tile<128, false>(p, grid, qm, km, vm, st);
     else
-      e = bf ? launch_ragged_tile_hd<64, true>(t, (unsigned)grid, qm, km, vm, st)
-             : launch_ragged_tile_hd<64, false>(t, (unsigned)grid, qm, km, vm, st);
-    if (e != cudaSuccess) return GQA_ERR_CUDA;
+      e = bf ? launch_ragged_tile<64, true>(p, grid, qm, km, vm, st) : launch_ragged_tile<64, false>(p, grid, qm, km, vm, st);
+  } else if (a.cache_fp8) {
+    e = bf ? launch_ragged_stream<128, true, true>(p, grid, km, vm, st) : launch_ragged_stream<128, false, true>(p, grid, km, vm, st);
+  } else if (a.head_dim == 128) {
+    e = bf ? launch_ragged_stream<128, true, false>(p, grid, km, vm, st) : launch_ragged_stream<128, false, false>(p, grid, km, vm, st);
+  } else {
+    e = bf ? launch_ragged_stream<64, true, false>(p, grid, km, vm, st) : launch_ragged_stream<64, false, false>(p, grid, km, vm, st);
   }
-
-  set_plan(p, sp);
-  p.min_rows = 0;
-  p.max_rows = tile ? kStreamMaxRows : INT_MAX;
-  if (sp.nsplit > 1) ragged_ws_carve(sp, s, counters, partials, &p);
-  const int64_t grid = (int64_t)sp.slots * a.num_kv_heads * sp.nsplit;
-  if (grid > INT_MAX) return GQA_ERR_INVALID_ARG;
-  if (a.cache_fp8)
-    e = bf ? launch_ragged_stream_hd<128, true, true>(p, (unsigned)grid, km, vm, st)
-           : launch_ragged_stream_hd<128, false, true>(p, (unsigned)grid, km, vm, st);
-  else if (a.head_dim == 128)
-    e = bf ? launch_ragged_stream_hd<128, true, false>(p, (unsigned)grid, km, vm, st)
-           : launch_ragged_stream_hd<128, false, false>(p, (unsigned)grid, km, vm, st);
-  else
-    e = bf ? launch_ragged_stream_hd<64, true, false>(p, (unsigned)grid, km, vm, st)
-           : launch_ragged_stream_hd<64, false, false>(p, (unsigned)grid, km, vm, st);
   return e == cudaSuccess ? GQA_OK : GQA_ERR_CUDA;
 }
 

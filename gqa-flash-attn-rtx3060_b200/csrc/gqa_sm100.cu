@@ -55,8 +55,7 @@ cudaError_t set_smem(K kernel, int bytes) {
   return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
 }
 
-cudaError_t prepare_ragged();  // gqa_serving.cuh
-int prepare_ragged_tile();
+int prepare_ragged();  // gqa_serving.cuh
 
 int init_device(int dev) {
   cudaDeviceProp prop;
@@ -114,9 +113,8 @@ int init_device(int dev) {
   chk(set_smem(gqa_stream_kernel<128, false, 1, false, true>, StreamCfg<128>::kSmemBytes));
   chk(set_smem(gqa_stream_kernel<64, true, 1, false, true>, StreamCfg<64>::kSmemBytes));
   chk(set_smem(gqa_stream_kernel<64, false, 1, false, true>, StreamCfg<64>::kSmemBytes));
-  chk(prepare_ragged());
   if (e != cudaSuccess) return GQA_ERR_CUDA;
-  return prepare_ragged_tile();
+  return prepare_ragged();
 }
 
 // Returns GQA_OK and the SM count of the current device, initialising it once.
