@@ -72,6 +72,7 @@ struct RaggedParams {
   float cap_most;
   float v_scale;          // e4m3 values
   int mods;               // cap or bias present
+  int linear_bias;        // no key past a token is visible to it
   RaggedTiling stream, tile;
   unsigned tile_ctas;     // CTAs of the tcgen05 form, the grid's first; the rest stream
 };

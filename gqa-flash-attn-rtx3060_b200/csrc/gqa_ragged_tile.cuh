@@ -15,8 +15,7 @@
 //  - Scores may be capped or biased (MOD), see below.
 //  - A tile whose tokens fit the first query tile runs solo: the two warpgroups take the
 //    even and the odd key tiles of the same 128 rows (own S, O, maximum and sum) and merge
-//    at the end. So a request of few rows keeps the tensor core and both warpgroups busy,
-//    and with 256 keys in flight a CTA streams as fast as HBM delivers.
+//    at the end, so that a request of few rows keeps both warpgroups busy.
 //  - O leaves through shared memory with ordinary 16-byte stores, since a tile may end
 //    where the next request's rows begin.
 //
@@ -71,14 +70,23 @@ __device__ __forceinline__ float max3_abs(float a, float b, float c) {
 template <int HD>
 struct RaggedTileCfg : PrefillCfg<HD> {
   using Base = PrefillCfg<HD>;
-  // A solo tile's second Q buffer is one more K/V slot, in front of the ring's first.
-  static constexpr int kMaxSlots = Base::kSlots + 1;
-  static constexpr int kNumBars = 2 + 2 * kMaxSlots + 2 + 2 * Base::kPParts + 2 + 1;
-  static constexpr int kMiscOff = Base::kBarOff + kNumBars * 8;
-  // tmem base, abort flag, last-CTA flag, work item, warp sums of the scan
+  static constexpr int kTileBytes = Base::kTileBytes;
+  // K and V have a ring each (K_j's slot is free once QK_j is done, V_j's only after the
+  // softmax and PV_j), filled by a warp each. A pair's rings start after its two Q tiles;
+  // a solo tile has one, and less work per key to hide the loads behind, so its rings are
+  // longer: they fill the shared memory that an SM has.
+  static constexpr int kPairSlots = HD == 128 ? 2 : 4;  // of each of K and V
+  static constexpr int kSoloSlots = HD == 128 ? 3 : 6;
+  static constexpr int kRingTiles = 2 * kPairSlots + 1 > 2 * kSoloSlots ? 2 * kPairSlots + 1 : 2 * kSoloSlots;
+  static constexpr int kBarOff = (1 + kRingTiles) * kTileBytes;
+  // q_full[2] k_full[S] k_empty[S] v_full[S] v_empty[S] s_full[2] p_full[2][kPParts] o_final[2] mma_done
+  static constexpr int kNumBars = 2 + 4 * kSoloSlots + 2 + 2 * Base::kPParts + 2 + 1;
+  // tmem base, abort flag, last-CTA flag, then the work item and the scan's warp sums
+  static constexpr int kMiscOff = kBarOff + kNumBars * 8;
   static constexpr int kWorkOff = kMiscOff + 16;
   static constexpr int kTileSmem = kWorkOff + 64 + 64 + 1024;
   static constexpr int kSmemBytes = kTileSmem > StreamCfg<HD>::kSmemBytes ? kTileSmem : StreamCfg<HD>::kSmemBytes;
+  static_assert(kSmemBytes <= 227 * 1024, "one CTA's shared memory");
 };
 
 template <int HD, bool BF16, int MOD>
@@ -94,7 +102,6 @@ __global__ void __launch_bounds__(384, 1)
   using Cfg = RaggedTileCfg<HD>;
   const RaggedTiling& tl = p.tile;
   constexpr int NSUB = Cfg::kNSub;
-  constexpr int SLOTS = Cfg::kMaxSlots;  // barriers; a pair uses one slot fewer
   constexpr int BN = Cfg::kBN;
 
   extern __shared__ uint8_t smem_raw[];
@@ -102,13 +109,15 @@ __global__ void __launch_bounds__(384, 1)
   const uint32_t base = (raw_base + 1023u) & ~1023u;
   uint8_t* const smem = smem_raw + (base - raw_base);
 
-  const uint32_t q_smem0 = base + Cfg::kQOff;
-  const uint32_t kv_smem0 = base + Cfg::kKVOff;
+  constexpr int MAXS = Cfg::kSoloSlots;  // barriers per ring
+  const uint32_t q_smem0 = base;
   const uint32_t bars = base + Cfg::kBarOff;
   const uint32_t bar_q_full = bars;                             // [2]
-  const uint32_t bar_kv_full = bars + 16;                       // [SLOTS]
-  const uint32_t bar_kv_empty = bar_kv_full + 8 * SLOTS;        // [SLOTS]
-  const uint32_t bar_s_full = bar_kv_empty + 8 * SLOTS;         // [2]
+  const uint32_t bar_k_full = bars + 16;                        // [MAXS] each
+  const uint32_t bar_k_empty = bar_k_full + 8 * MAXS;
+  const uint32_t bar_v_full = bar_k_empty + 8 * MAXS;
+  const uint32_t bar_v_empty = bar_v_full + 8 * MAXS;
+  const uint32_t bar_s_full = bar_v_empty + 8 * MAXS;           // [2]
   const uint32_t bar_p_full = bar_s_full + 16;                  // [2][kPParts]
   const uint32_t bar_o_final = bar_p_full + 16 * Cfg::kPParts;  // [2]
   const uint32_t bar_mma_done = bar_o_final + 16;
@@ -140,10 +149,7 @@ __global__ void __launch_bounds__(384, 1)
   if (tid == 0) {
     mbar_init(bar_q_full, 1);
     mbar_init(bar_q_full + 8, 1);
-    for (int s = 0; s < SLOTS; ++s) {
-      mbar_init(bar_kv_full + 8 * s, 1);
-      mbar_init(bar_kv_empty + 8 * s, 1);
-    }
+    for (int s = 0; s < 4 * MAXS; ++s) mbar_init(bar_k_full + 8 * s, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(bar_s_full + 8 * i, 1);
       for (int h = 0; h < Cfg::kPParts; ++h) mbar_init(bar_p_full + 8 * (Cfg::kPParts * i + h), 128);
@@ -229,8 +235,9 @@ __global__ void __launch_bounds__(384, 1)
   __syncthreads();
   if (split >= work->n_chunks) return;  // the whole CTA, before TMEM
   const bool solo = work->nq <= bm;
-  const int slots = solo ? SLOTS : SLOTS - 1;                          // ring slots in use,
-  const uint32_t kv_base = solo ? kv_smem0 - Cfg::kTileBytes : kv_smem0;  // the first of them
+  const int slots = solo ? MAXS : Cfg::kPairSlots;                       // of each ring
+  const uint32_t k_ring = q_smem0 + (solo ? 1 : 2) * Cfg::kTileBytes;
+  const uint32_t v_ring = k_ring + slots * Cfg::kTileBytes;
   if (warp == 8) {
     tmem_alloc(smem_u32(tmem_base_ptr), Cfg::kTmemCols);
     tmem_relinquish();
@@ -244,25 +251,28 @@ __global__ void __launch_bounds__(384, 1)
   static_assert(Cfg::kSoftmaxRegs == 208 && Cfg::kControlRegs == 88, "keep the asm immediates in sync");
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;" ::: "memory");
-    if (warp == 9) {
-      // ============================================================== producer
-      // Lane i brings box i / NSUB, 64 values of d at i % NSUB, of each K or V tile. Boxes
-      // past the last key get a block outside the cache: TMA fills them with zeros.
+    if (warp == 9 || warp == 10) {
+      // ============================================================== producers: K, V
+      // Lane i brings box i / NSUB, 64 values of d at i % NSUB, of each tile. Boxes past the
+      // last key get a block outside the cache: TMA fills them with zeros.
+      const bool is_v = warp == 10;
+      const CUtensorMap* map = is_v ? &vmap : &kmap;
+      const uint32_t full0 = is_v ? bar_v_full : bar_k_full, empty0 = is_v ? bar_v_empty : bar_k_empty;
       const int nk = work->nk;
       if (nk > 0) {
         if (lane == 0) {
-          tma_prefetch_desc(&qmap);
-          tma_prefetch_desc(&kmap);
-          tma_prefetch_desc(&vmap);
-          const int hq0 = kvh * p.group, t0 = work->t0;
+          tma_prefetch_desc(map);
+          if (!is_v) {
+            const int hq0 = kvh * p.group, t0 = work->t0;
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            if (i == 1 && solo) break;
-            mbar_arrive_expect_tx(bar_q_full + 8 * i, (uint32_t)(bm * p.group) * 128u * NSUB);
+            for (int i = 0; i < 2; ++i) {
+              if (i == 1 && solo) break;
+              mbar_arrive_expect_tx(bar_q_full + 8 * i, (uint32_t)(bm * p.group) * 128u * NSUB);
 #pragma unroll
-            for (int s = 0; s < NSUB; ++s)
-              tma_load_4d(q_smem0 + i * Cfg::kTileBytes + s * Cfg::kSubBytes, &qmap, bar_q_full + 8 * i, s * 64, hq0,
-                          t0 + i * bm, 0);
+              for (int s = 0; s < NSUB; ++s)
+                tma_load_4d(q_smem0 + i * Cfg::kTileBytes + s * Cfg::kSubBytes, &qmap, bar_q_full + 8 * i, s * 64, hq0,
+                            t0 + i * bm, 0);
+            }
           }
         }
         const int box = p.box, nbox = BN / box;
@@ -271,37 +281,33 @@ __global__ void __launch_bounds__(384, 1)
         const int k_hi = work->k_hi, key_first = work->key0 + my_box * box;
         const int* row_bt = p.block_table + (int64_t)work->b * p.bt_stride;
         const int mask = (1 << p.block_shift) - 1;
-        const uint32_t dst0 = kv_base + my_sub * Cfg::kSubBytes + (uint32_t)(my_box * box) * 128u;
-        int t = 0;
-        const int n_loads = 2 * nk;
-        int pb = 0;
+        const uint32_t dst0 = (is_v ? v_ring : k_ring) + my_sub * Cfg::kSubBytes + (uint32_t)(my_box * box) * 128u;
+        int j = 0, slot = 0, use = 0;
         bool ok = true;
-        int slot = 0, use = 0;
-        for (; t < n_loads; ++t) {
-          const int key = key_first + (t >> 1) * BN;
-          // Looked up once per tile (K loads; V reuses it), before the slot wait.
-          if ((t & 1) == 0) pb = (loads && key < k_hi) ? row_bt[key >> p.block_shift] : p.num_blocks;
+        for (; j < nk; ++j) {
+          const int key = key_first + j * BN;
+          // Looked up before the slot wait, so the table read overlaps it.
+          const int pb = (loads && key < k_hi) ? row_bt[key >> p.block_shift] : p.num_blocks;
           if (use > 0) {
-            ok = mbar_wait(bar_kv_empty + 8 * slot, (use - 1) & 1, abort_flag, 121);
+            ok = mbar_wait(empty0 + 8 * slot, (use - 1) & 1, abort_flag, 121);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
           }
-          if (!withheld_load(t)) {
-            const uint32_t full = bar_kv_full + 8 * slot;
+          if (!withheld_load(2 * j + is_v)) {
+            const uint32_t full = full0 + 8 * slot;
             if (lane == 0) mbar_arrive_expect_tx(full, Cfg::kTileBytes);
             __syncwarp();
-            if (loads)
-              tma_load_4d(dst0 + slot * Cfg::kTileBytes, (t & 1) ? &vmap : &kmap, full, my_sub * 64, kvh, key & mask, pb);
+            if (loads) tma_load_4d(dst0 + slot * Cfg::kTileBytes, map, full, my_sub * 64, kvh, key & mask, pb);
           }
           if (++slot == slots) {
             slot = 0;
             ++use;
           }
         }
-        if (t < n_loads && lane == 0) {  // aborted: let in-flight loads land before teardown
+        if (j < nk && lane == 0) {  // aborted: let in-flight loads land before teardown
           volatile int dummy = 0;
-          for (int u = max(0, t - slots); u < t; ++u)
-            if (!withheld_load(u)) mbar_wait(bar_kv_full + 8 * (u % slots), (u / slots) & 1, &dummy, 122);
+          for (int u = max(0, j - slots); u < j; ++u)
+            if (!withheld_load(2 * u + is_v)) mbar_wait(full0 + 8 * (u % slots), (u / slots) & 1, &dummy, 122);
         }
       }
       __syncwarp();
@@ -314,7 +320,7 @@ __global__ void __launch_bounds__(384, 1)
         auto issue_qk = [&](int i, int slot) {
           const uint32_t tS = tmem_base + (i ? Cfg::kColS1 : Cfg::kColS0);
           const uint32_t qa = q_smem0 + (solo ? 0 : i) * Cfg::kTileBytes;
-          const uint32_t kb = kv_base + slot * Cfg::kTileBytes;
+          const uint32_t kb = k_ring + slot * Cfg::kTileBytes;
 #pragma unroll
           for (int k = 0; k < HD / 16; ++k) {
             const uint32_t o = (k >> 2) * Cfg::kSubBytes + (k & 3) * 32;
@@ -324,7 +330,7 @@ __global__ void __launch_bounds__(384, 1)
         auto issue_pv = [&](int i, int slot, int h, bool acc) {
           const uint32_t tS = tmem_base + (i ? Cfg::kColS1 : Cfg::kColS0);
           const uint32_t tO = tmem_base + (i ? Cfg::kColO1 : Cfg::kColO0);
-          const uint32_t vb = kv_base + slot * Cfg::kTileBytes;
+          const uint32_t vb = v_ring + slot * Cfg::kTileBytes;
           constexpr int kPerPart = BN / 16 / Cfg::kPParts;
 #pragma unroll
           for (int kk = 0; kk < kPerPart; ++kk) {
@@ -334,19 +340,18 @@ __global__ void __launch_bounds__(384, 1)
           }
         };
         bool ok = mbar_wait(bar_q_full, 0, abort_flag, 130) &&
-                  (solo || mbar_wait(bar_q_full + 8, 0, abort_flag, 131)) && mbar_wait(bar_kv_full, 0, abort_flag, 132);
+                  (solo || mbar_wait(bar_q_full + 8, 0, abort_flag, 131)) && mbar_wait(bar_k_full, 0, abort_flag, 132);
         if (ok && !solo) {
-          constexpr int SLOTS = Cfg::kSlots;
+          constexpr int S = Cfg::kPairSlots;
           tc_fence_after();
           issue_qk(0, 0);
           umma_commit(bar_s_full);
           issue_qk(1, 0);
           umma_commit(bar_s_full + 8);
-          umma_commit(bar_kv_empty);  // K_0 consumed
+          umma_commit(bar_k_empty);  // K_0 consumed
           for (int j = 0; j < nk; ++j) {
-            const int tv = 2 * j + 1, sv = tv % SLOTS;
-            const int tk = 2 * j + 2, sk = tk % SLOTS;
-            if (!mbar_wait(bar_kv_full + 8 * sv, (tv / SLOTS) & 1, abort_flag, 133)) break;
+            const int sv = j % S, sk = (j + 1) % S;
+            if (!mbar_wait(bar_v_full + 8 * sv, (j / S) & 1, abort_flag, 133)) break;
             bool pv_ok = true;
 #pragma unroll
             for (int h = 0; h < Cfg::kPParts && pv_ok; ++h) {
@@ -359,7 +364,7 @@ __global__ void __launch_bounds__(384, 1)
             if (!pv_ok) break;
             const bool more = (j + 1 < nk);
             if (more) {
-              if (!mbar_wait(bar_kv_full + 8 * sk, (tk / SLOTS) & 1, abort_flag, 135)) break;
+              if (!mbar_wait(bar_k_full + 8 * sk, ((j + 1) / S) & 1, abort_flag, 135)) break;
               tc_fence_after();
               issue_qk(0, sk);
               umma_commit(bar_s_full);
@@ -375,32 +380,32 @@ __global__ void __launch_bounds__(384, 1)
               }
             }
             if (!pv_ok) break;
-            umma_commit(bar_kv_empty + 8 * sv);  // V_j consumed
+            umma_commit(bar_v_empty + 8 * sv);  // V_j consumed
             if (more) {
               issue_qk(1, sk);
               umma_commit(bar_s_full + 8);
-              umma_commit(bar_kv_empty + 8 * sk);  // K_{j+1} consumed
+              umma_commit(bar_k_empty + 8 * sk);  // K_{j+1} consumed
             } else {
               umma_commit(bar_o_final + 8);
             }
           }
         }
         if (ok && solo) {
-          // Key tile j belongs to warpgroup j & 1, which owns S_i and O_i, i = j & 1. Loads
-          // are K_0 V_0 K_1 V_1 ...; QK_0 and QK_1 go first, then PV_j and QK_{j + 2}.
+          // Key tile j belongs to warpgroup j & 1, which owns S_i and O_i, i = j & 1. QK_0
+          // and QK_1 go first, then PV_j and QK_{j + 2}.
           auto qk = [&](int j) -> bool {
-            const int t = 2 * j, sl = t % SLOTS;
-            if (!mbar_wait(bar_kv_full + 8 * sl, (t / SLOTS) & 1, abort_flag, 135)) return false;
+            const int sl = j % MAXS;
+            if (!mbar_wait(bar_k_full + 8 * sl, (j / MAXS) & 1, abort_flag, 135)) return false;
             tc_fence_after();
             issue_qk(j & 1, sl);
             umma_commit(bar_s_full + 8 * (j & 1));
-            umma_commit(bar_kv_empty + 8 * sl);  // K_j consumed
+            umma_commit(bar_k_empty + 8 * sl);  // K_j consumed
             return true;
           };
           bool go = qk(0) && (nk < 2 || qk(1));
           for (int j = 0; j < nk && go; ++j) {
-            const int i = j & 1, t = 2 * j + 1, sl = t % SLOTS;
-            go = mbar_wait(bar_kv_full + 8 * sl, (t / SLOTS) & 1, abort_flag, 133);
+            const int i = j & 1, sl = j % MAXS;
+            go = mbar_wait(bar_v_full + 8 * sl, (j / MAXS) & 1, abort_flag, 133);
 #pragma unroll
             for (int h = 0; h < Cfg::kPParts && go; ++h) {
               go = mbar_wait(bar_p_full + 8 * (Cfg::kPParts * i + h), (j >> 1) & 1, abort_flag, h ? 138 : 134);
@@ -410,7 +415,7 @@ __global__ void __launch_bounds__(384, 1)
               }
             }
             if (!go) break;
-            umma_commit(bar_kv_empty + 8 * sl);  // V_j consumed
+            umma_commit(bar_v_empty + 8 * sl);  // V_j consumed
             if (j + 2 < nk)
               go = qk(j + 2);
             else
@@ -436,74 +441,66 @@ __global__ void __launch_bounds__(384, 1)
     const uint32_t s_full = bar_s_full + 8 * wg;
     const uint32_t p_full = bar_p_full + 8 * Cfg::kPParts * wg;
 
-    // The row's interval, counted from this CTA's first key; idle rows and rows past the
-    // tile's tokens see nothing.
-    int lo_rel = 0, hi_rel = 0;
-    float dist0 = 0.f, slope = 0.f;
-    {
-      const int m = row / p.group, i = (solo ? 0 : wg * bm) + m;
-      if (m < bm && i < work->nq) {
-        RaggedWork w;
-        w.b = work->b;
-        w.len = work->len;
-        w.off = work->off_m0;
-        w.m0 = 0;
-        w.t0 = work->t0;
-        int pos;
-        ragged_row(p, w, i, pos, lo_rel, hi_rel);
-        if constexpr (MOD == kRaggedBias) {
-          slope = p.alibi[kvh * p.group + row % p.group] * 1.4426950408889634f;
-          dist0 = (float)(pos - work->key0);
-        }
-        lo_rel -= work->key0;
-        hi_rel -= work->key0;
+    // This warpgroup's key tiles: all of them, or of a solo tile every other one.
+    const int kstep = solo ? 2 * BN : BN;
+    int key = work->key0 + (solo ? wg * BN : 0);  // first key of the step's tile
+    const int n_steps = solo ? (work->nk + 1 - wg) >> 1 : work->nk;
+    // The row's interval, counted from `key`: columns [low, rem) are visible. Idle rows
+    // (past the tile's tokens, or of no head) count as seeing everything, so that they do
+    // not put their warp on the masked path; whatever is in their rows of S and P reaches
+    // their own rows of O alone, which are not stored.
+    int low = INT_MIN / 2, rem = INT_MAX / 2;
+    float dist = 0.f, slope = 0.f;  // position less that of column 0, with a distance bias
+    const int m_row = row / p.group, i_row = (solo ? 0 : wg * bm) + m_row;
+    const bool idle = m_row >= bm || i_row >= work->nq;
+    if (!idle) {
+      RaggedWork w;
+      w.b = work->b;
+      w.len = work->len;
+      w.off = work->off_m0;
+      w.m0 = 0;
+      w.t0 = work->t0;
+      int pos;
+      ragged_row(p, w, i_row, pos, low, rem);
+      if constexpr (MOD == kRaggedBias) {
+        slope = p.alibi[kvh * p.group + row % p.group] * 1.4426950408889634f;
+        dist = (float)(pos - key);
       }
+      low -= key;
+      rem -= key;
     }
+    const bool idle_warp = __all_sync(0xffffffffu, idle);  // only keeps the barriers going
     float m_run = -3.0e38f;
     float l_run = 0.f;
     bool ok = true;
-    // This warpgroup's key tiles: all of them, or of a solo tile every other one. Step n
-    // is key tile j.
-    const int nk = work->nk;
-    const int n_steps = solo ? (nk + 1 - wg) >> 1 : nk;
-    // Rows that see nothing at all (idle rows, rows past the tile's tokens) do no softmax: a warp
-    // of them only keeps the barriers going. What is left in its rows of P reaches its own rows of O alone.
-    const bool idle_warp = __all_sync(0xffffffffu, hi_rel <= lo_rel);
-    for (int n = 0; n < n_steps; ++n) {
-      const int j = solo ? 2 * n + wg : n;
+    for (int n = 0; n < n_steps; ++n, key += kstep, rem -= kstep, low -= kstep) {
       ok = mbar_wait(s_full, n & 1, abort_flag, 140 + wg);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc_fence_after();
-      {
+      if (key + BN > work->k_hi || key < work->k_lo) {
         // Keys of the tile that no row sees (past the last, or before the first in its
         // box) have P = 0, but their stale slots may hold NaN or Inf: each thread zeroes
         // its row of V, once V has landed and before P is published.
-        const int key = work->key0 + j * BN;
-        if (key + BN > work->k_hi || key < work->k_lo) {
-          const int tv = 2 * j + 1;
-          ok = mbar_wait(bar_kv_full + 8 * (tv % slots), (tv / slots) & 1, abort_flag, 144 + wg);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-          if (key + row >= work->k_hi || key + row < work->k_lo) {
-            const uint32_t vrow = kv_base + (tv % slots) * Cfg::kTileBytes + row * 128;
+        const int j = (key - work->key0) / BN;
+        ok = mbar_wait(bar_v_full + 8 * (j % slots), (j / slots) & 1, abort_flag, 144 + wg);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        if (key + row >= work->k_hi || key + row < work->k_lo) {
+          const uint32_t vrow = v_ring + (j % slots) * Cfg::kTileBytes + row * 128;
 #pragma unroll
-            for (int c = 0; c < NSUB * 8; ++c)
-              asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(vrow + (c >> 3) * Cfg::kSubBytes +
-                                                                          (c & 7) * 16),
-                           "r"(0u)
-                           : "memory");
-          }
-          fence_proxy_async_smem();
+          for (int c = 0; c < NSUB * 8; ++c)
+            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(vrow + (c >> 3) * Cfg::kSubBytes + (c & 7) * 16),
+                         "r"(0u)
+                         : "memory");
         }
+        fence_proxy_async_smem();
       }
       if (idle_warp) {
 #pragma unroll
         for (int h = 0; h < Cfg::kPParts; ++h) mbar_arrive(p_full + 8 * h);
         continue;
       }
-      const int rem = hi_rel - j * BN;   // columns [low, rem) are visible
-      const int low = lo_rel - j * BN;
       const bool masked = rem < BN || low > 0;
       uint32_t sr[128];
       tmem_ld32(tS + 0, sr + 0);
@@ -513,22 +510,27 @@ __global__ void __launch_bounds__(384, 1)
       tmem_ld32(tS + 64, sr + 64);
       tmem_ld32(tS + 96, sr + 96);
       float mx;
-      if constexpr (MOD == kRaggedBias) {
-        // Scores to log2 units with cap and bias, in place; then the mask and the maximum.
-        tmem_wait_ld();
-        reg_fence_n<64>(sr + 64);
-        const float d0 = dist0 - (float)(j * BN);
-        if (p.cap_in != 0.f) {
+      // With a bias: scores to log2 units in place, half a row at a time. Keys past the
+      // token are only visible with a prefix (or without causal); otherwise the bias is
+      // linear in the key, slope (c - distance of column 0).
+      auto biased = [&](int c0) {
+        const float d0 = dist - (float)(n * kstep);
+        if (p.cap_in == 0.f && p.linear_bias) {
+          const float b0 = -slope * d0;
 #pragma unroll
-          for (int c = 0; c < 128; ++c)
-            sr[c] = __float_as_uint(fmaf(-2.f * p.cap_out, fast_rcp(1.f + fast_exp2(__uint_as_float(sr[c]) * p.cap_in)),
-                                         fmaf(-slope, fabsf(d0 - (float)c), p.cap_out)));
+          for (int c = c0; c < c0 + 64; ++c)
+            sr[c] = __float_as_uint(fmaf(__uint_as_float(sr[c]), p.scale_log2, fmaf(slope, (float)c, b0)));
         } else {
 #pragma unroll
-          for (int c = 0; c < 128; ++c)
-            sr[c] = __float_as_uint(fmaf(__uint_as_float(sr[c]), p.scale_log2, -slope * fabsf(d0 - (float)c)));
+          for (int c = c0; c < c0 + 64; ++c) {
+            const float s = __uint_as_float(sr[c]);
+            float x = s * p.scale_log2;
+            if (p.cap_in != 0.f) x = fmaf(-2.f * p.cap_out, fast_rcp(1.f + fast_exp2(s * p.cap_in)), p.cap_out);
+            sr[c] = __float_as_uint(fmaf(-slope, fabsf(d0 - (float)c), x));
+          }
         }
-      }
+      };
+      if constexpr (MOD == kRaggedBias) biased(0);
       if (masked) {
 #pragma unroll
         for (int c = 0; c < 64; ++c) sr[c] = (c < rem && c >= low) ? sr[c] : __float_as_uint(-INFINITY);
@@ -545,10 +547,9 @@ __global__ void __launch_bounds__(384, 1)
       }
       mx0 = max3(mx0, __uint_as_float(sr[60]), __uint_as_float(sr[61]));
       mx1 = max3(mx1, __uint_as_float(sr[62]), __uint_as_float(sr[63]));
-      if constexpr (MOD != kRaggedBias) {
-        asm volatile("tcgen05.wait::ld.sync.aligned;" ::"f"(mx0), "f"(mx1), "f"(mx2), "f"(mx3) : "memory");
-        reg_fence_n<64>(sr + 64);
-      }
+      asm volatile("tcgen05.wait::ld.sync.aligned;" ::"f"(mx0), "f"(mx1), "f"(mx2), "f"(mx3) : "memory");
+      reg_fence_n<64>(sr + 64);
+      if constexpr (MOD == kRaggedBias) biased(64);
       if (masked) {
 #pragma unroll
         for (int c = 64; c < 128; ++c) sr[c] = (c < rem && c >= low) ? sr[c] : __float_as_uint(-INFINITY);
@@ -565,7 +566,7 @@ __global__ void __launch_bounds__(384, 1)
       if constexpr (MOD == kRaggedCap)
         mx = mx == -INFINITY ? mx : fmaf(-2.f * p.cap_out, fast_rcp(1.f + fast_exp2(mx * p.cap_in)), p.cap_out);
       const float m_new = fmaxf(m_run, mx);
-      const bool need = m_new > m_run + 8.0f;
+      const bool need = !idle && m_new > m_run + 8.0f;
       if (n > 0 && __any_sync(0xffffffffu, need)) {
         const float alpha = need ? fast_exp2(m_run - m_new) : 1.0f;
 #pragma unroll
@@ -618,7 +619,7 @@ __global__ void __launch_bounds__(384, 1)
             big1 = max3_abs(big1, __uint_as_float(sr[c + 2]), __uint_as_float(sr[c + 3]));
           }
         }
-        if (!any_masked && __all_sync(0xffffffffu, fmaxf(big, big1) <= p.cap_most)) {
+        if (!any_masked && __all_sync(0xffffffffu, idle || fmaxf(big, big1) <= p.cap_most)) {
           const float2 a0 = make_float2(p.cap_a[0], p.cap_a[0]), a1 = make_float2(p.cap_a[1], p.cap_a[1]);
           const float2 a2 = make_float2(p.cap_a[2], p.cap_a[2]), a3 = make_float2(p.cap_a[3], p.cap_a[3]);
           publish([&](float2 s) {
@@ -650,12 +651,13 @@ __global__ void __launch_bounds__(384, 1)
     }
     if (have_o) tc_fence_after();
 
-    if (solo && nk > 0) {
+    if (solo && work->nk > 0) {
       // Both warpgroups' MMAs are done after the first barrier, so the ring and Q are free:
       // the odd key tiles' O, m and l go through shared memory ([d][row] floats, rows
-      // fastest) into the even ones', whose warpgroup goes on alone.
-      float* const o1 = reinterpret_cast<float*>(smem + Cfg::kKVOff) + row;
-      float* const ml1 = reinterpret_cast<float*>(smem + Cfg::kKVOff + HD * 128 * 4) + row;
+      // fastest, past both warpgroups' staging tiles) into the even ones', whose warpgroup
+      // goes on alone.
+      float* const o1 = reinterpret_cast<float*>(smem + 2 * Cfg::kTileBytes) + row;
+      float* const ml1 = reinterpret_cast<float*>(smem + 2 * Cfg::kTileBytes + HD * 128 * 4) + row;
       asm volatile("bar.sync 3, 256;" ::: "memory");
       if (wg == 1) {
 #pragma unroll

@@ -382,6 +382,7 @@ int gqa_ragged_fwd(const gqa_ragged_args* args, void* stream) {
   if (a.softcap > 0.f) set_cap_polynomial(p, sc / a.softcap, a.softcap * kLog2e);
   p.v_scale = a.cache_fp8 ? a.v_scale : 1.f;
   p.mods = a.softcap > 0.f || a.alibi_slopes;
+  p.linear_bias = a.causal && !a.prefix_lens;
 
   RaggedPlan pl = plan_ragged(s, a.cache_fp8 != 0, sm);
   if (a.workspace) {
