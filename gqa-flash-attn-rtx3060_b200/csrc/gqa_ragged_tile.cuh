@@ -131,8 +131,6 @@ __global__ void __launch_bounds__(384, 1)
     int b, k_lo, k_hi;        // request; union of the rows' intervals
     int key0, nk, n_chunks;   // this CTA's first key, its 128-key tiles; chunks of the tile
     int unit;
-    int found;                // the scan's answer: request (-1: none) and tile of it
-    int local;
   };
   volatile Work* const work = reinterpret_cast<volatile Work*>(smem + Cfg::kWorkOff);
   int* const scan_sums = reinterpret_cast<int*>(smem + Cfg::kWorkOff + 64);
@@ -159,38 +157,62 @@ __global__ void __launch_bounds__(384, 1)
     *abort_flag = 0;
     fence_mbar_init();
     fence_proxy_async_smem();
-    work->found = -1;
   }
   pdl_wait();
   pdl_trigger();
 
-  // ---- which tile: count the tiles of every request that is this kernel's, and take
-  // number (total - 1 - tile_id). The first pass counts, the second finds; with at most
-  // 384 requests the lengths stay in registers in between.
+  // ---- which tile: count the tiles of every request that is this form's, and take number
+  // (total - 1 - tile_id). Everything about a request is loaded at once, so that the thread
+  // that finds the tile can describe it without another round trip.
+  struct Request {
+    int first, qn, len, prefix, tiles;
+  };
+  auto load = [&](int b) -> Request {
+    Request r{0, 0, 0, 0, 0};
+    if (b < p.n) {
+      r.first = p.cu[b];
+      r.qn = p.cu[b + 1];
+      r.len = p.seq_lens[b];
+      if (p.prefix) r.prefix = p.prefix[b];
+      (void)GQA_CHECK(r.len <= p.max_len, 906);
+      r.len = max(0, min(r.len, p.max_len));
+      r.qn = min(r.qn, p.num_tokens) - r.first;
+      if (r.first >= 0 && r.qn > 0 && (int64_t)r.qn * p.group >= tl.min_rows) r.tiles = (r.qn + tl.block_m - 1) / tl.block_m;
+    }
+    return r;
+  };
+  // The chunk's key range, from the union of the rows' intervals.
+  auto set_keys = [&](int k_lo, int k_hi) {
+    const int k_base = min(k_lo, k_hi) & ~(p.box - 1);  // where a box may start
+    const int k_first = k_base + split * tl.chunk;
+    const bool any = k_hi > k_lo;
+    work->k_lo = k_lo;
+    work->k_hi = k_hi;
+    work->key0 = k_first;
+    work->nk = any ? max(0, (min(k_first + tl.chunk, k_hi) - k_first + BN - 1) / BN) : 0;
+    work->n_chunks = any ? (k_hi - k_base + tl.chunk - 1) / tl.chunk : 1;
+  };
   {
-    auto tiles_of = [&](int b) -> int {
-      if (b >= p.n) return 0;
-      const int first = p.cu[b];
-      const int qn = min(p.cu[b + 1], p.num_tokens) - first;
-      if (first < 0 || qn <= 0 || (int64_t)qn * p.group < tl.min_rows) return 0;
-      return (qn + tl.block_m - 1) / tl.block_m;
-    };
     const int rounds = (p.n + 383) / 384;
-    const int mine = tiles_of(tid);
+    const Request mine = load(tid);
     int total = 0;
     for (int r = 0; r < rounds; ++r) {
-      const int s = __reduce_add_sync(0xffffffffu, r ? tiles_of(r * 384 + tid) : mine);
-      __syncthreads();
+      const int s = __reduce_add_sync(0xffffffffu, r ? load(r * 384 + tid).tiles : mine.tiles);
+      if (r) __syncthreads();
       if (lane == 0) scan_sums[warp] = s;
       __syncthreads();
       for (int w = 0; w < 12; ++w) total += scan_sums[w];
     }
     const int want = total - 1 - tile_id;
     if (want < 0) return;  // the whole CTA, before TMEM
+    if (warp == 8) {
+      tmem_alloc(smem_u32(tmem_base_ptr), Cfg::kTmemCols);
+      tmem_relinquish();
+    }
     int before = 0;
     for (int r = 0; r < rounds; ++r) {
-      const int c = r ? tiles_of(r * 384 + tid) : mine;
-      int incl = c;
+      const Request q = r ? load(r * 384 + tid) : mine;
+      int incl = q.tiles;
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) {
         const int y = __shfl_up_sync(0xffffffffu, incl, d);
@@ -206,46 +228,43 @@ __global__ void __launch_bounds__(384, 1)
         if (w < warp) at += scan_sums[w];
         before += scan_sums[w];
       }
-      at += incl - c;
-      if (c > 0 && want >= at && want < at + c) {
-        work->found = r * 384 + tid;
-        work->local = want - at;
+      at += incl - q.tiles;
+      if (want >= at && want < at + q.tiles) {
+        const int m0 = (want - at) * tl.block_m, nq = min(tl.block_m, q.qn - m0);
+        const int p_first = q.len - q.qn + m0;
+        int k_hi = q.len;
+        if (p.causal) k_hi = max(0, min(k_hi, max(p_first + nq, q.prefix)));
+        work->b = r * 384 + tid;
+        work->t0 = q.first + m0;
+        work->nq = nq;
+        work->off_m0 = p_first;
+        work->len = q.len;
+        work->unit = (int)(blockIdx.x / (unsigned)tl.nsplit);
+        set_keys(p.window > 0 ? max(0, p_first - p.window + 1) : 0, k_hi);
       }
     }
-    __syncthreads();
-  }
-  if (warp == 0) {
-    RaggedWork w;
-    const bool ok = ragged_work_at(p, tl, work->found, work->local * tl.block_m, lane, w);
-    if (lane == 0) {
-      const int k_first = w.k_base + split * tl.chunk;
-      work->t0 = w.t0;
-      work->nq = w.nq;
-      work->off_m0 = w.off + w.m0;
-      work->len = w.len;
-      work->b = w.b;
-      work->k_lo = w.k_lo;
-      work->k_hi = w.k_hi;
-      work->key0 = k_first;
-      work->nk = (ok && w.k_hi > w.k_lo) ? max(0, (min(k_first + tl.chunk, w.k_hi) - k_first + BN - 1) / BN) : 0;
-      work->n_chunks = ok ? w.n_chunks : 0;
-      work->unit = (int)(blockIdx.x / (unsigned)tl.nsplit);
-    }
-  }
-  __syncthreads();
-  if (split >= work->n_chunks) return;  // the whole CTA, before TMEM
-  const bool solo = work->nq <= bm;
-  const int slots = solo ? MAXS : Cfg::kPairSlots;                       // of each ring
-  const uint32_t k_ring = q_smem0 + (solo ? 1 : 2) * Cfg::kTileBytes;
-  const uint32_t v_ring = k_ring + slots * Cfg::kTileBytes;
-  if (warp == 8) {
-    tmem_alloc(smem_u32(tmem_base_ptr), Cfg::kTmemCols);
-    tmem_relinquish();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  if (p.key_starts) {
+    if (warp == 0) {
+      int s = INT_MAX;
+      for (int i = lane; i < work->nq; i += 32) s = min(s, p.key_starts[work->t0 + i]);
+      s = __reduce_min_sync(0xffffffffu, s);
+      if (lane == 0) set_keys(max(work->k_lo, s), work->k_hi);
+    }
+    __syncthreads();
+  }
   const uint32_t tmem_base = *tmem_base_ptr;
+  if (split >= work->n_chunks) {
+    if (warp == 8) tmem_dealloc(tmem_base, Cfg::kTmemCols);
+    return;
+  }
+  const bool solo = work->nq <= bm;
+  const int slots = solo ? MAXS : Cfg::kPairSlots;                       // of each ring
+  const uint32_t k_ring = q_smem0 + (solo ? 1 : 2) * Cfg::kTileBytes;
+  const uint32_t v_ring = k_ring + slots * Cfg::kTileBytes;
 
   // Register split as the dense prefill kernel's: 2 x 128 x 208 + 128 x 88 = 384 x 168.
   static_assert(Cfg::kSoftmaxRegs == 208 && Cfg::kControlRegs == 88, "keep the asm immediates in sync");
@@ -501,7 +520,7 @@ __global__ void __launch_bounds__(384, 1)
         for (int h = 0; h < Cfg::kPParts; ++h) mbar_arrive(p_full + 8 * h);
         continue;
       }
-      const bool masked = rem < BN || low > 0;
+      const bool cut_hi = __any_sync(0xffffffffu, rem < BN), cut_lo = __any_sync(0xffffffffu, low > 0);  // warp-uniform
       uint32_t sr[128];
       tmem_ld32(tS + 0, sr + 0);
       tmem_ld32(tS + 32, sr + 32);
@@ -531,10 +550,17 @@ __global__ void __launch_bounds__(384, 1)
         }
       };
       if constexpr (MOD == kRaggedBias) biased(0);
-      if (masked) {
+      auto mask = [&](int c0) {
+        if (cut_hi) {
 #pragma unroll
-        for (int c = 0; c < 64; ++c) sr[c] = (c < rem && c >= low) ? sr[c] : __float_as_uint(-INFINITY);
-      }
+          for (int c = c0; c < c0 + 64; ++c) sr[c] = (c < rem) ? sr[c] : __float_as_uint(-INFINITY);
+        }
+        if (cut_lo) {
+#pragma unroll
+          for (int c = c0; c < c0 + 64; ++c) sr[c] = (c >= low) ? sr[c] : __float_as_uint(-INFINITY);
+        }
+      };
+      mask(0);
       // Row max with three-input maxima, four independent chains.
       float mx0 = __uint_as_float(sr[0]), mx1 = __uint_as_float(sr[1]);
       float mx2 = __uint_as_float(sr[2]), mx3 = __uint_as_float(sr[3]);
@@ -550,10 +576,7 @@ __global__ void __launch_bounds__(384, 1)
       asm volatile("tcgen05.wait::ld.sync.aligned;" ::"f"(mx0), "f"(mx1), "f"(mx2), "f"(mx3) : "memory");
       reg_fence_n<64>(sr + 64);
       if constexpr (MOD == kRaggedBias) biased(64);
-      if (masked) {
-#pragma unroll
-        for (int c = 64; c < 128; ++c) sr[c] = (c < rem && c >= low) ? sr[c] : __float_as_uint(-INFINITY);
-      }
+      mask(64);
 #pragma unroll
       for (int c = 64; c < 128; c += 8) {
         mx0 = max3(mx0, __uint_as_float(sr[c]), __uint_as_float(sr[c + 1]));
@@ -611,7 +634,7 @@ __global__ void __launch_bounds__(384, 1)
       const float2 nm2 = make_float2(-m_run, -m_run);
       if constexpr (MOD == kRaggedCap) {
         float big = 0.f, big1 = 0.f;
-        const bool any_masked = __any_sync(0xffffffffu, masked);
+        const bool any_masked = cut_hi || cut_lo;
         if (!any_masked) {
 #pragma unroll
           for (int c = 0; c < 128; c += 4) {
@@ -651,70 +674,78 @@ __global__ void __launch_bounds__(384, 1)
     }
     if (have_o) tc_fence_after();
 
-    if (solo && work->nk > 0) {
-      // Both warpgroups' MMAs are done after the first barrier, so the ring and Q are free:
-      // the odd key tiles' O, m and l go through shared memory ([d][row] floats, rows
-      // fastest, past both warpgroups' staging tiles) into the even ones', whose warpgroup
-      // goes on alone.
-      float* const o1 = reinterpret_cast<float*>(smem + 2 * Cfg::kTileBytes) + row;
-      float* const ml1 = reinterpret_cast<float*>(smem + 2 * Cfg::kTileBytes + HD * 128 * 4) + row;
+    // What this thread writes of its row: all of it, or of a solo tile this warpgroup's
+    // half of the columns, in chunks of 32.
+    const int c_begin = solo ? wg * (HD / 64) : 0, c_end = solo ? c_begin + HD / 64 : HD / 32;
+    const int prow = (solo ? 0 : wg * 128) + row;  // row of the tile's 256 packed rows
+    float w_own = 1.f, w_other = 0.f;
+    const float* other = nullptr;
+    if (solo) {
+      // The warpgroups' O, m and l of the same rows: each gives the other, through shared
+      // memory ([warpgroup][column][row] floats, rows fastest, past the staging tile), the
+      // half that the other writes. After the first barrier both are done with the ring.
+      float* const xo = reinterpret_cast<float*>(smem + Cfg::kTileBytes);
+      float* const xm = xo + HD * 128;
       asm volatile("bar.sync 3, 256;" ::: "memory");
-      if (wg == 1) {
+      if (!idle_warp) {
+        const int oc = (1 - wg) * (HD / 64);
+        float* const to = xo + wg * (HD / 2) * 128 + row;
 #pragma unroll
-        for (int c = 0; c < HD / 32; ++c) {
+        for (int c = 0; c < HD / 64; ++c) {
           uint32_t orr[32];
           if (have_o) {
-            tmem_ld32(tO + c * 32, orr);
+            tmem_ld32(tO + (oc + c) * 32, orr);
             tmem_wait_ld();
             reg_fence(orr);
-          } else {
-#pragma unroll
-            for (int e = 0; e < 32; ++e) orr[e] = 0u;
           }
 #pragma unroll
-          for (int e = 0; e < 32; ++e) o1[(c * 32 + e) * 128] = __uint_as_float(orr[e]);
+          for (int e = 0; e < 32; ++e) to[(c * 32 + e) * 128] = have_o ? __uint_as_float(orr[e]) : 0.f;
         }
-        ml1[0] = m_run;
-        ml1[128] = l_run;
+        xm[wg * 256 + row] = m_run;
+        xm[wg * 256 + 128 + row] = l_run;
       }
       asm volatile("bar.sync 3, 256;" ::: "memory");
-      if (wg == 0 && have_o) {
-        const float M1 = ml1[0], Mx = fmaxf(m_run, M1);
-        const float w0 = fast_exp2(m_run - Mx), w1 = fast_exp2(M1 - Mx);
-        l_run = w0 * l_run + w1 * ml1[128];
-        m_run = Mx;
-#pragma unroll
-        for (int c = 0; c < HD / 32; ++c) {
-          uint32_t orr[32];
-          tmem_ld32(tO + c * 32, orr);
-          tmem_wait_ld();
-          reg_fence(orr);
-#pragma unroll
-          for (int e = 0; e < 32; ++e)
-            orr[e] = __float_as_uint(w0 * __uint_as_float(orr[e]) + w1 * o1[(c * 32 + e) * 128]);
-          tmem_st32(tO + c * 32, orr);
-        }
-        tmem_wait_st();
+      if (!idle_warp) {
+        const float m1 = xm[(1 - wg) * 256 + row], l1 = xm[(1 - wg) * 256 + 128 + row];
+        const float mx = fmaxf(m_run, m1);
+        w_own = have_o ? fast_exp2(m_run - mx) : 0.f;
+        w_other = fast_exp2(m1 - mx);
+        // In the even tiles' warpgroup's order, so that both get the same sum.
+        const float a = w_own * l_run, b = w_other * l1;
+        l_run = wg ? b + a : a + b;
+        m_run = mx;
+        other = xo + (1 - wg) * (HD / 2) * 128 + row;
       }
     }
-    const bool merged_away = solo && wg == 1;  // nothing left to write
 
     const int n_chunks = work->n_chunks, unit = work->unit;
     float L = l_run, M = m_run;
-    bool store = !merged_away;
-    const int prow = wg * 128 + row;  // row of the pair's 256 packed rows
-    const int64_t pbase = (int64_t)unit * tl.nsplit * 256 + prow;
-    if (n_chunks > 1) {
-      // Publish this chunk's partial, m, l [split][256 rows] and acc [split][d][256 rows];
-      // the tile's last CTA (ticket) folds them in chunk order.
-      if (!merged_away) {
-        __stcg(tl.ws_m + pbase + (int64_t)split * 256, m_run);
-        __stcg(tl.ws_l + pbase + (int64_t)split * 256, l_run);
-      }
-      float* acc_own = tl.ws_acc + ((int64_t)unit * tl.nsplit + split) * HD * 256 + prow;
+    bool store = true;
+    const uint32_t stage = q_smem0 + (solo ? 0 : wg) * Cfg::kTileBytes;
+    auto stage_chunk = [&](int c, const uint32_t (&orr)[32], float inv) {
 #pragma unroll
-      for (int c = 0; c < HD / 32; ++c) {
-        if (merged_away) break;
+      for (int e = 0; e < 4; ++e) {
+        const int chunk = 4 * c + e;  // 16-byte chunk along d
+#define GQA_OV(i) (__uint_as_float(orr[8 * e + (i)]) * inv)
+        const uint32_t w0 = pack2<BF16>(GQA_OV(0), GQA_OV(1));
+        const uint32_t w1 = pack2<BF16>(GQA_OV(2), GQA_OV(3));
+        const uint32_t w2 = pack2<BF16>(GQA_OV(4), GQA_OV(5));
+        const uint32_t w3 = pack2<BF16>(GQA_OV(6), GQA_OV(7));
+#undef GQA_OV
+        const uint32_t dst = stage + (chunk >> 3) * Cfg::kSubBytes + sw128_off(row, chunk & 7);
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(w0), "r"(w1), "r"(w2), "r"(w3)
+                     : "memory");
+      }
+    };
+    auto inverse = [](float l) { return l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l); };  // no key seen: 0; NaN stays NaN
+    const int64_t pbase = (int64_t)unit * tl.nsplit * 256 + prow;
+    if (!idle_warp) {
+      // O of the chunk to the staging tile, or, if the tile has several chunks, its partial:
+      // m, l [split][256 rows] and acc [split][d][256 rows].
+      const float inv = inverse(l_run);
+      float* acc_own = tl.ws_acc + ((int64_t)unit * tl.nsplit + split) * HD * 256 + prow;
+#pragma unroll 1
+      for (int c = c_begin; c < c_end; ++c) {
         uint32_t orr[32];
         if (have_o) {
           tmem_ld32(tO + c * 32, orr);
@@ -724,9 +755,26 @@ __global__ void __launch_bounds__(384, 1)
 #pragma unroll
           for (int e = 0; e < 32; ++e) orr[e] = ok ? 0u : 0x7fc00000u;
         }
+        if (solo) {
+          const float* x = other + (c - c_begin) * 32 * 128;
 #pragma unroll
-        for (int e = 0; e < 32; ++e) __stcg(acc_own + (c * 32 + e) * 256, __uint_as_float(orr[e]));
+          for (int e = 0; e < 32; ++e)
+            orr[e] = __float_as_uint(fmaf(w_other, x[e * 128], w_own * __uint_as_float(orr[e])));
+        }
+        if (n_chunks == 1) {
+          stage_chunk(c, orr, inv);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) __stcg(acc_own + (c * 32 + e) * 256, __uint_as_float(orr[e]));
+        }
       }
+      if (n_chunks > 1 && c_begin == 0) {
+        __stcg(tl.ws_m + pbase + (int64_t)split * 256, m_run);
+        __stcg(tl.ws_l + pbase + (int64_t)split * 256, l_run);
+      }
+    }
+    if (n_chunks > 1) {
+      // The tile's last CTA (ticket) folds the chunks in their order.
       asm volatile("bar.sync 3, 256;" ::: "memory");
       uint32_t* last_slot = tmem_base_ptr + 2;
       if (tid == 0) {
@@ -737,8 +785,8 @@ __global__ void __launch_bounds__(384, 1)
         if (last) tl.ws_cnt[unit] = 0u;
       }
       asm volatile("bar.sync 3, 256;" ::: "memory");
-      store = *last_slot != 0 && !merged_away;
-      if (store) {
+      store = *last_slot != 0;
+      if (store && !idle_warp) {
         for (int s0 = 0; s0 < n_chunks; s0 += 4) {
           float mv[4];
 #pragma unroll
@@ -759,78 +807,74 @@ __global__ void __launch_bounds__(384, 1)
           for (int i = 0; i < 4; ++i)
             if (s0 + i < n_chunks) L += fast_exp2(mv[i] - M) * lv[i];
         }
-      }
-    }
-    const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);  // no key seen: 0; a NaN sum stays NaN
-    const uint32_t stage = q_smem0 + wg * Cfg::kTileBytes;
+        const float inv = inverse(L);
+#pragma unroll 1
+        for (int c = c_begin; c < c_end; ++c) {
+          // Two chunks per pass: 64 independent loads in flight per thread. An index past
+          // the last chunk reads a valid partial at weight 0.
+          uint32_t orr[32];
 #pragma unroll
-    for (int c = 0; c < HD / 32; ++c) {
-      uint32_t orr[32];
-      if (n_chunks > 1) {
-        // Two chunks per pass: 64 independent loads in flight per thread. An index past
-        // the last chunk reads a valid partial at weight 0.
+          for (int e = 0; e < 32; ++e) orr[e] = 0u;
+          for (int s0 = 0; s0 < n_chunks; s0 += 2) {
+            const int sa = s0, sb = min(s0 + 1, n_chunks - 1);
+            const float wa = fast_exp2(__ldcg(tl.ws_m + pbase + (int64_t)sa * 256) - M);
+            const float wb = (s0 + 1 >= n_chunks) ? 0.f : fast_exp2(__ldcg(tl.ws_m + pbase + (int64_t)sb * 256) - M);
+            const float* xa = tl.ws_acc + ((int64_t)unit * tl.nsplit + sa) * HD * 256 + prow + c * 32 * 256;
+            const float* xb = tl.ws_acc + ((int64_t)unit * tl.nsplit + sb) * HD * 256 + prow + c * 32 * 256;
+            float va[32], vb[32];
 #pragma unroll
-        for (int e = 0; e < 32; ++e) orr[e] = 0u;
-        for (int s0 = 0; store && s0 < n_chunks; s0 += 2) {
-          const int sa = s0, sb = min(s0 + 1, n_chunks - 1);
-          const float wa = fast_exp2(__ldcg(tl.ws_m + pbase + (int64_t)sa * 256) - M);
-          const float wb = (s0 + 1 >= n_chunks) ? 0.f : fast_exp2(__ldcg(tl.ws_m + pbase + (int64_t)sb * 256) - M);
-          const float* xa = tl.ws_acc + ((int64_t)unit * tl.nsplit + sa) * HD * 256 + prow + c * 32 * 256;
-          const float* xb = tl.ws_acc + ((int64_t)unit * tl.nsplit + sb) * HD * 256 + prow + c * 32 * 256;
-          float va[32], vb[32];
+            for (int e = 0; e < 32; ++e) {
+              va[e] = __ldcg(xa + e * 256);
+              vb[e] = __ldcg(xb + e * 256);
+            }
 #pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            va[e] = __ldcg(xa + e * 256);
-            vb[e] = __ldcg(xb + e * 256);
+            for (int e = 0; e < 32; ++e)
+              orr[e] = __float_as_uint(fmaf(wb, vb[e], fmaf(wa, va[e], __uint_as_float(orr[e]))));
           }
-#pragma unroll
-          for (int e = 0; e < 32; ++e)
-            orr[e] = __float_as_uint(fmaf(wb, vb[e], fmaf(wa, va[e], __uint_as_float(orr[e]))));
+          stage_chunk(c, orr, inv);
         }
-      } else if (have_o) {
-        tmem_ld32(tO + c * 32, orr);
-        tmem_wait_ld();
-        reg_fence(orr);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 32; ++e) orr[e] = ok ? 0u : 0x7fc00000u;
-      }
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int chunk = 4 * c + e;  // 16-byte chunk along d
-#define GQA_OV(i) (__uint_as_float(orr[8 * e + (i)]) * inv)
-        const uint32_t w0 = pack2<BF16>(GQA_OV(0), GQA_OV(1));
-        const uint32_t w1 = pack2<BF16>(GQA_OV(2), GQA_OV(3));
-        const uint32_t w2 = pack2<BF16>(GQA_OV(4), GQA_OV(5));
-        const uint32_t w3 = pack2<BF16>(GQA_OV(6), GQA_OV(7));
-#undef GQA_OV
-        const uint32_t dst = stage + (chunk >> 3) * Cfg::kSubBytes + sw128_off(row, chunk & 7);
-        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(w0), "r"(w1), "r"(w2), "r"(w3)
-                     : "memory");
       }
     }
-    if (wg == 0)
+    // The staging tile is complete: one warpgroup's, or of a solo tile both's.
+    if (solo)
+      asm volatile("bar.sync 3, 256;" ::: "memory");
+    else if (wg == 0)
       asm volatile("bar.sync 1, 128;" ::: "memory");
     else
       asm volatile("bar.sync 2, 128;" ::: "memory");
     if (store) {
-      const int rows = max(0, min(work->nq - wg * bm, bm)) * p.group;  // rows of real tokens
-      const int tok0 = work->t0 + wg * bm;
-      if (p.lse && row < rows)
-        p.lse[(int64_t)(tok0 + row / p.group) * p.hq + kvh * p.group + row % p.group] =
+      const int rows = max(0, min(work->nq - (solo ? 0 : wg * bm), bm)) * p.group;  // rows of real tokens
+      const int tok0 = work->t0 + (solo ? 0 : wg * bm);
+      if (p.lse && row < rows && c_begin == 0)
+        p.lse[(int64_t)(tok0 + m_row) * p.hq + kvh * p.group + row % p.group] =
             L == 0.f ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
-      // 16 bytes per thread, a row's pieces on neighbouring threads.
+      // 16 bytes per thread, a row's pieces on neighbouring threads, `step` rows apart.
       constexpr int kPer = HD / 8;
-      for (int idx = row; idx < rows * kPer; idx += 128) {
-        const int r = idx / kPer, chunk = idx % kPer;
-        uint32_t w0, w1, w2, w3;
-        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                     : "=r"(w0), "=r"(w1), "=r"(w2), "=r"(w3)
-                     : "r"(stage + (chunk >> 3) * Cfg::kSubBytes + sw128_off(r, chunk & 7))
-                     : "memory");
-        const int tok = tok0 + r / p.group, head = kvh * p.group + r % p.group;
-        *reinterpret_cast<uint4*>(p.o + (int64_t)tok * p.o_st + (int64_t)head * p.o_sh + chunk * 8) =
-            make_uint4(w0, w1, w2, w3);
+      const int step = (solo ? 256 : 128) / kPer, chunk = tid % kPer;
+      int r = (solo ? tid : row) / kPer;
+      int tok = r / p.group, head = r - tok * p.group;
+      const int d_tok = step / p.group, d_head = step - d_tok * p.group;
+      uint16_t* const o0 = p.o + (int64_t)tok0 * p.o_st + (int64_t)kvh * p.group * p.o_sh + chunk * 8;
+      const uint32_t s0 = stage + (chunk >> 3) * Cfg::kSubBytes;
+      for (; r < rows; r += 4 * step) {
+        uint4 x[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          if (r + u * step < rows)
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(x[u].x), "=r"(x[u].y), "=r"(x[u].z), "=r"(x[u].w)
+                         : "r"(s0 + sw128_off(r + u * step, chunk & 7))
+                         : "memory");
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          if (r + u * step < rows) *reinterpret_cast<uint4*>(o0 + (int64_t)tok * p.o_st + (int64_t)head * p.o_sh) = x[u];
+          tok += d_tok;
+          head += d_head;
+          if (head >= p.group) {
+            head -= p.group;
+            ++tok;
+          }
+        }
       }
     }
   }

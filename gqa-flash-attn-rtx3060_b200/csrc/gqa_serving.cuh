@@ -34,9 +34,9 @@ int prepare_ragged() {
   int rc = GQA_OK;
   auto prep = [&](auto kernel, int smem, int regs) {
     if (set_smem(kernel, smem) != cudaSuccess) rc = rc ? rc : GQA_ERR_CUDA;
-    if (!rc && regs) rc = check_reg_split(kernel, PrefillCfg<128>::kThreads, regs);
+    if (!rc && regs) rc = check_reg_split(kernel, RaggedTileCfg<128>::kThreads, regs);
   };
-  constexpr int kRegs = PrefillCfg<128>::kRegsNeeded;
+  constexpr int kRegs = RaggedTileCfg<128>::kRegsNeeded;
 #define GQA_PREP_RAGGED(HD, BF)                                                              \
   prep(gqa_ragged_tile_kernel<HD, BF, kRaggedPlain>, RaggedTileCfg<HD>::kSmemBytes, kRegs);  \
   prep(gqa_ragged_tile_kernel<HD, BF, kRaggedCap>, RaggedTileCfg<HD>::kSmemBytes, kRegs);    \
@@ -81,14 +81,15 @@ int ragged_span(const RaggedShape& s, int block_m) {
   return (int)std::max<int64_t>(1, span);
 }
 
-// Key split of `units` tiles that see up to `stages` 128-key stages each; a CTA's fixed
-// cost is `fixed` stages. The lengths are not known here. One request: its length is the
+// Key split of `units` tiles that see up to `span` keys each, `keys` at a time (a stage);
+// a CTA's fixed cost is `fixed` stages. The lengths are not known here. One request: its length is the
 // bound, and the split that gives the fewest wave-stages is taken. Several: lengths
 // between a quarter of the bound and the bound are assumed, the CTAs dealt to the SMs as
 // they come free, so that the time is the mean load plus half of the last CTA's.
-void split_keys(RaggedTiling& t, int64_t units, int stages, int n, int sm_count, double fixed, int most) {
+void split_keys(RaggedTiling& t, int64_t units, int span, int keys, int n, int sm_count, double fixed, int most) {
+  const int stages = (span + keys - 1) / keys;
   t.nsplit = 1;
-  t.chunk = stages * 128;
+  t.chunk = stages * keys;
   double best = 1e300;
   for (int ns = 1; ns <= std::min(stages, most); ++ns) {
     const int chunk = (stages + ns - 1) / ns;
@@ -103,7 +104,7 @@ void split_keys(RaggedTiling& t, int64_t units, int stages, int n, int sm_count,
     if (cost < best - 1e-9) {
       best = cost;
       t.nsplit = ns;
-      t.chunk = chunk * 128;
+      t.chunk = chunk * keys;
     }
   }
 }
@@ -124,13 +125,10 @@ RaggedPlan plan_ragged(const RaggedShape& s, bool fp8, int sm_count) {
     const int64_t longest = std::min<int64_t>(s.n, (int64_t)s.tokens * s.group / std::max(1, t.min_rows));
     t.slots = (int)std::min<int64_t>((int64_t)s.tokens / t.block_m + longest, INT_MAX);
     const int64_t units = tiling_units(t, s.hkv);
-    const int stages = (ragged_span(s, t.block_m) + 127) / 128;
-    if (units < sm_count && units <= kServingCounters / 2) {
-      split_keys(t, units, stages, s.n, sm_count, 6.0, std::max(1, std::min(16, stages / 2)));
-    } else {
-      t.nsplit = 1;
-      t.chunk = stages * 128;
-    }
+    const int keys = s.head_dim == 128 ? RaggedTileCfg<128>::kBN : RaggedTileCfg<64>::kBN;
+    const int span = ragged_span(s, t.block_m) + keys;
+    const int most = (units < sm_count && units <= kServingCounters / 2) ? std::max(1, std::min(16, span / (2 * keys))) : 1;
+    split_keys(t, units, span, keys, s.n, sm_count, 6.0, most);
     pl.tile_ctas = units * t.nsplit;
   }
   if (stream) {
@@ -143,13 +141,8 @@ RaggedPlan plan_ragged(const RaggedShape& s, bool fp8, int sm_count) {
     t.min_rows = 0;
     t.max_rows = tile ? stream_rows : INT_MAX;
     const int64_t tiles = t.one_tile ? std::min(s.n, s.tokens) : std::min(t.slots, s.tokens);
-    const int stages = (ragged_span(s, t.block_m) + 127) / 128;
-    if (tiling_units(t, s.hkv) <= kServingCounters / 2) {
-      split_keys(t, tiles * s.hkv, stages, s.n, sm_count, 3.0, kMaxSplits);
-    } else {
-      t.nsplit = 1;
-      t.chunk = stages * 128;
-    }
+    split_keys(t, tiles * s.hkv, ragged_span(s, t.block_m), 128, s.n, sm_count, 3.0,
+               tiling_units(t, s.hkv) <= kServingCounters / 2 ? kMaxSplits : 1);
     pl.stream_ctas = tiling_units(t, s.hkv) * t.nsplit;
   }
   return pl;
@@ -362,7 +355,6 @@ int gqa_ragged_fwd(const gqa_ragged_args* args, void* stream) {
   p.bt_stride = a.bt_stride;
   p.block_shift = pow2_shift(a.block_size);
   p.num_blocks = a.num_blocks;
-  p.box = std::min(64, a.block_size);
   p.alibi = a.alibi_slopes;
   p.prefix = a.prefix_lens;
   p.key_starts = a.key_starts;
@@ -397,13 +389,14 @@ int gqa_ragged_fwd(const gqa_ragged_args* args, void* stream) {
     pl.stream_ctas /= std::max(1, pl.stream.nsplit);
     pl.tile_ctas /= std::max(1, pl.tile.nsplit);
     pl.stream.nsplit = pl.tile.nsplit = 1;
-    pl.stream.chunk = pl.tile.chunk = std::max(1, (a.max_seq_len + 127) / 128) * 128;
+    pl.stream.chunk = pl.tile.chunk = INT_MAX / 2 / 640 * 640;  // one chunk, a multiple of both forms' stages
   }
   if (pl.tile_ctas + pl.stream_ctas > INT_MAX) return GQA_ERR_INVALID_ARG;
   const unsigned grid = (unsigned)(pl.tile_ctas + pl.stream_ctas);
   p.stream = pl.stream;
   p.tile = pl.tile;
   p.tile_ctas = (unsigned)pl.tile_ctas;
+  p.box = std::min(64, a.block_size);
 
   CUtensorMap km, vm;
   rc = make_cache_map(&km, a.k_cache, a.k_strides, a.num_blocks, a.block_size, a.num_kv_heads, a.head_dim, p.box, a.cache_fp8);
