@@ -81,12 +81,11 @@ int ragged_span(const RaggedShape& s, int block_m) {
   return (int)std::max<int64_t>(1, span);
 }
 
-// Key split of `units` tiles that see up to `span` keys each, `keys` at a time (a stage);
-// a CTA's fixed cost is `fixed` stages. The lengths are not known here. One request: its length is the
-// bound, and the split that gives the fewest wave-stages is taken. Several: lengths
-// between a quarter of the bound and the bound are assumed, the CTAs dealt to the SMs as
-// they come free, so that the time is the mean load plus half of the last CTA's.
-void split_keys(RaggedTiling& t, int64_t units, int span, int keys, int n, int sm_count, double fixed, int most) {
+// Key split of `units` tiles that see up to `span` keys each, `keys` at a time (a stage),
+// for one CTA per SM: the split of the fewest wave-stages, a CTA's fixed cost (set-up,
+// pipeline ramp, merge, partials) counting `fixed` stages. Only the longest request's
+// bound is known; shorter ones use fewer chunks and their CTAs return at once.
+void split_keys(RaggedTiling& t, int64_t units, int span, int keys, int sm_count, double fixed, int most) {
   const int stages = (span + keys - 1) / keys;
   t.nsplit = 1;
   t.chunk = stages * keys;
@@ -94,13 +93,7 @@ void split_keys(RaggedTiling& t, int64_t units, int span, int keys, int n, int s
   for (int ns = 1; ns <= std::min(stages, most); ++ns) {
     const int chunk = (stages + ns - 1) / ns;
     if ((stages + chunk - 1) / chunk != ns) continue;
-    double cost;
-    if (n == 1) {
-      cost = std::ceil((double)units * ns / sm_count) * (chunk + fixed);
-    } else {
-      const double load = (double)units * (0.625 * stages + (0.625 * ns + 0.5) * fixed) / sm_count;
-      cost = std::max(chunk + fixed, load + 0.5 * (chunk + fixed));
-    }
+    const double cost = std::ceil((double)units * ns / sm_count) * (chunk + fixed);
     if (cost < best - 1e-9) {
       best = cost;
       t.nsplit = ns;
@@ -128,7 +121,7 @@ RaggedPlan plan_ragged(const RaggedShape& s, bool fp8, int sm_count) {
     const int keys = s.head_dim == 128 ? RaggedTileCfg<128>::kBN : RaggedTileCfg<64>::kBN;
     const int span = ragged_span(s, t.block_m) + keys;
     const int most = (units < sm_count && units <= kServingCounters / 2) ? std::max(1, std::min(16, span / (2 * keys))) : 1;
-    split_keys(t, units, span, keys, s.n, sm_count, 6.0, most);
+    split_keys(t, units, span, keys, sm_count, 12.0, most);
     pl.tile_ctas = units * t.nsplit;
   }
   if (stream) {
@@ -141,7 +134,7 @@ RaggedPlan plan_ragged(const RaggedShape& s, bool fp8, int sm_count) {
     t.min_rows = 0;
     t.max_rows = tile ? stream_rows : INT_MAX;
     const int64_t tiles = t.one_tile ? std::min(s.n, s.tokens) : std::min(t.slots, s.tokens);
-    split_keys(t, tiles * s.hkv, ragged_span(s, t.block_m), 128, s.n, sm_count, 3.0,
+    split_keys(t, tiles * s.hkv, ragged_span(s, t.block_m), 128, sm_count, 4.0,
                tiling_units(t, s.hkv) <= kServingCounters / 2 ? kMaxSplits : 1);
     pl.stream_ctas = tiling_units(t, s.hkv) * t.nsplit;
   }
@@ -264,13 +257,14 @@ int gqa_qk_norm_rope(const gqa_qk_norm_rope_args* args, void* stream) {
   if (cached && (!a.v_dst || a.block_size <= 0 || a.num_blocks < 0)) return GQA_ERR_INVALID_ARG;
   if (!cached && (a.v_dst || a.cache_fp8)) return GQA_ERR_INVALID_ARG;
   if (a.cache_fp8 && !(a.k_scale > 0.f && a.v_scale > 0.f)) return GQA_ERR_INVALID_ARG;
-  if (!aligned16(a.q_out) || !aligned16(a.k_dst) || !aligned16(a.v_dst) || !aligned16(a.q_weight) || !aligned16(a.k_weight))
+  if (!aligned16(a.q_out) || !aligned16(a.cos_sin) || !aligned16(a.k_dst) || !aligned16(a.v_dst) || !aligned16(a.q_weight) || !aligned16(a.k_weight))
     return GQA_ERR_ALIGNMENT;
   int rc = check_strides3(a.q, a.q_strides, 8);
   if (!rc) rc = check_strides3(a.k, a.k_strides, 8);
   if (!rc && cached) rc = check_strides3(a.v, a.v_strides, 8);
   if (rc) return rc;
-  rc = current_device(nullptr);
+  int sm = 0;
+  rc = current_device(&sm);
   if (rc) return rc;
   p.q = reinterpret_cast<const uint16_t*>(a.q);
   p.k = reinterpret_cast<const uint16_t*>(a.k);
@@ -294,20 +288,23 @@ int gqa_qk_norm_rope(const gqa_qk_norm_rope_args* args, void* stream) {
   p.rot = a.rotary_dim;
   p.axes = a.axes;
   p.max_pos = a.max_positions;
-  p.interleaved = a.interleaved ? 1 : 0;
   p.eps = a.eps;
   p.k_scale = a.k_scale;
   p.v_scale = a.v_scale;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const bool bf = a.dtype == GQA_DTYPE_BF16;
-  const dim3 grid(a.num_tokens);
+  const int item_rows = a.head_dim == 128 ? RopeCfg<128>::kItemRows : RopeCfg<64>::kItemRows;
+  const int64_t items = (int64_t)a.num_tokens * ((a.num_heads + 2 * a.num_kv_heads + item_rows - 1) / item_rows);
+  const dim3 grid((unsigned)std::min<int64_t>(items, kRopeCtas * sm));
   cudaError_t e;
-#define GQA_ROPE(D)                                                                    \
-  e = a.cache_fp8 ? (bf ? launch_pdl(gqa_rope_kernel<D, true, true>, grid, 256, 0, st, p) \
-                      : launch_pdl(gqa_rope_kernel<D, false, true>, grid, 256, 0, st, p)) \
-                : (bf ? launch_pdl(gqa_rope_kernel<D, true, false>, grid, 256, 0, st, p) \
-                      : launch_pdl(gqa_rope_kernel<D, false, false>, grid, 256, 0, st, p))
-  if (a.head_dim == 128) { GQA_ROPE(128); } else { GQA_ROPE(64); }
+#define GQA_ROPE(D, BF, F8)                                                                                     \
+  e = a.interleaved ? launch_pdl(gqa_rope_kernel<D, BF, F8, true>, grid, kRopeThreads, 0, st, p)                \
+                    : launch_pdl(gqa_rope_kernel<D, BF, F8, false>, grid, kRopeThreads, 0, st, p)
+#define GQA_ROPE_D(D)                                                                                           \
+  if (a.cache_fp8) { if (bf) { GQA_ROPE(D, true, true); } else { GQA_ROPE(D, false, true); } }                  \
+  else { if (bf) { GQA_ROPE(D, true, false); } else { GQA_ROPE(D, false, false); } }
+  if (a.head_dim == 128) { GQA_ROPE_D(128) } else { GQA_ROPE_D(64) }
+#undef GQA_ROPE_D
 #undef GQA_ROPE
   return e == cudaSuccess ? GQA_OK : GQA_ERR_CUDA;
 }

@@ -38,8 +38,8 @@ def _launch(q, k, v, positions, cos_sin, k_dst, v_dst, slots, block_size, num_bl
     if positions.dtype != torch.int32 or positions.dim() not in (1, 2) or positions.shape[-1] != num_tokens:
         raise ValueError("positions must be int32 (num_tokens,) or (axes, num_tokens)")
     axes = 1 if positions.dim() == 1 else positions.shape[0]
-    if cos_sin.dtype != torch.float32 or cos_sin.dim() != 2 or not cos_sin.is_contiguous():
-        raise ValueError("cos_sin must be a contiguous float32 (max_positions, rotary_dim)")
+    if cos_sin.dtype != torch.float32 or cos_sin.dim() != 2 or not cos_sin.is_contiguous() or cos_sin.data_ptr() & 15:
+        raise ValueError("cos_sin must be a contiguous, 16-byte aligned float32 (max_positions, rotary_dim)")
     max_positions, rotary_dim = cos_sin.shape
     if rotary_dim > head_dim or rotary_dim % 16:
         raise ValueError("rotary_dim must be a multiple of 16, at most head_dim")
