@@ -9,14 +9,17 @@
 // With several position axes (time, height, width) the frequencies are dealt to the axes
 // in consecutive sections.
 //
-// Bound by HBM: 2 x 2 B per value of q, k and v. D / 8 lanes hold one head's row, 16 bytes
-// per lane, and keep their cosines and sines in registers for all the token's heads that
-// they take, so the table is read once per token and lane group instead of once per head.
-// A token's heads are one item of work for a CTA (more than kRows per lane group: several
-// items). CTAs stay resident and go from item to item with the next item's position and slot
-// in flight, so that an item's rows and table entries leave together at its start; four
-// CTAs per SM overlap one item's latency with another's arithmetic. ROPE_FIGURES Everything
-// between the load and the one rounding of the store is fp32.
+// Bound by HBM (2 x 2 B per value of q, k and v) once it is not bound by instructions: the
+// norm and the rotation of a 16-bit value leave about ten of them per 4 bytes moved. So
+// D / 8 lanes hold one head's row as two 8-byte pieces, four values a and their four
+// partners b (no shuffles; for neighbouring pairs and for values past `rot` the pieces are
+// neighbours), arithmetic is packed two values at a time, and the work is cut into units
+// of two rows that share cosines and sines: two query heads, or a head's key and value, of
+// one token. Query and key-value units are different CTAs, so that a unit has no branches
+// on what a row is, and a lane group goes through its units by additions. The next unit's
+// position and slot are in flight while this one is turned, and its rows and table entries
+// leave together; ROPE_FIGURES. Everything between the load and the one rounding of the
+// store is fp32.
 #pragma once
 
 #include "gqa_cache.cuh"
@@ -41,221 +44,277 @@ struct RopeParams {
   const int64_t* slots;  // (T,), or null: k_dst is indexed by token
   int64_t num_slots;
   int num_tokens, hq, hkv, rot, axes, max_pos;
+  int q_ctas;  // CTAs of query units, the grid's first; the rest take keys and values
   int section_end[kMaxAxes];  // first frequency past each axis' section
   float eps, k_scale, v_scale;
 };
 
-// Eight 16-bit values as floats.
-template <bool BF16>
-__device__ __forceinline__ void unpack8(const uint4& x, float (&f)[8]) {
-  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 y = to_f32x2<BF16>(w[i]);
-    f[2 * i] = y.x;
-    f[2 * i + 1] = y.y;
-  }
+// Packed products of two values (one instruction; each rounded as the scalar one).
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 ra, rb, rd;\n\t"
+      "mov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\t"
+      "mul.rn.f32x2 rd, ra, rb;\n\tmov.b64 {%0, %1}, rd;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
 }
-template <bool BF16>
-__device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
-  return make_uint4(pack2<BF16>(f[0], f[1]), pack2<BF16>(f[2], f[3]), pack2<BF16>(f[4], f[5]),
-                    pack2<BF16>(f[6], f[7]));
-}
-// Eight floats over `scale`, as e4m3 (the cache write's rule: rounded to nearest even, saturated).
-__device__ __forceinline__ uint2 pack8_e4m3(const float (&f)[8], float scale) {
-  uint32_t w[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) w[i] = f32x2_to_e4m3x2(__fdiv_rn(f[2 * i], scale), __fdiv_rn(f[2 * i + 1], scale));
-  return make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
-}
+__device__ __forceinline__ float2 neg2(float2 a) { return make_float2(-a.x, -a.y); }
 
+// A lane's two pieces of a row.
+struct Piece {
+  uint2 a, b;
+};
 // Rows are read once: no place in L1.
-__device__ __forceinline__ uint4 ld_stream(const uint16_t* x) {
-  uint4 v;
-  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "l"(x)
-               : "memory");
+__device__ __forceinline__ Piece load_piece(const uint16_t* x, int da, int db) {
+  Piece v;
+  asm volatile("ld.global.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v.a.x), "=r"(v.a.y) : "l"(x + da) : "memory");
+  asm volatile("ld.global.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v.b.x), "=r"(v.b.y) : "l"(x + db) : "memory");
   return v;
+}
+__device__ __forceinline__ void store_piece(uint16_t* x, int da, int db, const Piece& v) {
+  *reinterpret_cast<uint2*>(x + da) = v.a;
+  *reinterpret_cast<uint2*>(x + db) = v.b;
+}
+template <bool BF16>
+__device__ __forceinline__ void unpack4(const uint2& x, float2 (&f)[2]) {
+  f[0] = to_f32x2<BF16>(x.x);
+  f[1] = to_f32x2<BF16>(x.y);
+}
+template <bool BF16>
+__device__ __forceinline__ uint2 pack4(const float2 (&f)[2]) {
+  return make_uint2(pack2<BF16>(f[0].x, f[0].y), pack2<BF16>(f[1].x, f[1].y));
+}
+// Four floats over `scale`, as e4m3 (the cache write's rule: rounded to nearest even, saturated).
+__device__ __forceinline__ uint32_t pack4_e4m3(const float2 (&f)[2], float scale) {
+  return f32x2_to_e4m3x2(__fdiv_rn(f[0].x, scale), __fdiv_rn(f[0].y, scale)) |
+         (f32x2_to_e4m3x2(__fdiv_rn(f[1].x, scale), __fdiv_rn(f[1].y, scale)) << 16);
+}
+template <bool BF16, bool FP8>
+__device__ __forceinline__ void store_cache(void* cache, int64_t at, int da, int db, const float2 (&a)[2], const float2 (&b)[2],
+                                            float scale) {
+  if constexpr (FP8) {
+    uint8_t* const x = reinterpret_cast<uint8_t*>(cache) + at;
+    *reinterpret_cast<uint32_t*>(x + da) = pack4_e4m3(a, scale);
+    *reinterpret_cast<uint32_t*>(x + db) = pack4_e4m3(b, scale);
+  } else {
+    store_piece(reinterpret_cast<uint16_t*>(cache) + at, da, db, Piece{pack4<BF16>(a), pack4<BF16>(b)});
+  }
 }
 
 constexpr int kRopeThreads = 256;
 constexpr int kRopeCtas = 4;  // per SM
 template <int D>
 struct RopeCfg {
-  static constexpr int kLanes = D / 8;                     // lanes per row
-  static constexpr int kGroups = kRopeThreads / kLanes;    // lane groups per CTA
-  static constexpr int kRows = D == 128 ? 3 : 2;           // rows per lane group and item
-  static constexpr int kItemRows = kGroups * kRows;        // 48 or 64 heads
+  static constexpr int kLanes = D / 8;                   // lanes per row
+  static constexpr int kGroups = kRopeThreads / kLanes;  // lane groups per CTA
 };
+
+// A lane's place in a row, and its frequencies.
+template <int D, bool INTER>
+struct RopeLane {
+  int da, db, f0, axis;
+  bool turned, one_axis;
+  unsigned mask;  // all lanes of the row; other rows of a warp may be of another token
+};
+
+// Norm (weights wa, wb; or none) and rotation of the lane's pieces a, b of one row.
+template <int D, bool BF16, bool INTER>
+__device__ __forceinline__ void rope_row(float2 (&a)[2], float2 (&b)[2], const RopeLane<D, INTER>& ln, bool norm, uint2 wa,
+                                         uint2 wb, float eps, const float2 (&cs)[2], const float2 (&sn)[2]) {
+  if (norm) {
+    float2 sq = mul2(a[0], a[0]);
+    sq = fma2(a[1], a[1], sq);
+    sq = fma2(b[0], b[0], sq);
+    sq = fma2(b[1], b[1], sq);
+    float ss = sq.x + sq.y;
+#pragma unroll
+    for (int o = 1; o < RopeCfg<D>::kLanes; o <<= 1) ss += __shfl_xor_sync(ln.mask, ss, o);
+    const float rs = rsqrtf(ss * (1.0f / D) + eps);
+    const float2 rs2 = make_float2(rs, rs);
+    float2 ga[2], gb[2];
+    unpack4<BF16>(wa, ga);
+    unpack4<BF16>(wb, gb);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      a[e] = mul2(mul2(a[e], rs2), ga[e]);
+      b[e] = mul2(mul2(b[e], rs2), gb[e]);
+    }
+  }
+  if (!ln.turned) return;  // past `rot`: as it is
+  // (a, b) -> (a c - b s, b c + a s)
+  if constexpr (INTER) {  // pairs (a0.x, a0.y), (a1.x, a1.y), (b0.x, b0.y), (b1.x, b1.y)
+    float2* const v[4] = {&a[0], &a[1], &b[0], &b[1]};
+    const float c[4] = {cs[0].x, cs[0].y, cs[1].x, cs[1].y}, s[4] = {sn[0].x, sn[0].y, sn[1].x, sn[1].y};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float2 x = *v[e];
+      *v[e] = make_float2(fmaf(x.y, -s[e], x.x * c[e]), fmaf(x.x, s[e], x.y * c[e]));
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const float2 x = a[e];
+      a[e] = fma2(b[e], neg2(sn[e]), mul2(x, cs[e]));
+      b[e] = fma2(x, sn[e], mul2(b[e], cs[e]));
+    }
+  }
+}
+
+// The units of one kind, from `first` on, `step` apart: unit u is head pair (or key-value
+// head) u % per_token of token u / per_token.
+template <int D, bool BF16, bool FP8, bool INTER, bool IS_Q>
+__device__ __forceinline__ void rope_units(const RopeParams& p, const RopeLane<D, INTER>& ln, unsigned first, unsigned step,
+                                           unsigned per_token) {
+  int t = (int)(first / per_token), u = (int)(first % per_token);
+  const int dt = (int)(step / per_token), du = (int)(step % per_token);
+  const int half = p.rot >> 1;
+  const uint16_t* const weight = IS_Q ? p.q_weight : p.k_weight;
+  uint2 wa = make_uint2(0u, 0u), wb = wa;
+  if (weight) {
+    wa = __ldg(reinterpret_cast<const uint2*>(weight + ln.da));
+    wb = __ldg(reinterpret_cast<const uint2*>(weight + ln.db));
+  }
+  struct Place {  // the token's position on the lane's (first) axis, and its slot
+    int at;
+    bool valid;
+    int64_t slot;
+  };
+  auto place = [&](int tok) {
+    Place x{0, true, tok};
+    bool past = false;
+    for (int a = 0; a < p.axes; ++a) {
+      const int pos = __ldg(p.positions + a * p.pos_stride + tok);
+      x.valid = x.valid && (unsigned)pos < (unsigned)p.max_pos;
+      past = past || pos >= p.max_pos;
+      if (a == ln.axis) x.at = pos;
+    }
+    if (past) report_device_error(GQA_ERR_INVALID_ARG, 212);
+    if (!IS_Q && p.slots) x.slot = __ldg(p.slots + tok);
+    return x;
+  };
+  if (t >= p.num_tokens) return;
+  Place next = place(t);
+  while (true) {
+    const Place it = next;
+    const int tok = t, un = u;
+    // The unit's two rows: query heads 2 un and 2 un + 1 (the last may be alone), or key
+    // and value of head un.
+    const bool both = IS_Q ? 2 * un + 1 < p.hq : p.v_dst != nullptr;
+    const uint16_t* const x0 = IS_Q ? p.q + tok * p.q_st + 2 * un * p.q_sh : p.k + tok * p.k_st + un * p.k_sh;
+    const uint16_t* const x1 = IS_Q ? x0 + p.q_sh : p.v + tok * p.v_st + un * p.v_sh;
+    const Piece r0 = load_piece(x0, ln.da, ln.db);
+    Piece r1{};
+    if (both) r1 = load_piece(x1, ln.da, ln.db);
+    float2 cs[2], sn[2];
+    if (ln.turned && it.valid) {
+      if (ln.one_axis) {
+        const float* row = p.table + (int64_t)it.at * p.rot + ln.f0;
+        const float4 c = __ldg(reinterpret_cast<const float4*>(row));
+        const float4 s = __ldg(reinterpret_cast<const float4*>(row + half));
+        cs[0] = make_float2(c.x, c.y); cs[1] = make_float2(c.z, c.w);
+        sn[0] = make_float2(s.x, s.y); sn[1] = make_float2(s.z, s.w);
+      } else {
+        float c[4], s[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          int axis = 0;
+#pragma unroll
+          for (int a = 1; a < kMaxAxes; ++a)
+            if (a < p.axes && ln.f0 + e >= p.section_end[a - 1]) axis = a;
+          const float* row = p.table + (int64_t)__ldg(p.positions + axis * p.pos_stride + tok) * p.rot + ln.f0 + e;
+          c[e] = __ldg(row);
+          s[e] = __ldg(row + half);
+        }
+        cs[0] = make_float2(c[0], c[1]); cs[1] = make_float2(c[2], c[3]);
+        sn[0] = make_float2(s[0], s[1]); sn[1] = make_float2(s[2], s[3]);
+      }
+    }
+    t += dt;
+    u += du;
+    if (u >= (int)per_token) {
+      u -= (int)per_token;
+      ++t;
+    }
+    const bool more = t < p.num_tokens;
+    if (more) next = place(t);
+
+    float2 a[2], b[2];
+    if constexpr (IS_Q) {
+      // A padding token's query is zero.
+      uint16_t* const o0 = p.q_out + ((int64_t)tok * p.hq + 2 * un) * D;
+      Piece y0{}, y1{};
+      if (it.valid) {
+        unpack4<BF16>(r0.a, a);
+        unpack4<BF16>(r0.b, b);
+        rope_row<D, BF16, INTER>(a, b, ln, weight != nullptr, wa, wb, p.eps, cs, sn);
+        y0 = Piece{pack4<BF16>(a), pack4<BF16>(b)};
+        unpack4<BF16>(r1.a, a);
+        unpack4<BF16>(r1.b, b);
+        rope_row<D, BF16, INTER>(a, b, ln, weight != nullptr, wa, wb, p.eps, cs, sn);
+        y1 = Piece{pack4<BF16>(a), pack4<BF16>(b)};
+      }
+      store_piece(o0, ln.da, ln.db, y0);
+      if (both) store_piece(o0 + D, ln.da, ln.db, y1);
+    } else {
+      int64_t dst = it.slot;
+      if (p.slots && (dst >= p.num_slots || !it.valid)) {
+        if (dst >= p.num_slots) report_device_error(GQA_ERR_INVALID_ARG, 213);
+        dst = -1;
+      }
+      if (dst >= 0) {
+        const int64_t at = (dst * p.hkv + un) * D;
+        if (it.valid) {
+          unpack4<BF16>(r0.a, a);
+          unpack4<BF16>(r0.b, b);
+          rope_row<D, BF16, INTER>(a, b, ln, weight != nullptr, wa, wb, p.eps, cs, sn);
+        } else {  // padding without a cache: zero
+          a[0] = a[1] = b[0] = b[1] = make_float2(0.f, 0.f);
+        }
+        store_cache<BF16, FP8>(p.k_dst, at, ln.da, ln.db, a, b, p.k_scale);
+        if (both) {
+          if constexpr (FP8) {
+            unpack4<BF16>(r1.a, a);
+            unpack4<BF16>(r1.b, b);
+            store_cache<BF16, FP8>(p.v_dst, at, ln.da, ln.db, a, b, p.v_scale);
+          } else {
+            store_piece(reinterpret_cast<uint16_t*>(p.v_dst) + at, ln.da, ln.db, r1);
+          }
+        }
+      }
+    }
+    if (!more) return;
+  }
+}
 
 // INTER: neighbouring pairs (2f, 2f + 1) instead of (f, f + rot / 2).
 template <int D, bool BF16, bool FP8, bool INTER>
 __global__ void __launch_bounds__(kRopeThreads, kRopeCtas) gqa_rope_kernel(const __grid_constant__ RopeParams p) {
   using Cfg = RopeCfg<D>;
-  constexpr int R = Cfg::kRows;
-  constexpr int NF = INTER ? 4 : 8;  // frequencies of a 16-byte piece
   pdl_wait();
   pdl_trigger();
-  const int sub = threadIdx.x % Cfg::kLanes;  // 16-byte piece of the row
-  const int grp = threadIdx.x / Cfg::kLanes;
-  const int d0 = sub * 8;
-  const int half = p.rot >> 1;
-  const bool turned = d0 < p.rot;
-  const bool second = d0 >= half;  // of a half-split pair (a piece lies in one half: rot % 16 == 0)
-  const int f0 = INTER ? d0 >> 1 : (second ? d0 - half : d0);  // the piece's first frequency
-  const int rows = p.hq + 2 * p.hkv;
-  const int per_token = (rows + Cfg::kItemRows - 1) / Cfg::kItemRows;
-  const int64_t items = (int64_t)p.num_tokens * per_token;
-  auto axis_of = [&](int f) {
-    int x = 0;
+  const int lane = threadIdx.x & 31, sub = threadIdx.x % Cfg::kLanes;
+  RopeLane<D, INTER> ln;
+  ln.f0 = 4 * sub;
+  ln.turned = 8 * sub < p.rot;
+  const bool split = !INTER && ln.turned;  // the pieces are half a rotation apart
+  ln.da = split ? ln.f0 : 8 * sub;
+  ln.db = split ? (p.rot >> 1) + ln.f0 : 8 * sub + 4;
+  ln.axis = 0;
+  int last = 0;
 #pragma unroll
-    for (int a = 1; a < kMaxAxes; ++a)
-      if (a < p.axes && f >= p.section_end[a - 1]) x = a;
-    return x;
-  };
-  const int axis = axis_of(f0);
-  const bool one_axis = axis == axis_of(f0 + NF - 1);  // or the piece spans sections
-  const int lane = threadIdx.x & 31;
-  const int shift = half >> 3;  // lanes between the two values of a half-split pair
-  const int src = (!INTER && turned) ? (second ? lane - shift : lane + shift) : lane;
-
-  struct Place {  // of an item: token, position on the piece's (first) axis, slot
-    int t, at;
-    bool valid, past;
-    int64_t slot;
-  };
-  auto place = [&](int64_t w) {
-    Place x;
-    x.t = (int)(w / per_token);
-    x.valid = true;
-    x.past = false;
-    x.at = 0;
-    for (int a = 0; a < p.axes; ++a) {
-      const int pos = __ldg(p.positions + a * p.pos_stride + x.t);
-      x.valid = x.valid && (unsigned)pos < (unsigned)p.max_pos;
-      x.past = x.past || pos >= p.max_pos;
-      if (a == axis) x.at = pos;
-    }
-    x.slot = p.slots ? __ldg(p.slots + x.t) : x.t;
-    return x;
-  };
-
-  int64_t w = blockIdx.x;
-  if (w >= items) return;
-  Place next = place(w);
-  for (; w < items; w += gridDim.x) {
-    const Place it = next;
-    const int r0 = (int)(w - (int64_t)it.t * per_token) * Cfg::kItemRows + grp;  // this lane group's first row
-    uint4 raw[R];
-#pragma unroll
-    for (int i = 0; i < R; ++i) {
-      const int r = r0 + i * Cfg::kGroups;
-      raw[i] = make_uint4(0u, 0u, 0u, 0u);
-      const uint16_t* x = nullptr;
-      if (r < p.hq) x = p.q + it.t * p.q_st + r * p.q_sh;
-      else if (r < p.hq + p.hkv) x = p.k + it.t * p.k_st + (r - p.hq) * p.k_sh;
-      else if (r < rows && p.v_dst) x = p.v + it.t * p.v_st + (r - p.hq - p.hkv) * p.v_sh;
-      if (x) raw[i] = ld_stream(x + d0);
-    }
-    // Frequency f0 + e turns value e of the piece, or, interleaved, values 2e and 2e + 1.
-    float cs[NF], sn[NF];
-#pragma unroll
-    for (int e = 0; e < NF; ++e) {
-      cs[e] = 1.f;
-      sn[e] = 0.f;
-    }
-    if (turned && it.valid) {
-      if (one_axis) {
-        const float* row = p.table + (int64_t)it.at * p.rot + f0;
-#pragma unroll
-        for (int v = 0; v < NF / 4; ++v) {
-          const float4 c = __ldg(reinterpret_cast<const float4*>(row) + v);
-          const float4 s = __ldg(reinterpret_cast<const float4*>(row + half) + v);
-          cs[4 * v] = c.x; cs[4 * v + 1] = c.y; cs[4 * v + 2] = c.z; cs[4 * v + 3] = c.w;
-          sn[4 * v] = s.x; sn[4 * v + 1] = s.y; sn[4 * v + 2] = s.z; sn[4 * v + 3] = s.w;
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < NF; ++e) {
-          const float* row = p.table + (int64_t)__ldg(p.positions + axis_of(f0 + e) * p.pos_stride + it.t) * p.rot + f0 + e;
-          cs[e] = __ldg(row);
-          sn[e] = __ldg(row + half);
-        }
-      }
-    }
-    if (w + gridDim.x < items) next = place(w + gridDim.x);
-
-    // A token whose position is negative is padding: its query is zero and nothing is
-    // cached. One past the table is the same, and reported.
-    if (it.past && threadIdx.x == 0) report_device_error(GQA_ERR_INVALID_ARG, 212);
-    if (!it.valid) {
-#pragma unroll
-      for (int i = 0; i < R; ++i) {
-        const int r = r0 + i * Cfg::kGroups;
-        const uint4 z = make_uint4(0u, 0u, 0u, 0u);
-        if (r < p.hq)
-          *reinterpret_cast<uint4*>(p.q_out + ((int64_t)it.t * p.hq + r) * D + d0) = z;
-        else if (r < p.hq + p.hkv && !p.slots)
-          *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p.k_dst) + ((int64_t)it.t * p.hkv + r - p.hq) * D + d0) = z;
-      }
-      continue;
-    }
-    int64_t dst = it.slot;
-    if (p.slots && dst >= p.num_slots) {
-      if (threadIdx.x == 0) report_device_error(GQA_ERR_INVALID_ARG, 213);
-      dst = -1;
-    }
-
-#pragma unroll
-    for (int i = 0; i < R; ++i) {
-      const int r = r0 + i * Cfg::kGroups;
-      const bool is_q = r < p.hq, is_k = !is_q && r < p.hq + p.hkv, is_v = !is_q && !is_k;
-      float f[8];
-      unpack8<BF16>(raw[i], f);
-      const uint16_t* weight = is_q ? p.q_weight : is_k ? p.k_weight : nullptr;
-      if (weight) {  // uniform over the row's lanes
-        float g[8], ss = 0.f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) ss = fmaf(f[e], f[e], ss);
-        // All lanes of the row are here; other rows of the warp may not be.
-        const unsigned mask = (Cfg::kLanes == 16 ? 0xffffu : 0xffu) << (lane & ~(Cfg::kLanes - 1));
-#pragma unroll
-        for (int o = 1; o < Cfg::kLanes; o <<= 1) ss += __shfl_xor_sync(mask, ss, o);
-        const float rs = rsqrtf(ss * (1.0f / D) + p.eps);
-        unpack8<BF16>(__ldg(reinterpret_cast<const uint4*>(weight + d0)), g);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] = f[e] * rs * g[e];
-      }
-      // (a, b) -> (a c - b s, b c + a s): the first of a pair takes -s, the second +s.
-      if constexpr (INTER) {
-        if (!is_v) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float a = f[2 * e], b = f[2 * e + 1];
-            f[2 * e] = fmaf(b, -sn[e], a * cs[e]);
-            f[2 * e + 1] = fmaf(a, sn[e], b * cs[e]);
-          }
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float g = __shfl_sync(0xffffffffu, f[e], src);
-          if (!is_v) f[e] = fmaf(g, second ? sn[e] : -sn[e], f[e] * cs[e]);
-        }
-      }
-      if (is_q) {
-        *reinterpret_cast<uint4*>(p.q_out + ((int64_t)it.t * p.hq + r) * D + d0) = pack8<BF16>(f);
-      } else if (dst >= 0 && r < rows && (is_k || p.v_dst)) {
-        void* to = is_k ? p.k_dst : p.v_dst;
-        const int64_t at = (dst * p.hkv + (is_k ? r - p.hq : r - p.hq - p.hkv)) * D + d0;
-        if constexpr (FP8)
-          *reinterpret_cast<uint2*>(reinterpret_cast<uint8_t*>(to) + at) = pack8_e4m3(f, is_k ? p.k_scale : p.v_scale);
-        else
-          *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(to) + at) = is_v ? raw[i] : pack8<BF16>(f);
-      }
-    }
+  for (int a = 1; a < kMaxAxes; ++a) {
+    if (a < p.axes && ln.f0 >= p.section_end[a - 1]) ln.axis = a;
+    if (a < p.axes && ln.f0 + 3 >= p.section_end[a - 1]) last = a;
   }
+  ln.one_axis = ln.axis == last;  // or the lane's frequencies span sections
+  ln.mask = (Cfg::kLanes == 16 ? 0xffffu : 0xffu) << (lane & ~(Cfg::kLanes - 1));
+  const unsigned grp = threadIdx.x / Cfg::kLanes;
+  if (blockIdx.x < (unsigned)p.q_ctas)
+    rope_units<D, BF16, FP8, INTER, true>(p, ln, blockIdx.x * Cfg::kGroups + grp, p.q_ctas * Cfg::kGroups, (p.hq + 1) >> 1);
+  else
+    rope_units<D, BF16, FP8, INTER, false>(p, ln, (blockIdx.x - p.q_ctas) * Cfg::kGroups + grp,
+                                           (gridDim.x - p.q_ctas) * Cfg::kGroups, p.hkv);
 }
 
 }  // namespace gqa

@@ -293,9 +293,19 @@ int gqa_qk_norm_rope(const gqa_qk_norm_rope_args* args, void* stream) {
   p.v_scale = a.v_scale;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const bool bf = a.dtype == GQA_DTYPE_BF16;
-  const int item_rows = a.head_dim == 128 ? RopeCfg<128>::kItemRows : RopeCfg<64>::kItemRows;
-  const int64_t items = (int64_t)a.num_tokens * ((a.num_heads + 2 * a.num_kv_heads + item_rows - 1) / item_rows);
-  const dim3 grid((unsigned)std::min<int64_t>(items, kRopeCtas * sm));
+  // Units of two rows; both kinds get CTAs in proportion, at most what fits the device at once.
+  const int groups = a.head_dim == 128 ? RopeCfg<128>::kGroups : RopeCfg<64>::kGroups;
+  const int64_t q_units = (int64_t)a.num_tokens * ((a.num_heads + 1) / 2), kv_units = (int64_t)a.num_tokens * a.num_kv_heads;
+  if (q_units > INT_MAX / 2 || kv_units > INT_MAX / 2) return GQA_ERR_INVALID_ARG;
+  const int64_t q_need = (q_units + groups - 1) / groups, kv_need = (kv_units + groups - 1) / groups;
+  const int64_t fit = (int64_t)kRopeCtas * sm;
+  int64_t q_ctas = q_need, kv_ctas = kv_need;
+  if (q_need + kv_need > fit) {
+    kv_ctas = std::max<int64_t>(1, std::min(kv_need, fit * kv_units / (q_units + kv_units)));
+    q_ctas = std::min(q_need, fit - kv_ctas);
+  }
+  p.q_ctas = (int)q_ctas;
+  const dim3 grid((unsigned)(q_ctas + kv_ctas));
   cudaError_t e;
 #define GQA_ROPE(D, BF, F8)                                                                                     \
   e = a.interleaved ? launch_pdl(gqa_rope_kernel<D, BF, F8, true>, grid, kRopeThreads, 0, st, p)                \
