@@ -1,4 +1,5 @@
-"""Builds libgqa_sm100.so (the C-ABI library) in-tree for sm_100a.
+"""Builds libgqa_sm100.so (the C-ABI library) in-tree for sm_100a, and the serving step's
+Python binding (_serving_ext.so, host code against torch's headers).
 
     python gqa-flash-attn-rtx3060_b200/build.py [--force] [--debug]
 
@@ -8,10 +9,12 @@ not link libcuda (the driver's tensor-map encoder is looked up at run time),
 so it loads on a machine without a GPU driver.
 """
 import argparse
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
@@ -28,6 +31,34 @@ NVCC_FLAGS = [
     "-Xcompiler", "-fPIC", "-shared",
     "-cudart", "static",
 ]
+
+
+EXT = os.path.join(HERE, "gqa_kernels", "_serving_ext.so")
+EXT_SOURCES = [os.path.join(CSRC, "serving_ext.cpp"), os.path.join(INCLUDE, "gqa_sm100.h")]
+
+
+def build_ext(force=False):
+    """Compiles gqa_kernels._serving_ext (g++, a few seconds) unless it is newer than its sources
+    and was built for the installed torch. Returns its path."""
+    torch_dir = list(importlib.util.find_spec("torch").submodule_search_locations)[0]
+    stamp = f"{torch_dir} {os.path.getmtime(os.path.join(torch_dir, 'version.py'))} {sys.version}\n"
+    if not force and os.path.exists(EXT) and all(os.path.getmtime(x) <= os.path.getmtime(EXT) for x in EXT_SOURCES):
+        with open(EXT, "rb") as f:
+            f.seek(-min(os.path.getsize(EXT), len(stamp)), os.SEEK_END)
+            if f.read() == stamp.encode():
+                return EXT
+    cuda = os.path.dirname(os.path.dirname(nvcc()))
+    tmp = EXT + ".tmp"
+    subprocess.run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-D_GLIBCXX_USE_CXX11_ABI=1",
+                    "-I", INCLUDE, "-I", os.path.join(torch_dir, "include"),
+                    "-I", os.path.join(torch_dir, "include", "torch", "csrc", "api", "include"),
+                    "-I", os.path.join(cuda, "include"), "-I", sysconfig.get_paths()["include"],
+                    EXT_SOURCES[0], "-o", tmp, "-L", os.path.join(torch_dir, "lib"),
+                    "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda"], check=True)
+    with open(tmp, "ab") as f:  # what it was built for, after the last byte that the loader reads
+        f.write(stamp.encode())
+    os.replace(tmp, EXT)
+    return EXT
 
 
 def _sources():
@@ -52,9 +83,10 @@ def nvcc():
 
 
 def build(force=False, verbose=False, debug=False):
-    """Compiles the library (or, with debug, its checked variant) unless it is newer
-    than every source. Returns its path."""
+    """Compiles the library (or, with debug, its checked variant) and the binding unless they
+    are newer than every source. Returns the library's path."""
     out = OUT_DEBUG if debug else OUT
+    build_ext(force)
     if not force and up_to_date(out):
         return out
     tmp = out + ".tmp"

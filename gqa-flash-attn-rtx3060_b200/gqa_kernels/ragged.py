@@ -11,20 +11,10 @@ packed into one request.
 """
 import torch
 
-from . import _lib, _serving
+from . import _serving
 from .qk_rope import qk_norm_rope_append
 
 __all__ = ["paged_ragged_attention", "RaggedPagedAttention"]
-
-
-def _optional(t, name, dtype, shape):
-    if t.dtype != dtype or t.shape != shape:
-        raise ValueError(f"{name} must be {dtype} {tuple(shape)}")
-    return t if t.is_contiguous() else t.contiguous()
-
-
-def _workspace_bytes(lib, args):
-    return lib.gqa_ragged_fwd_workspace_bytes(args)
 
 
 def paged_ragged_attention(query, key_cache, value_cache, block_tables, cu_query_lens, seq_lens, max_query_len=None,
@@ -67,68 +57,9 @@ def paged_ragged_attention(query, key_cache, value_cache, block_tables, cu_query
         gqa_flash_attn and paged_prefill give NaN, the reference's rule: here masks that
         leave a row empty are ordinary). Asynchronous on the current stream.
     """
-    if query.dim() != 3 or key_cache.dim() != 4:
-        raise ValueError("query must be (num_tokens, num_heads, head_dim) and the caches "
-                         "(num_blocks, block_size, num_kv_heads, head_dim)")
-    num_tokens, num_heads, head_dim = query.shape
-    num_blocks, block_size, num_kv_heads, hd = key_cache.shape
-    num_seqs = seq_lens.shape[0]
-    if hd != head_dim or value_cache.shape != key_cache.shape:
-        raise ValueError("key_cache and value_cache must be (num_blocks, block_size, num_kv_heads, head_dim)")
-    if num_heads % num_kv_heads:
-        raise ValueError("num_heads must be divisible by num_kv_heads")
-    dtype = _lib.dtype_code(query)
-    fp8 = key_cache.dtype == torch.float8_e4m3fn
-    if key_cache.dtype != value_cache.dtype or not (fp8 or key_cache.dtype == query.dtype):
-        raise TypeError("the caches must share query's dtype, or both be float8_e4m3fn")
-    if block_tables.dtype != torch.int32 or seq_lens.dtype != torch.int32 or cu_query_lens.dtype != torch.int32:
-        raise TypeError("block_tables, cu_query_lens and seq_lens must be int32")
-    if block_tables.dim() != 2 or block_tables.shape[0] != num_seqs or seq_lens.dim() != 1 \
-            or cu_query_lens.shape != (num_seqs + 1,):
-        raise ValueError("block_tables must be (num_seqs, max_blocks), seq_lens (num_seqs,) and cu_query_lens (num_seqs + 1,)")
-    if window is not None and window < 1:
-        raise ValueError("window must be at least 1")
-    if softcap < 0:
-        raise ValueError("softcap must not be negative")
-    if not causal and (window is not None or prefix_lens is not None):
-        raise ValueError("window and prefix_lens need causal")
-    if fp8 and not (k_scale > 0 and v_scale > 0):
-        raise ValueError("fp8 caches need positive k_scale and v_scale")
-    if alibi_slopes is not None:
-        alibi_slopes = _optional(alibi_slopes, "alibi_slopes", torch.float32, (num_heads,))
-    if prefix_lens is not None:
-        prefix_lens = _optional(prefix_lens, "prefix_lens", torch.int32, (num_seqs,))
-    if key_starts is not None:
-        key_starts = _optional(key_starts, "key_starts", torch.int32, (num_tokens,))
-    if out is None:
-        out = torch.empty_like(query, memory_format=torch.contiguous_format)
-    elif out.shape != query.shape or out.dtype != query.dtype:
-        raise ValueError("out must have query's shape and dtype")
-    index = _serving.device_index(query, key_cache, value_cache, block_tables, cu_query_lens, seq_lens, out, alibi_slopes,
-                                  prefix_lens, key_starts)
-    if not block_tables.is_contiguous():
-        block_tables = block_tables.contiguous()
-    if not seq_lens.is_contiguous():
-        seq_lens = seq_lens.contiguous()
-    if not cu_query_lens.is_contiguous():
-        cu_query_lens = cu_query_lens.contiguous()
-    if not _lib.tma_compatible(query):
-        query = query.contiguous()
-    max_blocks = block_tables.shape[1]
-    if max_seq_len is None or max_seq_len > max_blocks * block_size:
-        max_seq_len = max_blocks * block_size
-    lse = torch.empty((num_tokens, num_heads), dtype=torch.float32, device=query.device) if return_lse else None
-    _serving.call_with_workspace("gqa_ragged_fwd", _serving.RAGGED(
-        query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(),
-        block_tables.data_ptr(), cu_query_lens.data_ptr(), seq_lens.data_ptr(),
-        0 if alibi_slopes is None else alibi_slopes.data_ptr(), 0 if prefix_lens is None else prefix_lens.data_ptr(),
-        0 if key_starts is None else key_starts.data_ptr(),
-        *query.stride(), *key_cache.stride(), *value_cache.stride(), *out.stride(),
-        max_blocks, num_seqs, num_tokens, num_heads, num_kv_heads, head_dim, block_size, num_blocks,
-        num_tokens if max_query_len is None else max_query_len, max_seq_len, 0 if window is None else window,
-        1 if causal else 0, dtype, 1 if fp8 else 0,
-        head_dim ** -0.5 if scale is None else scale, softcap, k_scale, v_scale), index, _workspace_bytes)
-    return (out, lse) if return_lse else out
+    return (_serving._ext or _serving.load()).ragged(
+        query, key_cache, value_cache, block_tables, cu_query_lens, seq_lens, max_query_len, max_seq_len, scale, causal, softcap,
+        alibi_slopes, window, prefix_lens, key_starts, k_scale, v_scale, return_lse, out)
 
 
 class RaggedPagedAttention:

@@ -48,6 +48,7 @@ class StepPlan:
         """Unwritten buffers for plans of num_seqs requests and at most max_tokens tokens."""
         def i32(n):
             return torch.empty(n, dtype=torch.int32, device=device)
+        max_tokens = max(0, max_tokens)
         return cls(i32(num_seqs + 1), i32(num_seqs), i32(max_tokens),
                    torch.empty(max_tokens, dtype=torch.int64, device=device), i32(max_tokens),
                    torch.empty(num_seqs, dtype=torch.bool, device=device), i32(num_seqs), i32(1))
@@ -76,40 +77,9 @@ def plan_step(query_lens, context_lens, block_tables, blocks_held, free_blocks, 
         left, or more than its row has entries, is refused for this step, and so is every
         later one that needs any. Asynchronous on the current stream.
     """
-    n = query_lens.shape[0]
-    if block_tables.dim() != 2 or query_lens.shape != (n,) or context_lens.shape != (n,) or blocks_held.shape != (n,) \
-            or block_tables.shape[0] != n:
-        raise ValueError("query_lens, context_lens and blocks_held must be (n,) and block_tables (n, max_blocks)")
-    if free_blocks.dim() != 1 or free_count.shape != (1,):
-        raise ValueError("free_blocks must be (num_free,) and free_count (1,)")
-    for t in (query_lens, context_lens, block_tables, blocks_held, free_blocks, free_count):
-        if t.dtype != torch.int32:
-            raise TypeError("lengths, tables and the free list must be int32")
-    if block_size < 1 or block_size & (block_size - 1):
-        raise ValueError("block_size must be a power of two")
-    if max_tokens < 0:
-        raise ValueError("max_tokens must not be negative")
-    max_blocks = block_tables.shape[1]
-    if block_tables.stride(1) != 1 and max_blocks > 1:
-        raise ValueError("the rows of block_tables must be contiguous")
-    if n > 1 and block_tables.stride(0) < max_blocks:
-        raise ValueError("the rows of block_tables must not overlap")
-    for t in (query_lens, context_lens, blocks_held, free_blocks):
-        if t.shape[0] > 1 and t.stride(0) != 1:
-            raise ValueError("lengths and the free list must be contiguous")
-    index = _serving.device_index(query_lens, context_lens, block_tables, blocks_held, free_blocks, free_count)
     if out is None:
-        out = StepPlan.empty(n, max_tokens, query_lens.device)
-    else:
-        if out.seq_lens.shape[0] != n or out.positions.shape[0] != max_tokens or out.seq_lens.get_device() != index:
-            raise ValueError("out must be a StepPlan of this n, max_tokens and device")
-        if out.blocks_held.data_ptr() == blocks_held.data_ptr() or out.free_count.data_ptr() == free_count.data_ptr() \
-                or out.seq_lens.data_ptr() == context_lens.data_ptr():
-            raise ValueError("out must not hold the tensors that the plan is made from")
-    _serving.call("gqa_step_plan", _serving.STEP_PLAN(
-        query_lens.data_ptr(), context_lens.data_ptr(), block_tables.data_ptr(), blocks_held.data_ptr(),
-        free_blocks.data_ptr(), free_count.data_ptr(), out.cu_query_lens.data_ptr(), out.seq_lens.data_ptr(),
-        out.positions.data_ptr(), out.slot_mapping.data_ptr(), out.token_seqs.data_ptr(), out.granted.data_ptr(),
-        out.blocks_held.data_ptr(), out.free_count.data_ptr(), max(block_tables.stride(0), max_blocks),
-        n, max_blocks, free_blocks.shape[0], block_size, max_tokens), index)
+        out = StepPlan.empty(query_lens.shape[0], max_tokens, query_lens.device)
+    (_serving._ext or _serving.load()).step_plan(
+        query_lens, context_lens, block_tables, blocks_held, free_blocks, free_count, block_size, max_tokens, out.cu_query_lens,
+        out.seq_lens, out.positions, out.slot_mapping, out.token_seqs, out.granted, out.blocks_held, out.free_count)
     return out

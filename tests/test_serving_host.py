@@ -2,6 +2,7 @@
 GPU tests compare with, against one another on small cases."""
 import os
 import shutil
+import struct
 import subprocess
 
 import pytest
@@ -96,7 +97,8 @@ def verify(**kw):
     (dict(draft_tokens=i32(2, 65)), ValueError), (dict(cu_query_lens=i32(2)), ValueError), (dict(uniforms=torch.zeros(2, 2)), ValueError),
     (dict(exponentials=torch.zeros(2, 49)), ValueError), (dict(draft_probs=torch.zeros(2, 3, 49)), ValueError),
     (dict(draft_probs=bf(2, 3, 50)), TypeError), (dict(target_probs=torch.zeros(8, 50, dtype=torch.float64)), TypeError),
-    (dict(draft_tokens=torch.zeros(2, 3, dtype=torch.int64)), TypeError), (dict(), ValueError)])
+    (dict(draft_tokens=torch.zeros(2, 3, dtype=torch.int64)), TypeError), (dict(exponentials=None), ValueError),
+    (dict(draft_tokens=[1]), TypeError), (dict(), ValueError)])
 def test_verify_refuses(lib_path, kw, err):
     with pytest.raises(err):
         verify(**kw)
@@ -114,15 +116,22 @@ def test_layer_refuses():
         RaggedPagedAttention(8, 2, 128, rope_table(4, 128, device="cpu"), kv_cache_dtype="int8")
 
 
+# The structs' fields in order, as an FFI host packs them.
+STEP_PLAN = struct.Struct("@14Pq5i").pack
+QK_NORM_ROPE = struct.Struct("@11P10q16i3f").pack
+RAGGED = struct.Struct("@PN11P14q14i4f").pack
+VERIFY = struct.Struct("@PN8P6q5i").pack
+
+
 def test_c_entry_points_refuse_before_any_launch(lib_path):
     """The C ABI's own checks answer with a status, on a machine without a GPU."""
-    from gqa_kernels import _lib, _serving
+    from gqa_kernels import _lib
     lib = _lib.load()
     one = 1 << 20  # a non-null, aligned address that is never read
 
     def ragged(hq=8, hkv=2, d=128, block=64, dtype=1, fp8=0, causal=1, window=0, scale=0.1, cap=0.0, table=one, max_len=64,
                dstr=1, n=1):
-        return lib.gqa_ragged_fwd(_serving._WORKSPACE(0, 0) + _serving.RAGGED(
+        return lib.gqa_ragged_fwd(RAGGED(0, 0,
             one, one, one, one, 0, table, one, one, 0, 0, 0, 8, 8, 1, 8, 8, 8, dstr, 8, 8, 8, 1, 8, 8, 1,
             1, n, 1, hq, hkv, d, block, 4, 1, max_len, window, causal, dtype, fp8, scale, cap, 1.0, 1.0), None)
     assert ragged(hq=7) == 1 and ragged(d=96) == 2 and ragged(hq=130) == 2 and ragged(block=8) == 2 and ragged(block=48) == 2
@@ -131,18 +140,18 @@ def test_c_entry_points_refuse_before_any_launch(lib_path):
     assert ragged(dstr=2) == 3 and ragged(n=0) == 0 and lib.gqa_ragged_fwd(None, None) == 1
 
     def plan(held_out=2 * one, block=16, stride=4):
-        return lib.gqa_step_plan(_serving.STEP_PLAN(one, one, one, one, one, one, one, 3 * one, one, one, one, one, held_out, 2 * one,
+        return lib.gqa_step_plan(STEP_PLAN(one, one, one, one, one, one, one, 3 * one, one, one, one, one, held_out, 2 * one,
                                                     stride, 2, 4, 4, block, 8), None)
     assert plan(held_out=one) == 1 and plan(block=12) == 2 and plan(stride=3) == 1 and lib.gqa_step_plan(None, None) == 1
 
     def rotate(d=128, rot=128, axes=1, sections=(64, 0, 0, 0), slots=one, eps=1e-6, q=one):
-        return lib.gqa_qk_norm_rope(_serving.QK_NORM_ROPE(q, one, one, 0, 0, one, one, one, one, one, slots, 8, 8, 1, 8, 8, 1, 8, 8, 1, 0,
+        return lib.gqa_qk_norm_rope(QK_NORM_ROPE(q, one, one, 0, 0, one, one, one, one, one, slots, 8, 8, 1, 8, 8, 1, 8, 8, 1, 0,
                                                           *sections, axes, 9, rot, 0, 3, 8, 2, d, 16, 4, 1, 0, eps, 1.0, 1.0), None)
     assert rotate(d=80) == 2 and rotate(rot=24) == 2 and rotate(axes=5) == 2 and rotate(axes=2, sections=(60, 3, 0, 0)) == 1
     assert rotate(slots=0) == 1 and rotate(eps=-1.0) == 1 and rotate(q=one + 8) == 3 and lib.gqa_qk_norm_rope(None, None) == 1
 
     def check(k=2, vocab=9, dtype=2, n=1):
-        return lib.gqa_verify_drafts(_serving._WORKSPACE(0, 0) + _serving.VERIFY(one, one, 0, one, one, one, one, one, 2, 9, 0, 0, 2, 9,
+        return lib.gqa_verify_drafts(VERIFY(0, 0, one, one, 0, one, one, one, one, one, 2, 9, 0, 0, 2, 9,
                                                                                  n, 3, k, vocab, dtype), None)
     assert check(k=65) == 2 and check(vocab=0) == 1 and check(dtype=7) == 2 and check(n=20000) == 2 and check(n=0) == 0
     assert lib.gqa_verify_drafts(None, None) == 1 and lib.gqa_verify_greedy(None, None) == 1
@@ -151,12 +160,8 @@ def test_c_entry_points_refuse_before_any_launch(lib_path):
 @pytest.mark.skipif(shutil.which("gcc") is None, reason="no C compiler")
 def test_packed_structs_match_the_header(tmp_path):
     """The structs as a C compiler lays them out have the packed records' sizes and last fields' places."""
-    from gqa_kernels import _serving
-    ws = len(_serving._WORKSPACE(0, 0))
-    want = {"gqa_step_plan_args": ("max_tokens", _serving.STEP_PLAN(*[0] * 20)),
-            "gqa_qk_norm_rope_args": ("v_scale", _serving.QK_NORM_ROPE(*[0] * 40)),
-            "gqa_ragged_args": ("v_scale", bytes(ws) + _serving.RAGGED(*[0] * 43)),
-            "gqa_verify_args": ("dtype", bytes(ws) + _serving.VERIFY(*[0] * 19))}
+    want = {"gqa_step_plan_args": ("max_tokens", STEP_PLAN(*[0] * 20)), "gqa_qk_norm_rope_args": ("v_scale", QK_NORM_ROPE(*[0] * 40)),
+            "gqa_ragged_args": ("v_scale", RAGGED(*[0] * 45)), "gqa_verify_args": ("dtype", VERIFY(*[0] * 21))}
     src = tmp_path / "sizes.c"
     src.write_text('#include <stdio.h>\n#include "gqa_sm100.h"\nint main(void) {\n' + "".join(
         f'  printf("%zu %zu\\n", sizeof({t}), offsetof({t}, {f}));\n' for t, (f, _) in want.items()) + "  return 0;\n}\n")
