@@ -22,6 +22,7 @@
 #pragma once
 
 #include <climits>
+#include <type_traits>
 
 #include "gqa_common.cuh"
 
@@ -58,16 +59,21 @@ struct ProbType {
     else return __half2float(__ushort_as_half(x));
   }
   static __device__ __forceinline__ float load(const T* p) { return value(__ldg(p)); }
-  static __device__ __forceinline__ void load_vec(const T* p, float (&f)[Vec]) {
-    const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
+  static __device__ __forceinline__ void values(const uint4& v, float (&f)[Vec]) {
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float2 y = DT == kProbBf16 ? make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u))
-                                       : __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-      f[2 * i] = y.x;
-      f[2 * i + 1] = y.y;
+      f[2 * i] = value((T)w[i]);
+      f[2 * i + 1] = value((T)(w[i] >> 16));
     }
+  }
+  // The largest of a piece, two values per instruction; NaN only if all are.
+  static __device__ __forceinline__ float largest(const uint4& v) {
+    using H2 = typename std::conditional<DT == kProbBf16, __nv_bfloat162, __half2>::type;
+    auto h = [](const uint32_t& x) { return *reinterpret_cast<const H2*>(&x); };
+    const H2 m = __hmax2(__hmax2(h(v.x), h(v.y)), __hmax2(h(v.z), h(v.w)));
+    const uint32_t w = *reinterpret_cast<const uint32_t*>(&m);
+    return fmaxf(value((T)w), value((T)(w >> 16)));
   }
 };
 template <>
@@ -75,9 +81,11 @@ struct ProbType<kProbF32> {
   using T = float;
   static constexpr int Vec = 4;
   static __device__ __forceinline__ float load(const T* p) { return __ldg(p); }
-  static __device__ __forceinline__ void load_vec(const T* p, float (&f)[Vec]) {
-    const float4 v = __ldg(reinterpret_cast<const float4*>(p));
-    f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w;
+  static __device__ __forceinline__ void values(const uint4& v, float (&f)[Vec]) {
+    f[0] = __uint_as_float(v.x); f[1] = __uint_as_float(v.y); f[2] = __uint_as_float(v.z); f[3] = __uint_as_float(v.w);
+  }
+  static __device__ __forceinline__ float largest(const uint4& v) {
+    return fmaxf(max3(__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z)), __uint_as_float(v.w));
   }
 };
 
@@ -118,42 +126,45 @@ __device__ __forceinline__ bool verify_rows(const VerifyParams& p, int b, int& r
   return r0 >= 0 && rows > 0;
 }
 
-// Largest of entries [j0, j1) of a row: each thread takes its entries in rising order, so
-// the first largest is kept with a plain comparison.
+// Largest of entries [j0, j1) of a row. Each thread takes its 16-byte pieces in rising order
+// and compares a piece's largest value with its best; only a piece that has a larger one,
+// rare after the first few, is searched for the value's first place.
 template <typename PT>
 __device__ __forceinline__ Best scan_largest(const typename PT::T* row, int j0, int j1, bool vec) {
-  constexpr int V = PT::Vec, U = 4;
+  constexpr int V = PT::Vec, U = 8;
   Best best{-INFINITY, INT_MAX};
   auto take = [&](float f, int j) {
     if (f > best.score) best = Best{f, j};
   };
   if (vec) {
-    const int step = V * kVerifyThreads;
-    for (int j = j0 + V * (int)threadIdx.x; j < j1; j += U * step) {
-      float f[U][V];
+    constexpr int step = V * kVerifyThreads;
+    const int jv = j0 + (j1 - j0) / V * V;  // whole pieces; part boundaries are multiples of 8
+    for (int j = j0 + V * (int)threadIdx.x; j < jv; j += U * step) {
+      uint4 x[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (j + u * step + V <= j1) PT::load_vec(row + j + u * step, f[u]);
+      for (int u = 0; u < U; ++u) x[u] = __ldg(reinterpret_cast<const uint4*>(row + min(j + u * step, jv - V)));
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int at = j + u * step;
-        if (at + V <= j1) {
+        const float m = PT::largest(x[u]);
+        if (m > best.score && j + u * step < jv) {
+          float f[V];
+          PT::values(x[u], f);
+          int at = 0;
 #pragma unroll
-          for (int e = 0; e < V; ++e) take(f[u][e], at + e);
-        } else {
-          for (int e = at; e < j1; ++e) take(PT::load(row + e), e);
+          for (int e = V - 1; e >= 0; --e) at = f[e] == m ? e : at;
+          best = Best{m, j + u * step + at};
         }
       }
     }
+    for (int j = jv + (int)threadIdx.x; j < j1; j += kVerifyThreads) take(PT::load(row + j), j);
     return best;
   }
-  constexpr int US = 8;
-  for (int j = j0 + (int)threadIdx.x; j < j1; j += US * kVerifyThreads) {
-    float f[US];
+  for (int j = j0 + (int)threadIdx.x; j < j1; j += U * kVerifyThreads) {
+    float f[U];
 #pragma unroll
-    for (int u = 0; u < US; ++u) f[u] = j + u * kVerifyThreads < j1 ? PT::load(row + j + u * kVerifyThreads) : -INFINITY;
+    for (int u = 0; u < U; ++u) f[u] = j + u * kVerifyThreads < j1 ? PT::load(row + j + u * kVerifyThreads) : -INFINITY;
 #pragma unroll
-    for (int u = 0; u < US; ++u) take(f[u], j + u * kVerifyThreads);
+    for (int u = 0; u < U; ++u) take(f[u], j + u * kVerifyThreads);
   }
   return best;
 }
@@ -175,7 +186,7 @@ __device__ __forceinline__ Best scan_race(const typename PT::T* prow, const type
     const int step = V * kVerifyThreads;
     auto load4 = [&](const typename PT::T* p, float (&f)[V]) {
       if constexpr (sizeof(typename PT::T) == 4) {
-        PT::load_vec(p, f);
+        PT::values(__ldg(reinterpret_cast<const uint4*>(p)), f);
       } else {
         const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
         const typename PT::T h[4] = {(uint16_t)v.x, (uint16_t)(v.x >> 16), (uint16_t)v.y, (uint16_t)(v.y >> 16)};
