@@ -32,7 +32,7 @@
 // an odd polynomial fitted to tanh (tests/tanh_fit.py, absolute error 6.5e-7 of the cap)
 // whose last product merges with the subtraction of the maximum: four more operations per
 // score on the FMA pipe, which the exponentials leave half idle. Tiles with larger
-// scores, rare in models that cap them, and tiles that a mask cuts take the MUFU form.
+// scores, rare in models that cap them, take the MUFU form.
 #pragma once
 
 #include "gqa_prefill.cuh"
@@ -41,8 +41,10 @@
 namespace gqa {
 
 // Score transforms of an instantiation: kRaggedPlain none; kRaggedCap the cap alone
-// (monotone, so the row maximum is taken before it); kRaggedBias a distance bias, capped or not.
-enum : int { kRaggedPlain = 0, kRaggedCap = 1, kRaggedBias = 2 };
+// (monotone, so the row maximum is taken before it); kRaggedBias a distance bias alone,
+// kRaggedCapBias both. An instantiation each: code that a call does not use costs the
+// softmax warps registers (one for bias with and without a cap: 7 % slower without).
+enum : int { kRaggedPlain = 0, kRaggedCap = 1, kRaggedBias = 2, kRaggedCapBias = 3 };
 
 // tanh(y) ~ y (c0 + c1 y^2 + c2 y^4 + c3 y^6), |y| <= kTanhRange.
 constexpr float kTanhRange = 0.6f;
@@ -481,7 +483,7 @@ __global__ void __launch_bounds__(384, 1)
       w.t0 = work->t0;
       int pos;
       ragged_row(p, w, i_row, pos, low, rem);
-      if constexpr (MOD == kRaggedBias) {
+      if constexpr (MOD >= kRaggedBias) {
         slope = p.alibi[kvh * p.group + row % p.group] * 1.4426950408889634f;
         dist = (float)(pos - key);
       }
@@ -534,22 +536,36 @@ __global__ void __launch_bounds__(384, 1)
       // linear in the key, slope (c - distance of column 0).
       auto biased = [&](int c0) {
         const float d0 = dist - (float)(n * kstep);
-        if (p.cap_in == 0.f && p.linear_bias) {
+        auto each = [&](auto score) {
+#pragma unroll
+          for (int c = c0; c < c0 + 64; ++c)
+            sr[c] = __float_as_uint(fmaf(-slope, fabsf(d0 - (float)c), score(__uint_as_float(sr[c]))));
+        };
+        if constexpr (MOD == kRaggedCapBias) {
+          float big = 0.f, big1 = 0.f;
+#pragma unroll
+          for (int c = c0; c < c0 + 64; c += 4) {
+            big = max3_abs(big, __uint_as_float(sr[c]), __uint_as_float(sr[c + 1]));
+            big1 = max3_abs(big1, __uint_as_float(sr[c + 2]), __uint_as_float(sr[c + 3]));
+          }
+          if (__all_sync(0xffffffffu, idle || fmaxf(big, big1) <= p.cap_most)) {  // the cap's polynomial holds
+            each([&](float s) {
+              const float z = s * s;
+              return s * fmaf(fmaf(fmaf(p.cap_a[3], z, p.cap_a[2]), z, p.cap_a[1]), z, p.cap_a[0]);
+            });
+          } else {
+            each([&](float s) { return fmaf(-2.f * p.cap_out, fast_rcp(1.f + fast_exp2(s * p.cap_in)), p.cap_out); });
+          }
+        } else if (p.linear_bias) {
           const float b0 = -slope * d0;
 #pragma unroll
           for (int c = c0; c < c0 + 64; ++c)
             sr[c] = __float_as_uint(fmaf(__uint_as_float(sr[c]), p.scale_log2, fmaf(slope, (float)c, b0)));
         } else {
-#pragma unroll
-          for (int c = c0; c < c0 + 64; ++c) {
-            const float s = __uint_as_float(sr[c]);
-            float x = s * p.scale_log2;
-            if (p.cap_in != 0.f) x = fmaf(-2.f * p.cap_out, fast_rcp(1.f + fast_exp2(s * p.cap_in)), p.cap_out);
-            sr[c] = __float_as_uint(fmaf(-slope, fabsf(d0 - (float)c), x));
-          }
+          each([&](float s) { return s * p.scale_log2; });
         }
       };
-      if constexpr (MOD == kRaggedBias) biased(0);
+      if constexpr (MOD >= kRaggedBias) biased(0);
       auto mask = [&](int c0) {
         if (cut_hi) {
 #pragma unroll
@@ -575,7 +591,7 @@ __global__ void __launch_bounds__(384, 1)
       mx1 = max3(mx1, __uint_as_float(sr[62]), __uint_as_float(sr[63]));
       asm volatile("tcgen05.wait::ld.sync.aligned;" ::"f"(mx0), "f"(mx1), "f"(mx2), "f"(mx3) : "memory");
       reg_fence_n<64>(sr + 64);
-      if constexpr (MOD == kRaggedBias) biased(64);
+      if constexpr (MOD >= kRaggedBias) biased(64);
       mask(64);
 #pragma unroll
       for (int c = 64; c < 128; c += 8) {
@@ -633,22 +649,37 @@ __global__ void __launch_bounds__(384, 1)
       static_assert(kPairs == 32, "one 32-column store per part");
       const float2 nm2 = make_float2(-m_run, -m_run);
       if constexpr (MOD == kRaggedCap) {
+        // The polynomial if every visible score of the warp's rows is small enough.
+        const bool cut = cut_hi || cut_lo;
         float big = 0.f, big1 = 0.f;
-        const bool any_masked = cut_hi || cut_lo;
-        if (!any_masked) {
+        if (!cut) {
 #pragma unroll
           for (int c = 0; c < 128; c += 4) {
             big = max3_abs(big, __uint_as_float(sr[c]), __uint_as_float(sr[c + 1]));
             big1 = max3_abs(big1, __uint_as_float(sr[c + 2]), __uint_as_float(sr[c + 3]));
           }
+        } else {
+#pragma unroll
+          for (int c = 0; c < 128; ++c) {
+            const float s = __uint_as_float(sr[c]);
+            big = fmaxf(big, s == -INFINITY ? 0.f : fabsf(s));
+          }
         }
-        if (!any_masked && __all_sync(0xffffffffu, idle || fmaxf(big, big1) <= p.cap_most)) {
+        if (__all_sync(0xffffffffu, idle || fmaxf(big, big1) <= p.cap_most)) {
           const float2 a0 = make_float2(p.cap_a[0], p.cap_a[0]), a1 = make_float2(p.cap_a[1], p.cap_a[1]);
           const float2 a2 = make_float2(p.cap_a[2], p.cap_a[2]), a3 = make_float2(p.cap_a[3], p.cap_a[3]);
-          publish([&](float2 s) {
+          auto capped = [&](float2 s) {
             const float2 z = make_float2(s.x * s.x, s.y * s.y);
             return fma2(s, fma2(fma2(fma2(a3, z, a2), z, a1), z, a0), nm2);
-          });
+          };
+          if (!cut) {
+            publish(capped);
+          } else {
+            publish([&](float2 s) {
+              const float2 x = capped(s);
+              return make_float2(s.x == -INFINITY ? s.x : x.x, s.y == -INFINITY ? s.y : x.y);
+            });
+          }
         } else {
         const float cin = p.cap_in, cout2 = -2.f * p.cap_out, off = p.cap_out - m_run;
         publish([&](float2 s) {

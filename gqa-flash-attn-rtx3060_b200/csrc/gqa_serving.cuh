@@ -22,6 +22,8 @@ template <int HD, bool BF>
 cudaError_t launch_ragged_tile(const RaggedParams& p, unsigned grid, const CUtensorMap& qm, const CUtensorMap& km,
                                   const CUtensorMap& vm, cudaStream_t st) {
   using Cfg = RaggedTileCfg<HD>;
+  if (p.alibi && p.cap_in != 0.f)
+    return launch_pdl(gqa_ragged_tile_kernel<HD, BF, kRaggedCapBias>, grid, Cfg::kThreads, Cfg::kSmemBytes, st, p, qm, km, vm);
   if (p.alibi)
     return launch_pdl(gqa_ragged_tile_kernel<HD, BF, kRaggedBias>, grid, Cfg::kThreads, Cfg::kSmemBytes, st, p, qm, km, vm);
   if (p.cap_in != 0.f)
@@ -41,6 +43,7 @@ int prepare_ragged() {
   prep(gqa_ragged_tile_kernel<HD, BF, kRaggedPlain>, RaggedTileCfg<HD>::kSmemBytes, kRegs);  \
   prep(gqa_ragged_tile_kernel<HD, BF, kRaggedCap>, RaggedTileCfg<HD>::kSmemBytes, kRegs);    \
   prep(gqa_ragged_tile_kernel<HD, BF, kRaggedBias>, RaggedTileCfg<HD>::kSmemBytes, kRegs);   \
+  prep(gqa_ragged_tile_kernel<HD, BF, kRaggedCapBias>, RaggedTileCfg<HD>::kSmemBytes, kRegs); \
   prep(gqa_ragged_stream_kernel<HD, BF, false>, StreamCfg<HD>::kSmemBytes, 0)
   GQA_PREP_RAGGED(128, true); GQA_PREP_RAGGED(128, false); GQA_PREP_RAGGED(64, true); GQA_PREP_RAGGED(64, false);
 #undef GQA_PREP_RAGGED
