@@ -40,6 +40,8 @@
 
 namespace gqa {
 
+constexpr int kMaxRaggedChunks = 16;  // key chunks of a tile
+
 // Score transforms of an instantiation: kRaggedPlain none; kRaggedCap the cap alone
 // (monotone, so the row maximum is taken before it); kRaggedBias a distance bias alone,
 // kRaggedCapBias both. An instantiation each: code that a call does not use costs the
@@ -659,11 +661,14 @@ __global__ void __launch_bounds__(384, 1)
             big1 = max3_abs(big1, __uint_as_float(sr[c + 2]), __uint_as_float(sr[c + 3]));
           }
         } else {
+          float b2[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int c = 0; c < 128; ++c) {
             const float s = __uint_as_float(sr[c]);
-            big = fmaxf(big, s == -INFINITY ? 0.f : fabsf(s));
+            b2[c & 3] = fmaxf(b2[c & 3], s == -INFINITY ? 0.f : fabsf(s));
           }
+          big = fmaxf(b2[0], b2[1]);
+          big1 = fmaxf(b2[2], b2[3]);
         }
         if (__all_sync(0xffffffffu, idle || fmaxf(big, big1) <= p.cap_most)) {
           const float2 a0 = make_float2(p.cap_a[0], p.cap_a[0]), a1 = make_float2(p.cap_a[1], p.cap_a[1]);
@@ -818,49 +823,44 @@ __global__ void __launch_bounds__(384, 1)
       asm volatile("bar.sync 3, 256;" ::: "memory");
       store = *last_slot != 0;
       if (store && !idle_warp) {
-        for (int s0 = 0; s0 < n_chunks; s0 += 4) {
-          float mv[4];
+        // Every chunk's m and l at once (at most kMaxRaggedChunks), then their weights.
+        float mv[kMaxRaggedChunks], lv[kMaxRaggedChunks];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) mv[i] = __ldcg(tl.ws_m + pbase + (int64_t)min(s0 + i, n_chunks - 1) * 256);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) M = fmaxf(M, mv[i]);
+        for (int i = 0; i < kMaxRaggedChunks; ++i) {
+          const int64_t at = pbase + (int64_t)min(i, n_chunks - 1) * 256;
+          mv[i] = __ldcg(tl.ws_m + at);
+          lv[i] = __ldcg(tl.ws_l + at);
         }
+#pragma unroll
+        for (int i = 0; i < kMaxRaggedChunks; ++i) M = fmaxf(M, mv[i]);
         L = 0.f;
-        for (int s0 = 0; s0 < n_chunks; s0 += 4) {
-          float mv[4], lv[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int64_t o2 = pbase + (int64_t)min(s0 + i, n_chunks - 1) * 256;
-            mv[i] = __ldcg(tl.ws_m + o2);
-            lv[i] = __ldcg(tl.ws_l + o2);
-          }
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (s0 + i < n_chunks) L += fast_exp2(mv[i] - M) * lv[i];
-        }
+        for (int i = 0; i < kMaxRaggedChunks; ++i)
+          if (i < n_chunks) L += fast_exp2(mv[i] - M) * lv[i];
         const float inv = inverse(L);
 #pragma unroll 1
         for (int c = c_begin; c < c_end; ++c) {
-          // Two chunks per pass: 64 independent loads in flight per thread. An index past
+          // Four chunks per pass: 128 independent loads in flight per thread. An index past
           // the last chunk reads a valid partial at weight 0.
           uint32_t orr[32];
 #pragma unroll
           for (int e = 0; e < 32; ++e) orr[e] = 0u;
-          for (int s0 = 0; s0 < n_chunks; s0 += 2) {
-            const int sa = s0, sb = min(s0 + 1, n_chunks - 1);
-            const float wa = fast_exp2(__ldcg(tl.ws_m + pbase + (int64_t)sa * 256) - M);
-            const float wb = (s0 + 1 >= n_chunks) ? 0.f : fast_exp2(__ldcg(tl.ws_m + pbase + (int64_t)sb * 256) - M);
-            const float* xa = tl.ws_acc + ((int64_t)unit * tl.nsplit + sa) * HD * 256 + prow + c * 32 * 256;
-            const float* xb = tl.ws_acc + ((int64_t)unit * tl.nsplit + sb) * HD * 256 + prow + c * 32 * 256;
-            float va[32], vb[32];
+          for (int s0 = 0; s0 < n_chunks; s0 += 4) {
+            float wt[4], x[4][32];
 #pragma unroll
-            for (int e = 0; e < 32; ++e) {
-              va[e] = __ldcg(xa + e * 256);
-              vb[e] = __ldcg(xb + e * 256);
+            for (int i = 0; i < 4; ++i) {
+              const int si = min(s0 + i, n_chunks - 1);
+              wt[i] = __ldcg(tl.ws_m + pbase + (int64_t)si * 256);
+              const float* xi = tl.ws_acc + ((int64_t)unit * tl.nsplit + si) * HD * 256 + prow + c * 32 * 256;
+#pragma unroll
+              for (int e = 0; e < 32; ++e) x[i][e] = __ldcg(xi + e * 256);
             }
 #pragma unroll
-            for (int e = 0; e < 32; ++e)
-              orr[e] = __float_as_uint(fmaf(wb, vb[e], fmaf(wa, va[e], __uint_as_float(orr[e]))));
+            for (int i = 0; i < 4; ++i) {
+              wt[i] = s0 + i < n_chunks ? fast_exp2(wt[i] - M) : 0.f;
+#pragma unroll
+              for (int e = 0; e < 32; ++e) orr[e] = __float_as_uint(fmaf(wt[i], x[i][e], __uint_as_float(orr[e])));
+            }
           }
           stage_chunk(c, orr, inv);
         }

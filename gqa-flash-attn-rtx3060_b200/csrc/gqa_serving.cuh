@@ -123,7 +123,7 @@ RaggedPlan plan_ragged(const RaggedShape& s, bool fp8, int sm_count) {
     const int64_t units = tiling_units(t, s.hkv);
     const int keys = s.head_dim == 128 ? RaggedTileCfg<128>::kBN : RaggedTileCfg<64>::kBN;
     const int span = ragged_span(s, t.block_m) + keys;
-    const int most = (units < sm_count && units <= kServingCounters / 2) ? std::max(1, std::min(16, span / (2 * keys))) : 1;
+    const int most = (units < sm_count && units <= kServingCounters / 2) ? std::max(1, std::min(kMaxRaggedChunks, span / (2 * keys))) : 1;
     split_keys(t, units, span, keys, sm_count, 12.0, most);
     pl.tile_ctas = units * t.nsplit;
   }
@@ -445,12 +445,12 @@ struct VerifyPlan {
   int nsplit, part;
 };
 
-// CTAs per row: about one wave over the device, at least 1024 entries each. Four CTAs of
-// the race fit an SM (registers), five of the greedy scan, of whose rows -- the most that
-// the requests can have -- a good part is usually absent.
+// CTAs per row: about one wave over the device, at least 1024 entries each. Five CTAs fit
+// an SM (registers); of the greedy scan's rows -- the most that the requests can have -- a
+// good part is usually absent.
 VerifyPlan plan_verify(int64_t rows, int vocab, int sm_count, bool greedy) {
   VerifyPlan pl;
-  const int64_t want = (int64_t)sm_count * (greedy ? 8 : 4) / std::max<int64_t>(rows, 1);
+  const int64_t want = (int64_t)sm_count * (greedy ? 8 : 5) / std::max<int64_t>(rows, 1);
   const int64_t most = std::max(1, vocab / 1024);
   pl.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>(std::min(want, most), 256));
   pl.part = (((vocab + pl.nsplit - 1) / pl.nsplit) + 7) & ~7;

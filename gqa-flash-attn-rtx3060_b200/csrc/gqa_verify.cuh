@@ -173,7 +173,7 @@ __device__ __forceinline__ Best scan_largest(const typename PT::T* row, int j0, 
 template <typename PT>
 __device__ __forceinline__ Best scan_race(const typename PT::T* prow, const typename PT::T* qrow, const float* erow, int hidden,
                                           int j0, int j1, bool vec) {
-  constexpr int V = 4, U = 2, US = 8;
+  constexpr int V = 4, U = 2, US = 4;
   Best best{0.f, INT_MAX};
   auto take = [&](float pj, float qj, float ej, int j) {
     const float w = __fsub_rn(pj, qj);
@@ -219,8 +219,10 @@ __device__ __forceinline__ Best scan_race(const typename PT::T* prow, const type
     }
     return best;
   }
-  for (int j = j0 + (int)threadIdx.x; j < j1; j += US * kVerifyThreads) {
-    float a[US], c[US], e[US];
+  // Rows of an odd vocabulary: one value per load, coalesced; the next US of each row are in
+  // flight while these are compared.
+  float a[US], c[US], e[US];
+  auto load = [&](int j) {
 #pragma unroll
     for (int u = 0; u < US; ++u) {
       const int at = min(j + u * kVerifyThreads, j1 - 1);
@@ -228,9 +230,23 @@ __device__ __forceinline__ Best scan_race(const typename PT::T* prow, const type
       c[u] = qrow ? PT::load(qrow + at) : 0.f;
       e[u] = __ldg(erow + at);
     }
+  };
+  int j = j0 + (int)threadIdx.x;
+  if (j < j1) load(j);
+  while (j < j1) {
+    float a1[US], c1[US], e1[US];
+#pragma unroll
+    for (int u = 0; u < US; ++u) {
+      a1[u] = a[u];
+      c1[u] = c[u];
+      e1[u] = e[u];
+    }
+    const int next = j + US * kVerifyThreads;
+    if (next < j1) load(next);
 #pragma unroll
     for (int u = 0; u < US; ++u)
-      if (j + u * kVerifyThreads < j1) take(a[u], c[u], e[u], j + u * kVerifyThreads);
+      if (j + u * kVerifyThreads < j1) take(a1[u], c1[u], e1[u], j + u * kVerifyThreads);
+    j = next;
   }
   return best;
 }
