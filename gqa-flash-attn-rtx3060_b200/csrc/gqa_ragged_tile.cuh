@@ -1,6 +1,6 @@
 // tcgen05 / TMEM / TMA form of the ragged attention (gqa_ragged.cuh has the masks, the
 // scores and the work of a tile): requests of more than kRaggedStreamRows packed rows, i.e.
-// prompts, chunks of them and most drafts. The pipeline is the dense prefill kernel's (gqa_prefill.cuh): one CTA
+// prompts, chunks of them and long drafts. The pipeline is the dense prefill kernel's (gqa_prefill.cuh): one CTA
 // owns two 128-row query tiles of one (request, kv head), a TMA warp streams 128-key
 // tiles of K and V from the paged cache, one thread issues the UMMAs
 //   S_i = Q_i K_j^T (f32 in TMEM),   O_i += P_i V_j (P from TMEM)
@@ -33,6 +33,14 @@
 // whose last product merges with the subtraction of the maximum: four more operations per
 // score on the FMA pipe, which the exponentials leave half idle. Tiles with larger
 // scores, rare in models that cap them, take the MUFU form.
+//
+// Measured, 32 query and 8 kv heads of 128, bf16, two prompts' chunks of up to 4096 tokens
+// on up to 12288 cached keys: causal 985 us, 1080 TFLOP/s; capped 1.35 ms (2.3 ms with every
+// tile in the MUFU form); capped and with a distance bias 2.25 ms (3.8 ms). A pair's step
+// of 128 keys takes 2.0 us (the softmax chain, then the wait for its S), a solo step
+// 1.05 us per 128 keys, and a CTA about 10 us besides: the scan 2, the first S 2.5, a
+// masked tile 1.3, the epilogue 3 to 4. Slower, and not kept: P beside S in TMEM, which at
+// head size 128 leaves room for 64- or 80-key tiles only (677 and 836 TFLOP/s).
 #pragma once
 
 #include "gqa_prefill.cuh"
