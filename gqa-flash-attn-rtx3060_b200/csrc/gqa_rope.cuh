@@ -14,14 +14,17 @@
 // D / 8 lanes hold one head's row as two 8-byte pieces, four values a and their four
 // partners b (no shuffles; for neighbouring pairs and for values past `rot` the pieces are
 // neighbours), arithmetic is packed two values at a time, and the work is cut into units
-// of two rows that share cosines and sines: two query heads, or a head's key and value, of
-// one token. Query and key-value units are different CTAs, so that a unit has no branches
-// on what a row is, and a lane group goes through its units by additions. The next unit's
-// position and slot are in flight while this one is turned, and its rows and table entries
-// leave together. 16381 tokens of 32 query and 8 kv heads of 128, bf16, three axes: 86 us,
-// 4.8 TB/s, 0.73 of a plain copy; four CTAs per SM (64 registers a thread) measured best,
-// three hide less latency, five and six spill. 16 tokens: 4.7 us, a launch and three
-// dependent loads. Everything between the load and the one rounding of the store is fp32.
+// of four rows of one token that share cosines and sines: four query heads, or the keys
+// and values of two heads. Query and key-value units are different CTAs, so that a unit has
+// no branches on what a row is, and a lane group goes through its units by additions. The
+// next unit's position and slot are in flight while this one is turned, and its rows and
+// table entries leave together. Everything between the load and the one rounding of the
+// store is fp32.
+//
+// 16381 tokens of 32 query and 8 kv heads of 128, bf16, three axes: 79 us, 5.2 TB/s, 0.80
+// of a plain copy (units of two rows 85 us, of eight 80 with three CTAs per SM; four CTAs
+// are 64 registers a thread, three hide less latency and take 87, five and six spill; the
+// next unit's rows fetched ahead 94). 16 tokens: 4.6 us, a launch and three dependent loads.
 #pragma once
 
 #include "gqa_cache.cuh"
@@ -106,6 +109,7 @@ __device__ __forceinline__ void store_cache(void* cache, int64_t at, int da, int
 
 constexpr int kRopeThreads = 256;
 constexpr int kRopeCtas = 4;  // per SM
+constexpr int kRopeRows = 4;  // of a unit
 template <int D>
 struct RopeCfg {
   static constexpr int kLanes = D / 8;                   // lanes per row
@@ -163,8 +167,8 @@ __device__ __forceinline__ void rope_row(float2 (&a)[2], float2 (&b)[2], const R
   }
 }
 
-// The units of one kind, from `first` on, `step` apart: unit u is head pair (or key-value
-// head) u % per_token of token u / per_token.
+// The units of one kind, from `first` on, `step` apart: unit u is number u % per_token of
+// token u / per_token.
 template <int D, bool BF16, bool FP8, bool INTER, bool IS_Q>
 __device__ __forceinline__ void rope_units(const RopeParams& p, const RopeLane<D, INTER>& ln, unsigned first, unsigned step,
                                            unsigned per_token) {
@@ -200,14 +204,26 @@ __device__ __forceinline__ void rope_units(const RopeParams& p, const RopeLane<D
   while (true) {
     const Place it = next;
     const int tok = t, un = u;
-    // The unit's two rows: query heads 2 un and 2 un + 1 (the last may be alone), or key
-    // and value of head un.
-    const bool both = IS_Q ? 2 * un + 1 < p.hq : p.v_dst != nullptr;
-    const uint16_t* const x0 = IS_Q ? p.q + tok * p.q_st + 2 * un * p.q_sh : p.k + tok * p.k_st + un * p.k_sh;
-    const uint16_t* const x1 = IS_Q ? x0 + p.q_sh : p.v + tok * p.v_st + un * p.v_sh;
-    const Piece r0 = load_piece(x0, ln.da, ln.db);
-    Piece r1{};
-    if (both) r1 = load_piece(x1, ln.da, ln.db);
+    // The unit's rows: query heads kRopeRows un and on, or the key and the value of heads
+    // kRopeRows / 2 un and on; the last unit of a token may have fewer.
+    constexpr int kHeads = IS_Q ? kRopeRows : kRopeRows / 2;
+    const int h0 = kHeads * un, heads = min(kHeads, (IS_Q ? p.hq : p.hkv) - h0);
+    Piece r[kRopeRows];
+    if constexpr (IS_Q) {
+      const uint16_t* x = p.q + tok * p.q_st + h0 * p.q_sh;
+#pragma unroll
+      for (int i = 0; i < kHeads; ++i, x += p.q_sh)
+        if (i < heads) r[i] = load_piece(x, ln.da, ln.db);
+    } else {
+      const uint16_t* x = p.k + tok * p.k_st + h0 * p.k_sh;
+      const uint16_t* y = p.v + tok * p.v_st + h0 * p.v_sh;
+#pragma unroll
+      for (int i = 0; i < kHeads; ++i, x += p.k_sh, y += p.v_sh)
+        if (i < heads) {
+          r[2 * i] = load_piece(x, ln.da, ln.db);
+          if (p.v_dst) r[2 * i + 1] = load_piece(y, ln.da, ln.db);
+        }
+    }
     float2 cs[2], sn[2];
     if (ln.turned && it.valid) {
       if (ln.one_axis) {
@@ -244,20 +260,19 @@ __device__ __forceinline__ void rope_units(const RopeParams& p, const RopeLane<D
     float2 a[2], b[2];
     if constexpr (IS_Q) {
       // A padding token's query is zero.
-      uint16_t* const o0 = p.q_out + ((int64_t)tok * p.hq + 2 * un) * D;
-      Piece y0{}, y1{};
-      if (it.valid) {
-        unpack4<BF16>(r0.a, a);
-        unpack4<BF16>(r0.b, b);
-        rope_row<D, BF16, INTER>(a, b, ln, weight != nullptr, wa, wb, p.eps, cs, sn);
-        y0 = Piece{pack4<BF16>(a), pack4<BF16>(b)};
-        unpack4<BF16>(r1.a, a);
-        unpack4<BF16>(r1.b, b);
-        rope_row<D, BF16, INTER>(a, b, ln, weight != nullptr, wa, wb, p.eps, cs, sn);
-        y1 = Piece{pack4<BF16>(a), pack4<BF16>(b)};
-      }
-      store_piece(o0, ln.da, ln.db, y0);
-      if (both) store_piece(o0 + D, ln.da, ln.db, y1);
+      uint16_t* o = p.q_out + ((int64_t)tok * p.hq + h0) * D;
+#pragma unroll
+      for (int i = 0; i < kHeads; ++i, o += D)
+        if (i < heads) {
+          Piece y{};
+          if (it.valid) {
+            unpack4<BF16>(r[i].a, a);
+            unpack4<BF16>(r[i].b, b);
+            rope_row<D, BF16, INTER>(a, b, ln, weight != nullptr, wa, wb, p.eps, cs, sn);
+            y = Piece{pack4<BF16>(a), pack4<BF16>(b)};
+          }
+          store_piece(o, ln.da, ln.db, y);
+        }
     } else {
       int64_t dst = it.slot;
       if (p.slots && (dst >= p.num_slots || !it.valid)) {
@@ -265,24 +280,28 @@ __device__ __forceinline__ void rope_units(const RopeParams& p, const RopeLane<D
         dst = -1;
       }
       if (dst >= 0) {
-        const int64_t at = (dst * p.hkv + un) * D;
-        if (it.valid) {
-          unpack4<BF16>(r0.a, a);
-          unpack4<BF16>(r0.b, b);
-          rope_row<D, BF16, INTER>(a, b, ln, weight != nullptr, wa, wb, p.eps, cs, sn);
-        } else {  // padding without a cache: zero
-          a[0] = a[1] = b[0] = b[1] = make_float2(0.f, 0.f);
-        }
-        store_cache<BF16, FP8>(p.k_dst, at, ln.da, ln.db, a, b, p.k_scale);
-        if (both) {
-          if constexpr (FP8) {
-            unpack4<BF16>(r1.a, a);
-            unpack4<BF16>(r1.b, b);
-            store_cache<BF16, FP8>(p.v_dst, at, ln.da, ln.db, a, b, p.v_scale);
-          } else {
-            store_piece(reinterpret_cast<uint16_t*>(p.v_dst) + at, ln.da, ln.db, r1);
+        int64_t at = (dst * p.hkv + h0) * D;
+#pragma unroll
+        for (int i = 0; i < kHeads; ++i, at += D)
+          if (i < heads) {
+            if (it.valid) {
+              unpack4<BF16>(r[2 * i].a, a);
+              unpack4<BF16>(r[2 * i].b, b);
+              rope_row<D, BF16, INTER>(a, b, ln, weight != nullptr, wa, wb, p.eps, cs, sn);
+            } else {  // padding without a cache: zero
+              a[0] = a[1] = b[0] = b[1] = make_float2(0.f, 0.f);
+            }
+            store_cache<BF16, FP8>(p.k_dst, at, ln.da, ln.db, a, b, p.k_scale);
+            if (p.v_dst) {
+              if constexpr (FP8) {
+                unpack4<BF16>(r[2 * i + 1].a, a);
+                unpack4<BF16>(r[2 * i + 1].b, b);
+                store_cache<BF16, FP8>(p.v_dst, at, ln.da, ln.db, a, b, p.v_scale);
+              } else {
+                store_piece(reinterpret_cast<uint16_t*>(p.v_dst) + at, ln.da, ln.db, r[2 * i + 1]);
+              }
+            }
           }
-        }
       }
     }
     if (!more) return;
@@ -313,10 +332,10 @@ __global__ void __launch_bounds__(kRopeThreads, kRopeCtas) gqa_rope_kernel(const
   ln.mask = (Cfg::kLanes == 16 ? 0xffffu : 0xffu) << (lane & ~(Cfg::kLanes - 1));
   const unsigned grp = threadIdx.x / Cfg::kLanes;
   if (blockIdx.x < (unsigned)p.q_ctas)
-    rope_units<D, BF16, FP8, INTER, true>(p, ln, blockIdx.x * Cfg::kGroups + grp, p.q_ctas * Cfg::kGroups, (p.hq + 1) >> 1);
+    rope_units<D, BF16, FP8, INTER, true>(p, ln, blockIdx.x * Cfg::kGroups + grp, p.q_ctas * Cfg::kGroups, (p.hq + kRopeRows - 1) / kRopeRows);
   else
     rope_units<D, BF16, FP8, INTER, false>(p, ln, (blockIdx.x - p.q_ctas) * Cfg::kGroups + grp,
-                                           (gridDim.x - p.q_ctas) * Cfg::kGroups, p.hkv);
+                                           (gridDim.x - p.q_ctas) * Cfg::kGroups, (p.hkv + kRopeRows / 2 - 1) / (kRopeRows / 2));
 }
 
 }  // namespace gqa

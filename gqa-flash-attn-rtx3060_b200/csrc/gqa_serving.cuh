@@ -296,9 +296,10 @@ int gqa_qk_norm_rope(const gqa_qk_norm_rope_args* args, void* stream) {
   p.v_scale = a.v_scale;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const bool bf = a.dtype == GQA_DTYPE_BF16;
-  // Units of two rows; both kinds get CTAs in proportion, at most what fits the device at once.
+  // Both kinds of units get CTAs in proportion, at most what fits the device at once.
   const int groups = a.head_dim == 128 ? RopeCfg<128>::kGroups : RopeCfg<64>::kGroups;
-  const int64_t q_units = (int64_t)a.num_tokens * ((a.num_heads + 1) / 2), kv_units = (int64_t)a.num_tokens * a.num_kv_heads;
+  const int64_t q_units = (int64_t)a.num_tokens * ((a.num_heads + kRopeRows - 1) / kRopeRows);
+  const int64_t kv_units = (int64_t)a.num_tokens * ((a.num_kv_heads + kRopeRows / 2 - 1) / (kRopeRows / 2));
   if (q_units > INT_MAX / 2 || kv_units > INT_MAX / 2) return GQA_ERR_INVALID_ARG;
   const int64_t q_need = (q_units + groups - 1) / groups, kv_need = (kv_units + groups - 1) / groups;
   const int64_t fit = (int64_t)kRopeCtas * sm;
