@@ -178,9 +178,13 @@ __device__ __forceinline__ float fast_rcp(float x) {
 }
 
 // Score in log2 units. 2 MUFU operations for the cap; exact at both ends (2^inf -> tanh 1).
-__device__ __forceinline__ float ragged_score(const RaggedParams& p, float s, float slope, int pos, int key) {
-  float x = s * p.scale_log2;
-  if (p.cap_in != 0.f) x = fmaf(-2.f * p.cap_out, fast_rcp(1.f + fast_exp2(s * p.cap_in)), p.cap_out);
+struct RaggedScore {  // in registers: the parameters are not in constant memory of a function
+  float scale, cap_in, cap_out;
+  int mods;
+};
+__device__ __forceinline__ float ragged_score(const RaggedScore& sc, float s, float slope, int pos, int key) {
+  float x = s * sc.scale;
+  if (sc.cap_in != 0.f) x = fmaf(-2.f * sc.cap_out, fast_rcp(1.f + fast_exp2(s * sc.cap_in)), sc.cap_out);
   return fmaf(-slope, fabsf((float)(pos - key)), x);
 }
 
@@ -270,7 +274,7 @@ __device__ __forceinline__ void ragged_stream_compute(const RaggedParams& p, con
   for (int i = 0; i < NACC; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
   float m_run[2] = {-INFINITY, -INFINITY};
   float l_run[2] = {0.f, 0.f};
-  const float scale = p.scale_log2;
+  const RaggedScore sc{p.scale_log2, p.cap_in, p.cap_out, p.mods};
 
   for (int t = 0; t < n_stages; ++t) {
     const int slot = t % Cfg::kStages;
@@ -328,7 +332,7 @@ __device__ __forceinline__ void ragged_stream_compute(const RaggedParams& p, con
         for (int e = 0; e < 4; ++e) {
           const int key = key_w + gr + 8 * (e >> 1), h = e & 1;
           const float raw = st[0][e] + st[1][e];
-          const float x = p.mods ? ragged_score(p, raw, slope_r[h], pos_r[h], key) : raw * scale;
+          const float x = sc.mods ? ragged_score(sc, raw, slope_r[h], pos_r[h], key) : raw * sc.scale;
           s[e] = (key >= lo_r[h] && key < hi_r[h]) ? x : -INFINITY;
           mx[h] = fmaxf(mx[h], s[e]);
         }
@@ -427,7 +431,7 @@ __device__ __forceinline__ void ragged_stream_compute(const RaggedParams& p, con
           for (int e = 0; e < 4; ++e) {
             const int h = e >> 1;
             const int key = key_w + nb * 8 + gc * 2 + (e & 1);
-            const float x = p.mods ? ragged_score(p, s[nb][e], slope_r[h], pos_r[h], key) : s[nb][e] * scale;
+            const float x = sc.mods ? ragged_score(sc, s[nb][e], slope_r[h], pos_r[h], key) : s[nb][e] * sc.scale;
             s[nb][e] = (key >= lo_r[h] && key < hi_r[h]) ? x : -INFINITY;
             mx[h] = fmaxf(mx[h], s[nb][e]);
           }
@@ -790,6 +794,16 @@ __device__ __forceinline__ void ragged_stream_cta(const RaggedParams& p, const C
   } else if constexpr (FP8) {  // 16-bit tiles have at most kRaggedStreamRows rows
     ragged_stream_compute<HD, BF16, 4, FP8, false>(p, w, smem, base, k_begin, k_end, n_stages, unit, split, kvh);
   }
+}
+
+// The streaming form as a function of its own, for the tcgen05 kernel with a distance bias,
+// whose softmax warps otherwise spill more (two chunks beside 30 decodes, with bias and
+// window: 229 us inlined, 213 so; heads of 64: 194 and 183). With a cap, inlined is ahead
+// (16 capped drafts 55 us, 65 so), and plain steps do not care (305 us both).
+template <int HD, bool BF16>
+__device__ __noinline__ void ragged_stream_beside(const RaggedParams& p, const CUtensorMap* kmap, const CUtensorMap* vmap,
+                                                  unsigned cta) {
+  ragged_stream_cta<HD, BF16, false>(p, kmap, vmap, cta);
 }
 
 // Steps whose requests all stream.

@@ -108,7 +108,10 @@ __global__ void __launch_bounds__(384, 1)
   // The step's short requests stream in the grid's last CTAs: they fill the SMs as the
   // tiles run out.
   if (blockIdx.x >= p.tile_ctas) {
-    ragged_stream_cta<HD, BF16, false>(p, &kmap, &vmap, blockIdx.x - p.tile_ctas);
+    if constexpr (MOD == kRaggedBias)
+      ragged_stream_beside<HD, BF16>(p, &kmap, &vmap, blockIdx.x - p.tile_ctas);
+    else
+      ragged_stream_cta<HD, BF16, false>(p, &kmap, &vmap, blockIdx.x - p.tile_ctas);
     return;
   }
   using Cfg = RaggedTileCfg<HD>;
