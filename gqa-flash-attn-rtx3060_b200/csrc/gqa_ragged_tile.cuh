@@ -36,7 +36,7 @@
 // scores, rare in models that cap them, take the MUFU form.
 //
 // Measured, 32 query and 8 kv heads of 128, bf16, two prompts' chunks of up to 4096 tokens
-// on up to 12288 cached keys: causal 985 us, 1080 TFLOP/s; capped 1.29 ms (2.3 ms with every
+// on up to 12288 cached keys: causal 985 us, 1080 TFLOP/s; capped 1.26 ms (2.3 ms with every
 // tile in the MUFU form); capped and with a distance bias 1.8 ms (3.8 ms). A pair's step
 // of 128 keys takes 2.0 us (the softmax chain, then the wait for its S), a solo step
 // 1.05 us per 128 keys, and a CTA about 10 us besides: the scan 2, the first S 2.5, a
@@ -72,6 +72,10 @@ inline void set_cap_polynomial(RaggedParams& p, double scale_over_cap, double ca
   }
   p.cap_most = (float)(kTanhRange / scale_over_cap);
 }
+
+// With bf16, a bound of the row's scores may stand for their maximum: P has fp32's range.
+// At most this large (log2 units), so that the smallest P, 2^-2 kBoundMost, is far from it.
+constexpr float kBoundMost = 44.f;
 
 // Three-input maximum of magnitudes.
 __device__ __forceinline__ float max3_abs(float a, float b, float c) {
@@ -594,6 +598,16 @@ __global__ void __launch_bounds__(384, 1)
         }
       };
       if constexpr (MOD >= kRaggedBias) biased(0);
+      // With a cap and bf16 the largest magnitude, hidden scores' included, is all that a
+      // tile needs: it says whether the polynomial holds, and its multiple by the
+      // polynomial's slope at 0 bounds the row's scores and serves as their maximum. The
+      // maximum itself is taken where the polynomial does not hold. (f16 has no exponents
+      // for P that far below 1: maximum and magnitude both, 5 to 9 % slower.)
+      constexpr bool kMagnitude = MOD == kRaggedCap && BF16;
+      auto most = [&](float m, uint32_t a, uint32_t b) {
+        if constexpr (kMagnitude) return max3_abs(m, __uint_as_float(a), __uint_as_float(b));
+        else return max3(m, __uint_as_float(a), __uint_as_float(b));
+      };
       auto mask = [&](int c0) {
         if (cut_hi) {
 #pragma unroll
@@ -604,33 +618,47 @@ __global__ void __launch_bounds__(384, 1)
           for (int c = c0; c < c0 + 64; ++c) sr[c] = (c >= low) ? sr[c] : __float_as_uint(-INFINITY);
         }
       };
-      mask(0);
+      if constexpr (!kMagnitude) mask(0);
       // Row max with three-input maxima, four independent chains.
       float mx0 = __uint_as_float(sr[0]), mx1 = __uint_as_float(sr[1]);
       float mx2 = __uint_as_float(sr[2]), mx3 = __uint_as_float(sr[3]);
 #pragma unroll
       for (int c = 4; c < 60; c += 8) {
-        mx0 = max3(mx0, __uint_as_float(sr[c]), __uint_as_float(sr[c + 1]));
-        mx1 = max3(mx1, __uint_as_float(sr[c + 2]), __uint_as_float(sr[c + 3]));
-        mx2 = max3(mx2, __uint_as_float(sr[c + 4]), __uint_as_float(sr[c + 5]));
-        mx3 = max3(mx3, __uint_as_float(sr[c + 6]), __uint_as_float(sr[c + 7]));
+        mx0 = most(mx0, sr[c], sr[c + 1]);
+        mx1 = most(mx1, sr[c + 2], sr[c + 3]);
+        mx2 = most(mx2, sr[c + 4], sr[c + 5]);
+        mx3 = most(mx3, sr[c + 6], sr[c + 7]);
       }
-      mx0 = max3(mx0, __uint_as_float(sr[60]), __uint_as_float(sr[61]));
-      mx1 = max3(mx1, __uint_as_float(sr[62]), __uint_as_float(sr[63]));
+      mx0 = most(mx0, sr[60], sr[61]);
+      mx1 = most(mx1, sr[62], sr[63]);
       asm volatile("tcgen05.wait::ld.sync.aligned;" ::"f"(mx0), "f"(mx1), "f"(mx2), "f"(mx3) : "memory");
       reg_fence_n<64>(sr + 64);
       if constexpr (MOD >= kRaggedBias) biased(64);
-      mask(64);
+      if constexpr (!kMagnitude) mask(64);
 #pragma unroll
       for (int c = 64; c < 128; c += 8) {
-        mx0 = max3(mx0, __uint_as_float(sr[c]), __uint_as_float(sr[c + 1]));
-        mx1 = max3(mx1, __uint_as_float(sr[c + 2]), __uint_as_float(sr[c + 3]));
-        mx2 = max3(mx2, __uint_as_float(sr[c + 4]), __uint_as_float(sr[c + 5]));
-        mx3 = max3(mx3, __uint_as_float(sr[c + 6]), __uint_as_float(sr[c + 7]));
+        mx0 = most(mx0, sr[c], sr[c + 1]);
+        mx1 = most(mx1, sr[c + 2], sr[c + 3]);
+        mx2 = most(mx2, sr[c + 4], sr[c + 5]);
+        mx3 = most(mx3, sr[c + 6], sr[c + 7]);
       }
       mx = fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3));
+      bool small = false;  // kMagnitude: the polynomial holds for every score of the warp's rows
+      if constexpr (kMagnitude) {
+        small = __all_sync(0xffffffffu, idle || (mx <= p.cap_most && mx * p.cap_a[0] <= kBoundMost));
+        mask(0);
+        mask(64);
+        if (small) {
+          // |tanh y| <= |y|; hidden scores say nothing of a row that sees none of the tile.
+          mx = max(low, 0) < min(rem, BN) ? mx * p.cap_a[0] : -INFINITY;
+        } else {
+          mx = -INFINITY;
+#pragma unroll
+          for (int c = 0; c < 128; c += 2) mx = max3(mx, __uint_as_float(sr[c]), __uint_as_float(sr[c + 1]));
+        }
+      }
       if constexpr (MOD == kRaggedPlain) mx *= p.scale_log2;
-      if constexpr (MOD == kRaggedCap)
+      if (MOD == kRaggedCap && !small)
         mx = mx == -INFINITY ? mx : fmaf(-2.f * p.cap_out, fast_rcp(1.f + fast_exp2(mx * p.cap_in)), p.cap_out);
       const float m_new = fmaxf(m_run, mx);
       const bool need = !idle && m_new > m_run + 8.0f;
@@ -679,6 +707,7 @@ __global__ void __launch_bounds__(384, 1)
       if constexpr (MOD == kRaggedCap) {
         // The polynomial if every visible score of the warp's rows is small enough.
         const bool cut = cut_hi || cut_lo;
+        if constexpr (!kMagnitude) {
         float big = 0.f, big1 = 0.f;
         if (!cut) {
 #pragma unroll
@@ -696,7 +725,9 @@ __global__ void __launch_bounds__(384, 1)
           big = fmaxf(b2[0], b2[1]);
           big1 = fmaxf(b2[2], b2[3]);
         }
-        if (__all_sync(0xffffffffu, idle || fmaxf(big, big1) <= p.cap_most)) {
+          small = __all_sync(0xffffffffu, idle || fmaxf(big, big1) <= p.cap_most);
+        }
+        if (small) {
           const float2 a0 = make_float2(p.cap_a[0], p.cap_a[0]), a1 = make_float2(p.cap_a[1], p.cap_a[1]);
           const float2 a2 = make_float2(p.cap_a[2], p.cap_a[2]), a3 = make_float2(p.cap_a[3], p.cap_a[3]);
           auto capped = [&](float2 s) {

@@ -89,6 +89,23 @@ def test_documents(mix, softcap):
         key_starts=torch.tensor(starts, dtype=torch.int32, device="cuda"))
 
 
+@pytest.mark.parametrize("first,n", [(100, 256), (200, 200 + 33), (64, 1000)])
+def test_low_scores_after_hidden_small_ones(first, n):
+    """A document whose scores are all far below 0, after one with scores near 0 that it does
+    not see: what it does not see sets no scale for it."""
+    d, block, cap = 128, 16, 1000.0
+    q, kc, vc, bt, cu, lens = paged_batch([(n, 0)], 8, 2, d, block, torch.bfloat16, 21, 0.0)
+    q += 20.0
+    for k in range(n):
+        row = kc[bt[0, k // block], k % block]
+        row.copy_(row * 0.05 - 1.3 if k >= first else row * 0.01)
+    starts = torch.zeros(n, dtype=torch.int32, device="cuda")
+    starts[first:] = first
+    out = paged_ragged_attention(q, kc, vc, bt, cu, lens, softcap=cap, key_starts=starts)
+    o, _, a = attention64(q, kc, vc, bt, [(n, 0)], softcap=cap, starts=starts)
+    check_attention(out, o, a, torch.bfloat16)
+
+
 def test_rows_that_see_nothing_are_zero():
     """Key starts past the token, at the end of the keys, and a request whose cache is
     shorter than its new tokens: zero rows and -inf, their neighbours untouched."""
