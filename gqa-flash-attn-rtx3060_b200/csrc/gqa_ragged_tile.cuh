@@ -32,8 +32,8 @@
 // an odd polynomial fitted to tanh (tests/tanh_fit.py, absolute error 6.5e-7 of the cap)
 // whose last product merges with the subtraction of the maximum: four more operations per
 // pair of scores (packed; 5 % faster than with a scalar square) on the FMA pipe, which the
-// exponentials leave half idle. Tiles with larger
-// scores, rare in models that cap them, take the MUFU form.
+// exponentials leave half idle. Tiles with larger scores, rare in models that cap them,
+// take the MUFU form.
 //
 // Measured, 32 query and 8 kv heads of 128, bf16, two prompts' chunks of up to 4096 tokens
 // on up to 12288 cached keys: causal 985 us, 1080 TFLOP/s; capped 1.26 ms (2.3 ms with every

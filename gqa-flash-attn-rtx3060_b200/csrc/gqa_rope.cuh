@@ -21,7 +21,7 @@
 // table entries leave together. Everything between the load and the one rounding of the
 // store is fp32.
 //
-// 16381 tokens of 32 query and 8 kv heads of 128, bf16, three axes: 79 us, 5.2 TB/s, 0.80
+// 16381 tokens of 32 query and 8 kv heads of 128, bf16, three axes: 79 to 83 us, 5.1 TB/s, 0.78
 // of a plain copy (units of two rows 85 us, of eight 80 with three CTAs per SM; four CTAs
 // are 64 registers a thread, three hide less latency and take 87, five and six spill; the
 // next unit's rows fetched ahead 94). 16 tokens: 4.6 us, a launch and three dependent loads.
@@ -322,10 +322,12 @@ __global__ void __launch_bounds__(kRopeThreads, kRopeCtas) gqa_rope_kernel(const
   ln.mask = (Cfg::kLanes == 16 ? 0xffffu : 0xffu) << (lane & ~(Cfg::kLanes - 1));
   const unsigned grp = threadIdx.x / Cfg::kLanes;
   if (blockIdx.x < (unsigned)p.q_ctas)
-    rope_units<D, BF16, FP8, INTER, true>(p, ln, blockIdx.x * Cfg::kGroups + grp, p.q_ctas * Cfg::kGroups, (p.hq + kRopeRows - 1) / kRopeRows);
+    rope_units<D, BF16, FP8, INTER, true>(p, ln, blockIdx.x * Cfg::kGroups + grp, p.q_ctas * Cfg::kGroups,
+                                          (p.hq + kRopeRows - 1) / kRopeRows);
   else
     rope_units<D, BF16, FP8, INTER, false>(p, ln, (blockIdx.x - p.q_ctas) * Cfg::kGroups + grp,
-                                           (gridDim.x - p.q_ctas) * Cfg::kGroups, (p.hkv + kRopeRows / 2 - 1) / (kRopeRows / 2));
+                                           (gridDim.x - p.q_ctas) * Cfg::kGroups,
+                                           (p.hkv + kRopeRows / 2 - 1) / (kRopeRows / 2));
 }
 
 }  // namespace gqa
