@@ -10,6 +10,7 @@ namespace {
 // The ticket counters of these entry points have a fixed place at the workspace's start,
 // so calls of any kind and shape share one workspace without zeroing it in between.
 constexpr int kServingCounters = 16384;
+static_assert(kServingCounters * 4 == GQA_SERVING_COUNTER_BYTES, "the part of a workspace that callers zero");
 
 template <int HD, bool BF, bool F8>
 cudaError_t launch_ragged_stream(const RaggedParams& p, unsigned grid, const CUtensorMap& km, const CUtensorMap& vm,

@@ -16,8 +16,10 @@
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <cuda_runtime_api.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <atomic>
 #include <cmath>
 #include <climits>
 #include <map>
@@ -149,15 +151,47 @@ at::Tensor empty(at::IntArrayRef sizes, at::ScalarType dtype, int device) {
 
 // ----------------------------------------------------------------------------- workspaces
 // One per (device, stream); its counters have the same place for every call, so nothing is
-// zeroed after its allocation, and it only grows. Every workspace ever handed out is kept: a
-// captured graph may still use it.
+// zeroed after its allocation, and it only grows. Every one ever handed out is kept: a call
+// that took it may still be queued.
+//
+// A stream that is being captured has another one for as long as that capture lasts: its
+// counters are zeroed by the graph, before its first call, so that every replay starts from
+// zero whatever ran before it (other graphs of the same stream, or a replay that an expired
+// wait ended). It lives as long as the graph, and replays of different graphs may overlap.
 struct Workspace {
   void* ptr = nullptr;
   size_t bytes = 0;
 };
+struct CapturedWorkspace {
+  unsigned long long capture = 0;  // ids are not reused
+  Workspace ws;
+};
 std::map<std::pair<int, void*>, Workspace> g_workspaces;
+std::map<std::pair<int, void*>, CapturedWorkspace> g_captured;
 std::vector<at::Tensor>* g_buffers = nullptr;  // never freed: the interpreter may be gone before it
 std::mutex g_mutex;
+
+// Buffers whose graphs are gone. The runtime says so on a thread of its own, from which
+// no CUDA call may be made: a later call frees them.
+std::vector<at::Tensor*>* g_gone = nullptr;
+std::atomic<bool> g_any_gone{false};
+std::mutex g_gone_mutex;
+
+void CUDART_CB graph_gone(void* buffer) {
+  std::lock_guard<std::mutex> lock(g_gone_mutex);
+  if (!g_gone) g_gone = new std::vector<at::Tensor*>();
+  g_gone->push_back(static_cast<at::Tensor*>(buffer));
+  g_any_gone.store(true);
+}
+void free_gone() {
+  std::vector<at::Tensor*> gone;
+  {
+    std::lock_guard<std::mutex> lock(g_gone_mutex);
+    if (g_gone) gone.swap(*g_gone);
+    g_any_gone.store(false);
+  }
+  for (at::Tensor* t : gone) delete t;
+}
 
 Workspace grow_workspace(int device, void* stream, size_t need) {
   std::lock_guard<std::mutex> lock(g_mutex);
@@ -172,6 +206,30 @@ Workspace grow_workspace(int device, void* stream, size_t need) {
   }
   return ws;
 }
+
+void check_cuda(cudaError_t e, const char* what) {
+  if (e == cudaSuccess) return;
+  PyErr_Format(PyExc_RuntimeError, "%s failed: %s", what, cudaGetErrorString(e));
+  throw PyError{};
+}
+
+// A workspace of at least `need` bytes for calls that are captured on `stream` into `graph`.
+Workspace captured_workspace(int device, void* stream, unsigned long long capture, cudaGraph_t graph, size_t need) {
+  std::lock_guard<std::mutex> lock(g_mutex);
+  CapturedWorkspace& c = g_captured[{device, stream}];
+  if (c.capture == capture && c.ws.bytes >= need) return c.ws;
+  need = std::max<size_t>(need, GQA_SERVING_COUNTER_BYTES);
+  auto* buf = new at::Tensor(empty({(int64_t)need}, at::kByte, device));
+  cudaUserObject_t owner = nullptr;
+  const cudaError_t e = cudaUserObjectCreate(&owner, buf, graph_gone, 1, cudaUserObjectNoDestructorSync);
+  if (e != cudaSuccess) delete buf;
+  check_cuda(e, "cudaUserObjectCreate");
+  check_cuda(cudaGraphRetainUserObject(graph, owner, 1, cudaGraphUserObjectMove), "cudaGraphRetainUserObject");
+  check_cuda(cudaMemsetAsync(buf->data_ptr(), 0, GQA_SERVING_COUNTER_BYTES, static_cast<cudaStream_t>(stream)), "cudaMemsetAsync");
+  c = CapturedWorkspace{capture, Workspace{buf->data_ptr(), need}};
+  return c.ws;
+}
+
 void drop_workspaces(int device) {
   std::lock_guard<std::mutex> lock(g_mutex);
   for (auto it = g_workspaces.begin(); it != g_workspaces.end();)
@@ -188,6 +246,17 @@ void on_device(int device, const char* what, F f) {
 template <typename A, typename F, typename N>
 void with_workspace(int device, const char* what, A& args, F f, N need) {
   on_device(device, what, [&](cudaStream_t st) {
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    unsigned long long capture = 0;
+    cudaGraph_t graph = nullptr;
+    check_cuda(cudaStreamGetCaptureInfo(st, &status, &capture, &graph), "cudaStreamGetCaptureInfo");
+    if (status == cudaStreamCaptureStatusActive) {
+      const Workspace ws = captured_workspace(device, st, capture, graph, need(&args));
+      args.workspace = ws.ptr;
+      args.workspace_bytes = ws.bytes;
+      return f(&args, st);
+    }
+    if (g_any_gone.load(std::memory_order_relaxed)) free_gone();
     Workspace ws;
     {
       std::lock_guard<std::mutex> lock(g_mutex);

@@ -408,10 +408,14 @@ int gqa_qk_norm_rope(const gqa_qk_norm_rope_args* args, void* stream);
  * e4m3 caches (cache_fp8, scales as gqa_paged_fwd_kv8) need head_dim 128. max_query_len
  * and max_seq_len bound the lengths and must hold; longer sequences are clipped.
  * Workspace: gqa_ragged_fwd_workspace_bytes of the same arguments (workspace and
- * pointers are not looked at), zeroed before its first use; every call leaves its
- * counters zero, whatever its shape, so calls of all shapes on one stream share one
- * workspace. Too little gives GQA_ERR_WORKSPACE; NULL leaves the key axis unsplit.
+ * pointers are not looked at), its first GQA_SERVING_COUNTER_BYTES zeroed before its
+ * first use; every call leaves these counters zero, whatever its shape, so calls of all
+ * shapes on one stream share one workspace. After a device error they are to be zeroed
+ * again. A captured graph should have one of its own that it zeroes itself: one that other
+ * graphs or streams use at the same time gives wrong results. Too little gives
+ * GQA_ERR_WORKSPACE; NULL leaves the key axis unsplit.
  */
+#define GQA_SERVING_COUNTER_BYTES 65536
 typedef struct {
   void* workspace;
   size_t workspace_bytes;
