@@ -78,10 +78,12 @@ class Server:
         # what followed a token; one column more for what is not to be remembered
         self.successor = torch.zeros(n, model.vocab + 1, dtype=torch.int32, device=dev)
         self.max_len = max_blocks * block_size
+        self.counts = None  # of the last decode()
 
     def step(self, ids, query_lens, max_query_len, drafts, temperature, generator):
         """One step: ids the packed new tokens, query_lens (n,) how many each request has, drafts
-        (n, k) the drafted ones among them. Returns (tokens (n, k + 1), num_tokens (n,))."""
+        (n, k) the drafted ones among them. Returns (tokens (n, k + 1), num_tokens (n,)): -1 and 0
+        for a request that the pool refused."""
         plan = plan_step(query_lens, self.context_lens, self.block_tables, self.blocks_held, self.free_blocks, self.free_count,
                          self.block_size, ids.shape[0])
         logits = self.model.forward(ids, self.caches, plan, self.block_tables, max_query_len, self.max_len)
@@ -97,8 +99,11 @@ class Server:
             uniforms = torch.rand(self.n, k, generator=generator, device=ids.device)
             exponentials = torch.empty(self.n, probs.shape[1], device=ids.device).exponential_(generator=generator)
             tokens, num = verify_drafts(drafts, probs, None, uniforms, exponentials, cu)
-        # What is cached and stands: everything but the refused drafts. Requests that the pool
-        # refused keep their length (their tokens have no slots).
+        # The tokens of a request that the pool refused have no slots: their keys were not cached,
+        # and what was computed from their rows means nothing.
+        tokens = torch.where(plan.granted[:, None], tokens, -1)
+        num = torch.where(plan.granted, num, 0)
+        # What is cached and stands: everything but the refused drafts.
         stands = query_lens - (k + 1) + num
         self.context_lens = torch.where(plan.granted, self.context_lens + stands, self.context_lens)
         self.blocks_held, self.free_count = plan.blocks_held, plan.free_count
@@ -107,6 +112,9 @@ class Server:
     def prefill(self, prompts, temperature=0, generator=None):
         """All prompts in one ragged step; returns each request's first own token."""
         lens = [len(p) for p in prompts]
+        blocks = [-(-x // self.block_size) for x in lens]
+        if sum(blocks) > self.free_blocks.numel() or max(blocks) > self.block_tables.shape[1]:
+            raise ValueError("the pool or a row of the block tables is too small for the prompts")
         ids = torch.tensor([t for p in prompts for t in p], device="cuda")
         for b, p in enumerate(prompts):
             if len(p) > 1:
@@ -118,8 +126,10 @@ class Server:
 
     def decode(self, last, steps, num_drafts, temperature=0, generator=None):
         """`steps` steps from the requests' last tokens; returns the emitted tokens (n, steps, k + 1),
-        -1 where a draft was refused, without waiting for the device."""
-        emitted = []
+        -1 where a draft was refused, without waiting for the device. `counts` (n, steps) holds how
+        many of each step's are new: 0 for a request that the pool refused, which stays where
+        it is and whose first entry is the token that it goes on from, again."""
+        emitted, counts = [], []
         rows = torch.arange(self.n, device="cuda")
         lens = torch.full((self.n,), num_drafts + 1, dtype=torch.int32, device="cuda")
         for _ in range(steps):
@@ -128,11 +138,14 @@ class Server:
                 chain.append(self.successor[rows, chain[-1].long()])
             ids = torch.stack(chain, 1)  # (n, k + 1): the last token and its drafts
             tokens, num = self.step(ids.flatten().long(), lens, num_drafts + 1, ids[:, 1:].int().contiguous(), temperature, generator)
-            emitted.append(tokens)
             # remember what followed what: the accepted tokens, each after the one before it
             before = torch.cat([last[:, None], tokens[:, :-1]], 1)
             self.successor[rows[:, None], torch.where(tokens >= 0, before, self.model.vocab).long()] = tokens
-            last = tokens.gather(1, (num - 1)[:, None].long())[:, 0]
+            tokens[:, 0] = torch.where(num > 0, tokens[:, 0], last)
+            last = tokens.gather(1, (num - 1).clamp(min=0)[:, None].long())[:, 0]
+            emitted.append(tokens)
+            counts.append(num)
+        self.counts = torch.stack(counts, 1)
         return torch.stack(emitted, 1)
 
 
@@ -157,10 +170,10 @@ def main():
     last = server.prefill(prompts, a.temperature, g)
     torch.cuda.synchronize()
     t0 = time.perf_counter()
-    out = server.decode(last, a.steps, a.drafts, a.temperature, g)
+    server.decode(last, a.steps, a.drafts, a.temperature, g)
     torch.cuda.synchronize()
     seconds = time.perf_counter() - t0
-    kept = int((out >= 0).sum())
+    kept = int(server.counts.sum())
     print(f"{a.requests} requests, {a.steps} steps of 1 + {a.drafts} tokens: {kept} tokens, {kept / (a.requests * a.steps):.2f} per "
           f"request and step, {kept / seconds:.0f} tokens/s; device error word {check_device_error()}")
 

@@ -98,7 +98,8 @@ class RaggedPagedAttention:
         """qkv (num_tokens, (num_heads + 2 num_kv_heads) * head_dim), the fused projection of the
         packed tokens; plan a StepPlan of at least num_tokens. positions defaults to the
         plan's (pass (axes, num_tokens) for several axes). Returns (num_tokens, num_heads *
-        head_dim); rows of padding tokens are undefined."""
+        head_dim); rows of padding tokens are undefined, and those of a request that the plan
+        did not grant (its keys are not cached) mean nothing and have to be left unused."""
         t = qkv.shape[0]
         x = qkv.view(t, self.num_heads + 2 * self.num_kv_heads, self.head_dim)
         q = x[:, :self.num_heads]

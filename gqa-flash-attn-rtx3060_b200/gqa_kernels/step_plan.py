@@ -30,7 +30,9 @@ class StepPlan:
     slot_mapping: int64 (max_tokens,), its cache slot; -1 past the step's tokens and for
         requests that were not granted.
     token_seqs: int32 (max_tokens,), its request; -1 past the step's.
-    granted: bool (n,), whether the pool and the table had room for the request.
+    granted: bool (n,), whether the pool and the table had room for the request. The tokens of
+        one that was not are still packed, so that the offsets fit the step's rows, but what
+        later operators make of them is not to be used.
     blocks_held: int32 (n,), entries in use of each table row after the step.
     free_count: int32 (1,), free blocks left after the step.
     """
