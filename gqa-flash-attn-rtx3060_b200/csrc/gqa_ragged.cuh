@@ -124,8 +124,8 @@ __device__ __forceinline__ bool ragged_work_at(const RaggedParams& p, const Ragg
                                                RaggedWork& w) {
   w.b = b;
   w.m0 = m0;
-  const int first = p.cu[b];
-  const int qn = min(p.cu[b + 1], p.num_tokens) - first;
+  const int first = p.cu[b], end = p.cu[b + 1];
+  const int qn = min(end, p.num_tokens) - first;  // the rows that there are
   if (first < 0 || m0 < 0 || m0 >= qn) return false;
   const int64_t qrows = (int64_t)qn * p.group;
   if (qrows < tl.min_rows || qrows > tl.max_rows) return false;
@@ -133,7 +133,9 @@ __device__ __forceinline__ bool ragged_work_at(const RaggedParams& p, const Ragg
   w.nq = min(tl.block_m, qn - w.m0);
   (void)GQA_CHECK(p.seq_lens[w.b] <= p.max_len, 906);
   w.len = max(0, min(p.seq_lens[w.b], p.max_len));
-  w.off = w.len - qn;
+  // Positions go by the request's own numbers: a step cut to fewer rows, or keys past the
+  // bound, leave the other tokens where they are.
+  w.off = max(0, p.seq_lens[w.b]) - (end - first);
   const int p_first = w.off + w.m0, p_last = p_first + w.nq - 1;
   w.k_hi = w.len;
   if (p.causal) {

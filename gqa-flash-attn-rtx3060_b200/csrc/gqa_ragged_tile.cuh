@@ -185,16 +185,17 @@ __global__ void __launch_bounds__(384, 1)
   // (total - 1 - tile_id). Everything about a request is loaded at once, so that the thread
   // that finds the tile can describe it without another round trip.
   struct Request {
-    int first, qn, len, prefix, tiles;
+    int first, qn, len, off, prefix, tiles;  // off: position of the request's token 0 (see ragged_work_at)
   };
   auto load = [&](int b) -> Request {
-    Request r{0, 0, 0, 0, 0};
+    Request r{0, 0, 0, 0, 0, 0};
     if (b < p.n) {
       r.first = p.cu[b];
       r.qn = p.cu[b + 1];
       r.len = p.seq_lens[b];
       if (p.prefix) r.prefix = p.prefix[b];
       (void)GQA_CHECK(r.len <= p.max_len, 906);
+      r.off = max(0, r.len) - (r.qn - r.first);
       r.len = max(0, min(r.len, p.max_len));
       r.qn = min(r.qn, p.num_tokens) - r.first;
       if (r.first >= 0 && r.qn > 0 && (int64_t)r.qn * p.group >= tl.min_rows) r.tiles = (r.qn + tl.block_m - 1) / tl.block_m;
@@ -251,7 +252,7 @@ __global__ void __launch_bounds__(384, 1)
       at += incl - q.tiles;
       if (want >= at && want < at + q.tiles) {
         const int m0 = (want - at) * tl.block_m, nq = min(tl.block_m, q.qn - m0);
-        const int p_first = q.len - q.qn + m0;
+        const int p_first = q.off + m0;
         int k_hi = q.len;
         if (p.causal) k_hi = max(0, min(k_hi, max(p_first + nq, q.prefix)));
         work->b = r * 384 + tid;
