@@ -609,7 +609,16 @@ __global__ void __launch_bounds__(384, 1)
         if constexpr (kMagnitude) return max3_abs(m, __uint_as_float(a), __uint_as_float(b));
         else return max3(m, __uint_as_float(a), __uint_as_float(b));
       };
+      float big = 0.f, big1 = 0.f;  // f16 with a cap: the largest magnitude, hidden scores' included
+      auto magnitude = [&](int c0) {
+#pragma unroll
+        for (int c = c0; c < c0 + 64; c += 4) {
+          big = max3_abs(big, __uint_as_float(sr[c]), __uint_as_float(sr[c + 1]));
+          big1 = max3_abs(big1, __uint_as_float(sr[c + 2]), __uint_as_float(sr[c + 3]));
+        }
+      };
       auto mask = [&](int c0) {
+        if (MOD == kRaggedCap && !kMagnitude && (cut_hi || cut_lo)) magnitude(c0);  // of other tiles later
         if (cut_hi) {
 #pragma unroll
           for (int c = c0; c < c0 + 64; ++c) sr[c] = (c < rem) ? sr[c] : __float_as_uint(-INFINITY);
@@ -659,8 +668,10 @@ __global__ void __launch_bounds__(384, 1)
         }
       }
       if constexpr (MOD == kRaggedPlain) mx *= p.scale_log2;
+      // A visible score may be -inf itself, and its cap is -cap: in the cap's MUFU form the
+      // column says what is hidden, not the value.
       if (MOD == kRaggedCap && !small)
-        mx = mx == -INFINITY ? mx : fmaf(-2.f * p.cap_out, fast_rcp(1.f + fast_exp2(mx * p.cap_in)), p.cap_out);
+        mx = max(low, 0) >= min(rem, BN) ? -INFINITY : fmaf(-2.f * p.cap_out, fast_rcp(1.f + fast_exp2(mx * p.cap_in)), p.cap_out);
       const float m_new = fmaxf(m_run, mx);
       const bool need = !idle && m_new > m_run + 8.0f;
       if (n > 0 && __any_sync(0xffffffffu, need)) {
@@ -685,14 +696,14 @@ __global__ void __launch_bounds__(384, 1)
       const float sc = MOD == kRaggedPlain ? p.scale_log2 : 1.0f;
       float2 sum2[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
       constexpr int kPairs = 64 / Cfg::kPParts;
-      auto publish = [&](auto shifted) {  // shifted(pair) = x - m of two neighbouring scores
+      auto publish = [&](auto shifted) {  // shifted(column, pair) = x - m of two neighbouring scores
 #pragma unroll
         for (int h = 0; h < Cfg::kPParts; ++h) {
           uint32_t pk[kPairs];
 #pragma unroll
           for (int c = 0; c < kPairs; ++c) {
             const int col = 2 * kPairs * h + 2 * c;
-            const float2 x = shifted(make_float2(__uint_as_float(sr[col]), __uint_as_float(sr[col + 1])));
+            const float2 x = shifted(col, make_float2(__uint_as_float(sr[col]), __uint_as_float(sr[col + 1])));
             const float2 pv = make_float2(fast_exp2(x.x), fast_exp2(x.y));
             sum2[c & 3] = add2(sum2[c & 3], pv);
             pk[c] = pack2<BF16>(pv.x, pv.y);
@@ -706,26 +717,13 @@ __global__ void __launch_bounds__(384, 1)
       static_assert(kPairs == 32, "one 32-column store per part");
       const float2 nm2 = make_float2(-m_run, -m_run);
       if constexpr (MOD == kRaggedCap) {
-        // The polynomial if every visible score of the warp's rows is small enough.
+        // The polynomial if every score of the warp's rows is small enough.
         const bool cut = cut_hi || cut_lo;
         if constexpr (!kMagnitude) {
-        float big = 0.f, big1 = 0.f;
-        if (!cut) {
-#pragma unroll
-          for (int c = 0; c < 128; c += 4) {
-            big = max3_abs(big, __uint_as_float(sr[c]), __uint_as_float(sr[c + 1]));
-            big1 = max3_abs(big1, __uint_as_float(sr[c + 2]), __uint_as_float(sr[c + 3]));
+          if (!cut) {
+            magnitude(0);
+            magnitude(64);
           }
-        } else {
-          float b2[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int c = 0; c < 128; ++c) {
-            const float s = __uint_as_float(sr[c]);
-            b2[c & 3] = fmaxf(b2[c & 3], s == -INFINITY ? 0.f : fabsf(s));
-          }
-          big = fmaxf(b2[0], b2[1]);
-          big1 = fmaxf(b2[2], b2[3]);
-        }
           small = __all_sync(0xffffffffu, idle || fmaxf(big, big1) <= p.cap_most);
         }
         if (small) {
@@ -736,23 +734,23 @@ __global__ void __launch_bounds__(384, 1)
             return fma2(s, fma2(fma2(fma2(a3, z, a2), z, a1), z, a0), nm2);
           };
           if (!cut) {
-            publish(capped);
+            publish([&](int, float2 s) { return capped(s); });
           } else {
-            publish([&](float2 s) {
+            publish([&](int, float2 s) {
               const float2 x = capped(s);
               return make_float2(s.x == -INFINITY ? s.x : x.x, s.y == -INFINITY ? s.y : x.y);
             });
           }
         } else {
-        const float cin = p.cap_in, cout2 = -2.f * p.cap_out, off = p.cap_out - m_run;
-        publish([&](float2 s) {
-          return make_float2(s.x == -INFINITY ? s.x : fmaf(cout2, fast_rcp(1.f + fast_exp2(s.x * cin)), off),
-                             s.y == -INFINITY ? s.y : fmaf(cout2, fast_rcp(1.f + fast_exp2(s.y * cin)), off));
-        });
+          const float cin = p.cap_in, cout2 = -2.f * p.cap_out, off = p.cap_out - m_run;
+          publish([&](int c, float2 s) {
+            return make_float2(c < rem && c >= low ? fmaf(cout2, fast_rcp(1.f + fast_exp2(s.x * cin)), off) : -INFINITY,
+                               c + 1 < rem && c + 1 >= low ? fmaf(cout2, fast_rcp(1.f + fast_exp2(s.y * cin)), off) : -INFINITY);
+          });
         }
       } else {
         const float2 sc2 = make_float2(sc, sc);
-        publish([&](float2 s) { return fma2(s, sc2, nm2); });
+        publish([&](int, float2 s) { return fma2(s, sc2, nm2); });
       }
       const float2 s01 = add2(sum2[0], sum2[1]);
       const float2 s23 = add2(sum2[2], sum2[3]);
