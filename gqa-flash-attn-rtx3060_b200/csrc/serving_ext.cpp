@@ -124,22 +124,27 @@ int device_of(std::initializer_list<const at::Tensor*> ts) {
 }
 
 // Rows that the kernels read in 16-byte pieces: d stride 1, the others multiples of
-// `multiple`, base 16-byte aligned; other layouts are copied once.
+// `multiple`, base 16-byte aligned; other layouts are copied once. (contiguous() would not
+// copy a tensor that is contiguous on another base.) A dimension of size 1 may have any
+// stride, since no element lies a stride away.
 bool rows_ok(const at::Tensor& t, int64_t multiple) {
   const int64_t n = t.dim();
   if (t.stride(n - 1) != 1 && t.size(n - 1) != 1) return false;
   if (reinterpret_cast<uintptr_t>(t.const_data_ptr()) & 15) return false;
   for (int64_t i = 0; i + 1 < n; ++i)
-    if (t.stride(i) % multiple != 0 || t.stride(i) < 0) return false;
+    if (t.size(i) != 1 && (t.stride(i) % multiple != 0 || t.stride(i) < 0)) return false;
   return true;
 }
-at::Tensor rows(const at::Tensor& t) { return rows_ok(t, 8) ? t : t.contiguous(); }
+at::Tensor rows(const at::Tensor& t) { return rows_ok(t, 8) ? t : t.clone(at::MemoryFormat::Contiguous); }
 at::Tensor flat(const at::Tensor& t) { return !t.defined() || t.is_contiguous() ? t : t.contiguous(); }
 bool last_dim_ok(const at::Tensor& t) { return t.stride(-1) == 1 || t.size(-1) <= 1; }
-void strides3(const at::Tensor& t, int64_t* out) {
-  out[0] = t.stride(0);
-  out[1] = t.stride(1);
-  out[2] = 1;
+// The strides that the library gets, a dimension of size 1 as if it were contiguous.
+void strides_of(const at::Tensor& t, int64_t* out) {
+  int64_t next = 1;
+  for (int64_t i = t.dim() - 1; i >= 0; --i) {
+    out[i] = t.size(i) == 1 ? next : t.stride(i);
+    next = out[i] * t.size(i);
+  }
 }
 template <typename T>
 T* data(const at::Tensor& t) {
@@ -431,9 +436,9 @@ PyObject* norm_rope(PyObject* const* a) {
   g.k_dst = k_out.data_ptr();
   g.v_dst = data<void>(vc);
   g.slot_mapping = data<int64_t>(slots);
-  strides3(q, g.q_strides);
-  strides3(k, g.k_strides);
-  if (cached) strides3(v, g.v_strides);
+  strides_of(q, g.q_strides);
+  strides_of(k, g.k_strides);
+  if (cached) strides_of(v, g.v_strides);
   g.pos_stride = axes > 1 ? pos.stride(0) : 0;
   g.axes = (int)axes;
   g.max_positions = dim32(table, 0);
@@ -517,12 +522,10 @@ PyObject* ragged(PyObject* const* a) {
   g.alibi_slopes = data<float>(alibi);
   g.prefix_lens = data<int>(prefix);
   g.key_starts = data<int>(starts);
-  strides3(q, g.q_strides);
-  for (int i = 0; i < 4; ++i) {
-    g.k_strides[i] = kc.stride(i);
-    g.v_strides[i] = vc.stride(i);
-  }
-  for (int i = 0; i < 3; ++i) g.o_strides[i] = out.stride(i);
+  strides_of(q, g.q_strides);
+  strides_of(kc, g.k_strides);
+  strides_of(vc, g.v_strides);
+  strides_of(out, g.o_strides);
   g.bt_stride = dim32(bt, 1);
   g.num_seqs = dim32(lens, 0);
   g.num_tokens = dim32(q, 0);
