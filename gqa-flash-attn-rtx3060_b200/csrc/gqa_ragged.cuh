@@ -131,11 +131,15 @@ __device__ __forceinline__ bool ragged_work_at(const RaggedParams& p, const Ragg
   if (qrows < tl.min_rows || qrows > tl.max_rows) return false;
   w.t0 = first + w.m0;
   w.nq = min(tl.block_m, qn - w.m0);
-  (void)GQA_CHECK(p.seq_lens[w.b] <= p.max_len, 906);
-  w.len = max(0, min(p.seq_lens[w.b], p.max_len));
+  const int len = max(0, p.seq_lens[w.b]);
+  if (lane == 0) {  // bounds that do not hold
+    if (tl.one_tile && qn > tl.block_m) report_device_error(GQA_ERR_INVALID_ARG, 214);  // rows past the tile stay unwritten
+    if (len > p.max_len) report_device_error(GQA_ERR_INVALID_ARG, 215);
+  }
+  w.len = min(len, p.max_len);
   // Positions go by the request's own numbers: a step cut to fewer rows, or keys past the
   // bound, leave the other tokens where they are.
-  w.off = max(0, p.seq_lens[w.b]) - (end - first);
+  w.off = len - (end - first);
   const int p_first = w.off + w.m0, p_last = p_first + w.nq - 1;
   w.k_hi = w.len;
   if (p.causal) {

@@ -194,9 +194,9 @@ __global__ void __launch_bounds__(384, 1)
       r.qn = p.cu[b + 1];
       r.len = p.seq_lens[b];
       if (p.prefix) r.prefix = p.prefix[b];
-      (void)GQA_CHECK(r.len <= p.max_len, 906);
-      r.off = max(0, r.len) - (r.qn - r.first);
-      r.len = max(0, min(r.len, p.max_len));
+      r.len = max(0, r.len);
+      r.off = r.len - (r.qn - r.first);
+      r.len = min(r.len, p.max_len);
       r.qn = min(r.qn, p.num_tokens) - r.first;
       if (r.first >= 0 && r.qn > 0 && (int64_t)r.qn * p.group >= tl.min_rows) r.tiles = (r.qn + tl.block_m - 1) / tl.block_m;
     }
@@ -260,6 +260,7 @@ __global__ void __launch_bounds__(384, 1)
         work->nq = nq;
         work->off_m0 = p_first;
         work->len = q.len;
+        if (p.seq_lens[r * 384 + tid] > p.max_len) report_device_error(GQA_ERR_INVALID_ARG, 215);
         work->unit = (int)(blockIdx.x / (unsigned)tl.nsplit);
         set_keys(p.window > 0 ? max(0, p_first - p.window + 1) : 0, k_hi);
       }

@@ -37,8 +37,10 @@ def paged_ragged_attention(query, key_cache, value_cache, block_tables, cu_query
         seq_lens: int32 (num_seqs,), cached keys of each request, its new tokens' included:
             token i of q new ones is at position seq_lens[b] - q + i.
         max_query_len, max_seq_len: upper bounds of the query lengths and of seq_lens, which
-            size the launch; they must hold (keys past max_seq_len are not seen). Defaults:
-            num_tokens and the tables' capacity.
+            size the launch; they must hold. Keys past max_seq_len are not seen, and rows past
+            max_query_len may stay unwritten; both are reported through the device error
+            word (gqa_kernels.check_device_error()). Defaults: num_tokens and the tables'
+            capacity.
         scale: softmax scale; defaults to head_dim ** -0.5.
         causal: a token sees the keys up to its own position; False: all of the request's.
         softcap: scores become softcap * tanh(score / softcap); 0: not.

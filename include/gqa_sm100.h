@@ -406,7 +406,9 @@ int gqa_qk_norm_rope(const gqa_qk_norm_rope_args* args, void* stream);
  * gqa_fwd's NaN, which is the reference's rule) and lse -inf. lse (num_tokens,
  * num_heads), float32, natural log, may be NULL. Groups of up to 64 heads, any number.
  * e4m3 caches (cache_fp8, scales as gqa_paged_fwd_kv8) need head_dim 128. max_query_len
- * and max_seq_len bound the lengths and must hold; longer sequences are clipped.
+ * and max_seq_len bound the lengths and must hold: a request with more tokens may have
+ * rows unwritten (reported: GQA_ERR_INVALID_ARG, site 214), keys past max_seq_len are not
+ * seen (reported, site 215).
  * Workspace: gqa_ragged_fwd_workspace_bytes of the same arguments (workspace and
  * pointers are not looked at), its first GQA_SERVING_COUNTER_BYTES zeroed before its
  * first use; every call leaves these counters zero, whatever its shape, so calls of all

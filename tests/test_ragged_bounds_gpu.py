@@ -47,3 +47,41 @@ def test_a_step_cut_to_fewer_rows_keeps_its_positions(reqs, rows, case):
         at += qn
     out = paged_ragged_attention(q[:rows], kc, vc, bt, cu, lens, **kw)
     check_attention(out, o[:rows], a[:rows], torch.bfloat16)
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_a_request_longer_than_its_bound_is_reported(fp8):
+    """Streamed requests have as many tiles as max_query_len needs: more tokens than it says
+    are left out, and the error word says so."""
+    reqs = [(1, 50), (9, 100), (2, 7)]
+    q, kc, vc, bt, cu, lens = paged_batch(reqs, 8, 2, 128, 64, torch.bfloat16, 1)
+    if fp8:
+        kc, vc = kc.to(torch.float8_e4m3fn), vc.to(torch.float8_e4m3fn)
+    out = paged_ragged_attention(q, kc, vc, bt, cu, lens, max_query_len=9)
+    torch.cuda.synchronize()
+    assert check_device_error() == (0, 0)
+    got = torch.full_like(q, 7.0)
+    paged_ragged_attention(q, kc, vc, bt, cu, lens, max_query_len=2, out=got)
+    torch.cuda.synchronize()
+    assert check_device_error() == (GQA_ERR_INVALID_ARG, 214)
+    kept = torch.ones(12, dtype=torch.bool, device="cuda")
+    kept[3:10] = False
+    assert ((got.float() - out.float())[kept].abs() <= 0.02 * out.float().abs().max()).all() and (got[~kept] == 7.0).all()
+
+
+@pytest.mark.parametrize("reqs", [[(1, 700), (2, 90)], [(200, 500), (2, 90)]])  # streamed, tcgen05
+def test_a_length_past_its_bound_is_reported(reqs):
+    """Keys past max_seq_len are not seen; tokens keep their positions."""
+    q, kc, vc, bt, cu, lens = paged_batch(reqs, 8, 2, 128, 16, torch.bfloat16, 2)
+    bound = 600
+    out = paged_ragged_attention(q, kc, vc, bt, cu, lens, max_seq_len=bound, alibi_slopes=slopes(8))
+    torch.cuda.synchronize()
+    assert check_device_error() == (GQA_ERR_INVALID_ARG, 215)
+    first, n = 0, sum(reqs[0])
+    assert n > bound
+    k, v = (x[bt[0].long()].flatten(0, 1)[:bound].double().repeat_interleave(4, 1) for x in (kc, vc))
+    pos = torch.arange(reqs[0][1], n, device="cuda")[:, None]
+    key = torch.arange(bound, device="cuda")
+    x = torch.einsum("qhd,khd->hqk", q[:reqs[0][0]].double(), k) * 128 ** -0.5 - slopes(8).double()[:, None, None] * (pos - key).abs()
+    p = x.masked_fill(key > pos, float("-inf")).softmax(-1)
+    check_attention(out[:reqs[0][0]], torch.einsum("hqk,khd->qhd", p, v), torch.einsum("hqk,khd->qhd", p, v.abs()), torch.bfloat16)
