@@ -14,13 +14,17 @@
 // request's tokens get slot -1 (paged writes skip it) and its length stays ctx_b.
 //
 // Integer work bound by latency: a few dependent loads and one scan. Every CTA scans the
-// requests itself (1024 at a time, q in the low and need in the high half of one 64-bit
-// sum), which costs less than a second launch or a grid-wide wait, and writes the
+// requests itself (1024 at a time), which costs less than a second launch or a grid-wide
+// wait, and writes the
 // tokens, table entries and per-request results of its own share. A new table entry is
 // computed from the free stack rather than read back from the table, so no CTA depends
-// on another's stores. 8 requests of one token: 3.4 us; 1024 requests with 65536 new
+// on another's stores. Lengths come from the device unchecked, so both sums stay at
+// 2^31 - 1 where they would pass it (which sums of any order agree on) and cannot come round
+// to one that the step or the pool could serve. 8 requests of one token: 3.4 us; 1024 requests with 65536 new
 // tokens: 5.4 us, one scan longer.
 #pragma once
+
+#include <climits>
 
 #include "gqa_common.cuh"
 
@@ -45,6 +49,21 @@ struct StepPlanParams {
   int n, max_blocks, num_free, block_shift, max_tokens;
 };
 
+// Sum of two values up to 2^31 - 1, and no more than that.
+__device__ __forceinline__ unsigned sum_to_limit(unsigned a, unsigned b) { return min(a + b, (unsigned)INT_MAX); }
+
+// Inclusive sums of both over a warp.
+__device__ __forceinline__ void scan_to_limit(unsigned& a, unsigned& b, int lane) {
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const unsigned y = __shfl_up_sync(0xffffffffu, a, d), z = __shfl_up_sync(0xffffffffu, b, d);
+    if (lane >= d) {
+      a = sum_to_limit(a, y);
+      b = sum_to_limit(b, z);
+    }
+  }
+}
+
 __global__ void __launch_bounds__(1024) gqa_step_plan_kernel(const StepPlanParams p) {
   constexpr int kChunk = 1024;  // requests scanned at a time
   __shared__ int s_cu[kChunk + 1];  // first token of each request of the chunk
@@ -52,18 +71,17 @@ __global__ void __launch_bounds__(1024) gqa_step_plan_kernel(const StepPlanParam
   __shared__ int s_held[kChunk];
   __shared__ int s_off[kChunk];   // blocks taken by earlier requests
   __shared__ int s_need[kChunk];  // new blocks, -1: refused
-  __shared__ unsigned long long s_warp[32];
+  __shared__ uint2 s_warp[32];  // sums of q and need
   pdl_wait();
   pdl_trigger();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int nthreads = blockDim.x, nwarps = nthreads >> 5;
   const int block = 1 << p.block_shift;
-  const int free_count = max(0, min(*p.free_count, p.num_free));
-  unsigned long long carry = 0;  // sums over the chunks before this one
-  int taken = 0;                 // blocks taken so far (granted requests)
+  const int free_count = max(0, min(min(*p.free_count, p.num_free), INT_MAX - 1));  // below a sum at its limit
+  unsigned carry_q = 0, carry_need = 0;  // sums over the chunks before this one
+  int taken = 0;                         // blocks taken so far (granted requests)
   for (int c0 = 0; c0 < p.n || c0 == 0; c0 += kChunk) {
     const int cn = min(kChunk, p.n - c0);
-    unsigned long long run = carry;
     int chunk_taken = 0;
     for (int i0 = 0; i0 < cn; i0 += nthreads) {  // one pass when the block has a thread per request
       const int i = i0 + tid, b = c0 + i;
@@ -74,53 +92,50 @@ __global__ void __launch_bounds__(1024) gqa_step_plan_kernel(const StepPlanParam
         ctx = max(0, p.context_lens[b]);
         held = min(max(0, p.blocks_held[b]), p.max_blocks);
         const int64_t after = ((int64_t)ctx + q + block - 1) >> p.block_shift;
-        fits = after <= p.max_blocks;
+        fits = after <= p.max_blocks && (int64_t)ctx + q <= INT_MAX;
         need = fits ? max(0, (int)after - held) : 0;
       }
-      unsigned long long x = ((unsigned long long)(unsigned)need << 32) | (unsigned)q;
-      unsigned long long incl = x;
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const unsigned long long y = __shfl_up_sync(0xffffffffu, incl, d);
-        if (lane >= d) incl += y;
-      }
-      if (lane == 31) s_warp[warp] = incl;
+      unsigned first_q = q, upto = need;
+      scan_to_limit(first_q, upto, lane);
+      if (lane == 31) s_warp[warp] = make_uint2(first_q, upto);
+      first_q = __shfl_up_sync(0xffffffffu, first_q, 1);  // the requests before this one
+      if (lane == 0) first_q = 0;
       __syncthreads();
-      unsigned long long before = run, all = run;
-      for (int w = 0; w < nwarps; ++w) {
-        const unsigned long long y = s_warp[w];
-        if (w < warp) before += y;
-        all += y;
-      }
-      incl += before;
-      const int upto = (int)(incl >> 32);
-      const bool ok = fits && (need == 0 || upto <= free_count);
+      // Every warp scans the warps' sums.
+      uint2 y = lane < nwarps ? s_warp[lane] : make_uint2(0u, 0u);
+      scan_to_limit(y.x, y.y, lane);
+      const unsigned before_q = __shfl_sync(0xffffffffu, y.x, max(0, warp - 1));
+      const unsigned before_need = __shfl_sync(0xffffffffu, y.y, max(0, warp - 1));
+      first_q = sum_to_limit(first_q, sum_to_limit(carry_q, warp ? before_q : 0u));
+      upto = sum_to_limit(upto, sum_to_limit(carry_need, warp ? before_need : 0u));
+      const bool ok = fits && (need == 0 || upto <= (unsigned)free_count);
       if (i < cn) {
-        s_cu[i] = (int)(unsigned)(incl - x);
+        s_cu[i] = (int)first_q;
         s_ctx[i] = ctx;
         s_held[i] = held;
-        s_off[i] = upto - need;
+        s_off[i] = (int)upto - need;
         s_need[i] = ok ? need : -1;
-        if (ok && need > 0) chunk_taken = max(chunk_taken, upto);
+        if (ok && need > 0) chunk_taken = max(chunk_taken, (int)upto);
         if (blockIdx.x == 0) {
-          p.cu_query_lens[b] = (int)(unsigned)(incl - x);
+          p.cu_query_lens[b] = (int)first_q;
           p.seq_lens[b] = ok ? ctx + q : ctx;
           p.granted[b] = ok ? 1 : 0;
           p.blocks_held_out[b] = held + (ok ? need : 0);
         }
       }
-      run = all;
+      carry_q = sum_to_limit(carry_q, __shfl_sync(0xffffffffu, y.x, 31));
+      carry_need = sum_to_limit(carry_need, __shfl_sync(0xffffffffu, y.y, 31));
       __syncthreads();
     }
-    if (tid == 0) s_cu[max(cn, 0)] = (int)(unsigned)run;
+    if (tid == 0) s_cu[max(cn, 0)] = (int)carry_q;
     if (blockIdx.x == 0) {
       // blocks taken: the largest running sum among the granted requests that need any
       const int m = __reduce_max_sync(0xffffffffu, chunk_taken);
-      if (lane == 0) s_warp[warp] = (unsigned long long)(unsigned)m;
+      if (lane == 0) s_warp[warp].x = m;
     }
     __syncthreads();
     if (blockIdx.x == 0 && tid == 0)
-      for (int w = 0; w < nwarps; ++w) taken = max(taken, (int)s_warp[w]);
+      for (int w = 0; w < nwarps; ++w) taken = max(taken, (int)s_warp[w].x);
 
     // New table entries: a warp per request, the requests dealt over the grid.
     for (int i = blockIdx.x + gridDim.x * warp; i < cn; i += gridDim.x * nwarps) {
@@ -133,17 +148,17 @@ __global__ void __launch_bounds__(1024) gqa_step_plan_kernel(const StepPlanParam
     const int t_end = min(p.max_tokens, s_cu[max(cn, 0)]);
     const int stride = gridDim.x * nthreads;
     // this thread's first token of its grid-strided share that is not before the chunk
-    int t = blockIdx.x * nthreads + tid;
+    unsigned t = blockIdx.x * nthreads + tid;  // its last step may pass 2^31
     if (cn > 0) {
-      const int first = s_cu[0];
-      if (t < first) t += (int)(((int64_t)first - t + stride - 1) / stride) * stride;
-      for (; t < t_end; t += stride) {
+      const unsigned first = s_cu[0];
+      if (t < first) t += (first - t + stride - 1) / stride * stride;
+      for (; t < (unsigned)t_end; t += stride) {
         int lo = 0, hi = cn;  // the last request whose first token is <= t (the empty ones before it skipped)
         while (hi - lo > 1) {
           const int mid = (lo + hi) >> 1;
-          if (s_cu[mid] <= t) lo = mid; else hi = mid;
+          if ((unsigned)s_cu[mid] <= t) lo = mid; else hi = mid;
         }
-        const int pos = s_ctx[lo] + (t - s_cu[lo]);
+        const int pos = (int)(s_ctx[lo] + (t - s_cu[lo]));  // a refused request's may wrap
         int64_t slot = -1;
         if (s_need[lo] >= 0) {
           const int col = pos >> p.block_shift, held = s_held[lo];
@@ -156,18 +171,16 @@ __global__ void __launch_bounds__(1024) gqa_step_plan_kernel(const StepPlanParam
         p.token_seqs[t] = c0 + lo;
       }
     }
-    carry = run;
     __syncthreads();  // the shared arrays are free for the next chunk
   }
-  const int total = (int)(unsigned)carry;
   if (blockIdx.x == 0 && tid == 0) {
-    p.cu_query_lens[p.n] = total;
+    p.cu_query_lens[p.n] = (int)carry_q;
     *p.free_count_out = free_count - taken;
-    if (total > p.max_tokens) report_device_error(GQA_ERR_INVALID_ARG, 211);
+    if (carry_q > (unsigned)p.max_tokens) report_device_error(GQA_ERR_INVALID_ARG, 211);
   }
   // Padding tokens past the step's own.
-  for (int t = blockIdx.x * nthreads + tid; t < p.max_tokens; t += gridDim.x * nthreads) {
-    if (t < total) continue;
+  for (unsigned t = blockIdx.x * nthreads + tid; t < (unsigned)p.max_tokens; t += gridDim.x * nthreads) {
+    if (t < carry_q) continue;
     p.positions[t] = -1;
     p.slot_mapping[t] = -1;
     p.token_seqs[t] = -1;
