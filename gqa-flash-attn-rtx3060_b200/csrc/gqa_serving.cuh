@@ -65,7 +65,9 @@ int check_ragged_shape(const gqa_ragged_args& a, RaggedShape* s) {
   if (a.head_dim != 64 && a.head_dim != 128) return GQA_ERR_UNSUPPORTED;
   if (a.num_heads / a.num_kv_heads > kStreamMaxRows) return GQA_ERR_UNSUPPORTED;
   *s = RaggedShape{a.num_seqs, a.num_tokens, a.num_heads, a.num_kv_heads, a.num_heads / a.num_kv_heads,
-                   std::min(a.max_query_len, a.num_tokens), a.max_seq_len, a.head_dim, a.window, a.causal ? 1 : 0,
+                   std::min(a.max_query_len, a.num_tokens), a.max_seq_len, a.head_dim,
+                   a.window < a.max_seq_len ? a.window : 0,  // a window of all keys is none, and its arithmetic may overflow
+                   a.causal ? 1 : 0,
                    a.prefix_lens != nullptr};
   return GQA_OK;
 }
@@ -370,7 +372,7 @@ int gqa_ragged_fwd(const gqa_ragged_args* args, void* stream) {
   p.alibi = a.alibi_slopes;
   p.prefix = a.prefix_lens;
   p.key_starts = a.key_starts;
-  p.window = a.window;
+  p.window = s.window;
   p.causal = s.causal;
   p.n = a.num_seqs;
   p.num_tokens = a.num_tokens;

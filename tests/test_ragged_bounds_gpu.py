@@ -85,3 +85,16 @@ def test_a_length_past_its_bound_is_reported(reqs):
     x = torch.einsum("qhd,khd->hqk", q[:reqs[0][0]].double(), k) * 128 ** -0.5 - slopes(8).double()[:, None, None] * (pos - key).abs()
     p = x.masked_fill(key > pos, float("-inf")).softmax(-1)
     check_attention(out[:reqs[0][0]], torch.einsum("hqk,khd->qhd", p, v), torch.einsum("hqk,khd->qhd", p, v.abs()), torch.bfloat16)
+
+
+@pytest.mark.parametrize("reqs,lens", [([(6, 0), (1, 40)], [3, 41]), ([(150, 0), (2, 40)], [130, 42])])  # streamed, tcgen05
+@pytest.mark.parametrize("window", [(1 << 31) - 1, (1 << 31) - 100, 1 << 20])
+def test_a_window_of_everything(reqs, lens, window):
+    """With a window past all keys a request's mask is the causal one, also where its first
+    rows lie before position 0 (fewer cached keys than new tokens)."""
+    q, kc, vc, bt, cu, _ = paged_batch(reqs, 8, 2, 128, 16, torch.bfloat16, 3)
+    out, lse = paged_ragged_attention(q, kc, vc, bt, cu, torch.tensor(lens, dtype=torch.int32, device="cuda"), window=window,
+                                      return_lse=True)
+    o, l64, a = attention64(q, kc, vc, bt, reqs, lens=lens)
+    check_attention(out, o, a, torch.bfloat16)
+    assert torch.equal(torch.isinf(lse), torch.isinf(l64))
