@@ -53,6 +53,23 @@ int prepare_ragged() {
   return rc;
 }
 
+// current_device() for the ragged attention: its kernels are loaded and checked at its own
+// first call on the device, so that a caller of the dense entry points does not pay for them
+// and cannot be refused because of them.
+int current_device_ragged(int* sm_count) {
+  const int rc = current_device(sm_count);
+  if (rc) return rc;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return GQA_ERR_NO_DEVICE;
+  std::lock_guard<std::mutex> lock(g_mutex);
+  DeviceState& st = g_devices[dev];
+  if (!st.ragged_ready) {
+    st.ragged_status = prepare_ragged();
+    st.ragged_ready = true;
+  }
+  return st.ragged_status;
+}
+
 struct RaggedShape {
   int n, tokens, hq, hkv, group, max_q, max_len, head_dim, window, causal, prefix;
 };
@@ -354,7 +371,7 @@ int gqa_ragged_fwd(const gqa_ragged_args* args, void* stream) {
   if (!rc && (a.k_strides[3] != 1 || a.v_strides[3] != 1 || !aligned16(a.k_cache) || !aligned16(a.v_cache))) rc = GQA_ERR_ALIGNMENT;
   if (rc) return rc;
   int sm = 0;
-  rc = current_device(&sm);
+  rc = current_device_ragged(&sm);
   if (rc) return rc;
 
   RaggedParams p{};

@@ -33,6 +33,8 @@ struct DeviceState {
   bool ready = false;
   int status = GQA_OK;
   int sm_count = 0;
+  bool ragged_ready = false;  // the ragged attention's kernels (gqa_serving.cuh)
+  int ragged_status = GQA_OK;
 };
 
 // The prefill kernel rebalances registers with setmaxnreg; the increase can only
@@ -54,8 +56,6 @@ template <typename K>
 cudaError_t set_smem(K kernel, int bytes) {
   return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
 }
-
-int prepare_ragged();  // gqa_serving.cuh
 
 int init_device(int dev) {
   cudaDeviceProp prop;
@@ -114,7 +114,7 @@ int init_device(int dev) {
   chk(set_smem(gqa_stream_kernel<64, true, 1, false, true>, StreamCfg<64>::kSmemBytes));
   chk(set_smem(gqa_stream_kernel<64, false, 1, false, true>, StreamCfg<64>::kSmemBytes));
   if (e != cudaSuccess) return GQA_ERR_CUDA;
-  return prepare_ragged();
+  return GQA_OK;
 }
 
 // Returns GQA_OK and the SM count of the current device, initialising it once.
