@@ -1,5 +1,6 @@
 """Builds libgqa_sm100.so (the C-ABI library) in-tree for sm_100a, and the serving step's
-Python binding (_serving_ext.so, host code against torch's headers).
+Python binding (_serving_ext.so, host code against torch's headers). The library needs
+nvcc alone; the binding, which only Python callers use, is left out without torch or g++.
 
     python gqa-flash-attn-rtx3060_b200/build.py [--force] [--debug]
 
@@ -9,12 +10,14 @@ not link libcuda (the driver's tensor-map encoder is looked up at run time),
 so it loads on a machine without a GPU driver.
 """
 import argparse
+import contextlib
 import importlib.util
 import os
 import shutil
 import subprocess
 import sys
 import sysconfig
+import uuid
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
@@ -37,10 +40,26 @@ EXT = os.path.join(HERE, "gqa_kernels", "_serving_ext.so")
 EXT_SOURCES = [os.path.join(CSRC, "serving_ext.cpp"), os.path.join(INCLUDE, "gqa_sm100.h")]
 
 
+@contextlib.contextmanager
+def _written(out):
+    """A path of its own to write, put in `out`'s place at the end: builds may run at the same time."""
+    tmp = f"{out}.{uuid.uuid4().hex}.tmp"
+    try:
+        yield tmp
+        os.replace(tmp, out)
+    finally:
+        if os.path.exists(tmp):
+            os.remove(tmp)
+
+
 def build_ext(force=False):
     """Compiles gqa_kernels._serving_ext (g++, a few seconds) unless it is newer than its sources
-    and was built for the installed torch. Returns its path."""
-    torch_dir = list(importlib.util.find_spec("torch").submodule_search_locations)[0]
+    and was built for the installed torch. Returns its path, or None without torch or g++."""
+    torch_spec = importlib.util.find_spec("torch")
+    if torch_spec is None or shutil.which("g++") is None:
+        print(f"{os.path.basename(EXT)} is not built: {'g++' if torch_spec else 'torch'} is missing", file=sys.stderr)
+        return None
+    torch_dir = list(torch_spec.submodule_search_locations)[0]
     stamp = f"{torch_dir} {os.path.getmtime(os.path.join(torch_dir, 'version.py'))} {sys.version}\n"
     if not force and os.path.exists(EXT) and all(os.path.getmtime(x) <= os.path.getmtime(EXT) for x in EXT_SOURCES):
         with open(EXT, "rb") as f:
@@ -48,16 +67,17 @@ def build_ext(force=False):
             if f.read() == stamp.encode():
                 return EXT
     cuda = os.path.dirname(os.path.dirname(nvcc()))
-    tmp = EXT + ".tmp"
-    subprocess.run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-D_GLIBCXX_USE_CXX11_ABI=1",
-                    "-I", INCLUDE, "-I", os.path.join(torch_dir, "include"),
-                    "-I", os.path.join(torch_dir, "include", "torch", "csrc", "api", "include"),
-                    "-I", os.path.join(cuda, "include"), "-I", sysconfig.get_paths()["include"],
-                    EXT_SOURCES[0], "-o", tmp, "-L", os.path.join(torch_dir, "lib"),
-                    "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda"], check=True)
-    with open(tmp, "ab") as f:  # what it was built for, after the last byte that the loader reads
-        f.write(stamp.encode())
-    os.replace(tmp, EXT)
+    abi = subprocess.run([sys.executable, "-c", "import torch; print(int(torch.compiled_with_cxx11_abi()))"], check=True,
+                         capture_output=True, text=True).stdout.strip()
+    with _written(EXT) as tmp:
+        subprocess.run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
+                        "-I", INCLUDE, "-I", os.path.join(torch_dir, "include"),
+                        "-I", os.path.join(torch_dir, "include", "torch", "csrc", "api", "include"),
+                        "-I", os.path.join(cuda, "include"), "-I", sysconfig.get_paths()["include"],
+                        EXT_SOURCES[0], "-o", tmp, "-L", os.path.join(torch_dir, "lib"),
+                        "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda"], check=True)
+        with open(tmp, "ab") as f:  # what it was built for, after the last byte that the loader reads
+            f.write(stamp.encode())
     return EXT
 
 
@@ -86,17 +106,15 @@ def build(force=False, verbose=False, debug=False):
     """Compiles the library (or, with debug, its checked variant) and the binding unless they
     are newer than every source. Returns the library's path."""
     out = OUT_DEBUG if debug else OUT
+    if force or not up_to_date(out):
+        with _written(out) as tmp:
+            cmd = [nvcc(), *NVCC_FLAGS, *(["-DGQA_DEBUG_CHECKS"] if debug else []), "-I", INCLUDE, "-o", tmp,
+                   os.path.join(CSRC, "gqa_sm100.cu")]
+            if verbose:
+                cmd.insert(1, "-Xptxas=-v")
+                print(" ".join(cmd), flush=True)
+            subprocess.run(cmd, check=True)
     build_ext(force)
-    if not force and up_to_date(out):
-        return out
-    tmp = out + ".tmp"
-    cmd = [nvcc(), *NVCC_FLAGS, *(["-DGQA_DEBUG_CHECKS"] if debug else []), "-I", INCLUDE, "-o", tmp,
-           os.path.join(CSRC, "gqa_sm100.cu")]
-    if verbose:
-        cmd.insert(1, "-Xptxas=-v")
-        print(" ".join(cmd), flush=True)
-    subprocess.run(cmd, check=True)
-    os.replace(tmp, out)
     return out
 
 
