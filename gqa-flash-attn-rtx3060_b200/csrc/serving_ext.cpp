@@ -367,6 +367,8 @@ PyObject* norm_rope(PyObject* const* a) {
   g.k_scale = (float)number(a[14]);
   g.v_scale = (float)number(a[15]);
   const bool cached = kc.defined();
+  CHECK_VALUE(cached || (!v.defined() && !vc.defined() && !slots.defined()),
+              "the cache write needs key_cache, value_cache and slot_mapping");
   if (cached) {
     CHECK_VALUE(v.defined() && vc.defined() && slots.defined() && v.sizes() == k.sizes() && kc.dim() == 4 && vc.sizes() == kc.sizes() &&
                     kc.size(2) == hkv && kc.size(3) == d,
