@@ -6,7 +6,9 @@
 //              lo = max(0, p - window + 1, key_starts[token])
 //
 // which covers causal, prefix, window and document masks and their mixtures; a row whose
-// interval is empty gives 0 (and log-sum-exp -inf). Scores, in log2 units:
+// interval is empty gives 0 (and log-sum-exp -inf). Keys that no row of a tile sees may hold
+// anything; a NaN or infinite value of a key that some row sees may reach the tile's other
+// rows too, as 0 x NaN. Scores, in log2 units:
 //
 //   x = s * scale * log2 e                                    or, capped,
 //   x = cap * log2 e * tanh(s * scale / cap),  tanh y = 1 - 2 / (1 + 2^(2 y log2 e))
@@ -19,8 +21,9 @@
 // of one (tile, kv head)'s keys through a 192 KB TMA ring, and the last CTA of a tile
 // combines the chunks' partials. The key range of a tile is the union of its rows'
 // intervals, so keys before a window or a document are not read at all. 48 requests of
-// one token, 32 query and 8 kv heads of 128, up to 16384 bf16 keys (2.2 GB): 318 us,
-// 6.8 TB/s, the rate of a plain copy. A single short request is bound by latency: about
+// one token, 32 query and 8 kv heads of 128, up to 16384 bf16 keys (2.13 GB): 314 to 319
+// us, 6.7 TB/s, where a plain copy, which writes as well, moves 6.5. The same over e4m3
+// caches (1.06 GB): 213 us, 5.0 TB/s. A single short request is bound by latency: about
 // 4 us for the launch, the lengths, the first loads and the join, then 0.7 us per 128
 // keys of a chunk.
 //
@@ -183,7 +186,8 @@ __device__ __forceinline__ float fast_rcp(float x) {
   return y;
 }
 
-// Score in log2 units. 2 MUFU operations for the cap; exact at both ends (2^inf -> tanh 1).
+// Score in log2 units. 2 MUFU operations for the cap; exact at both ends (2^inf -> tanh 1,
+// so a score of -inf is -cap).
 struct RaggedScore {  // in registers: the parameters are not in constant memory of a function
   float scale, cap_in, cap_out;
   int mods;
@@ -197,7 +201,8 @@ __device__ __forceinline__ float ragged_score(const RaggedScore& sc, float s, fl
 #define GQA_CBAR() asm volatile("bar.sync 1, %0;" ::"n"(CT) : "memory")  // the compute warps
 
 // The compute warps of one streaming CTA, for tiles of up to 16 RG packed rows. Template
-// parameters as gqa_stream_kernel's: FP8 = e4m3 caches (HD 128, both MMAs in f16), NT = at
+// parameters as gqa_stream_kernel's: FP8 = e4m3 caches (HD 128, both MMAs in f16, to which
+// bf16 queries are rounded: exact from 2^-14 to 65504, infinite above), NT = at
 // most 8 rows, MMAs transposed. The scores and the accumulators are fp32; P is rounded to
 // the values' 16-bit type for its MMA, as the dense kernels round it (relative error
 // 2^-9, as large as the output's own rounding).

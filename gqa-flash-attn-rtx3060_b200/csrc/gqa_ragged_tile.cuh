@@ -31,13 +31,14 @@
 //   cap log2 e tanh(y) = s (a0 + a1 s^2 + a2 s^4 + a3 s^6),
 // an odd polynomial fitted to tanh (tests/tanh_fit.py, absolute error 6.5e-7 of the cap)
 // whose last product merges with the subtraction of the maximum: four more operations per
-// pair of scores (packed; 5 % faster than with a scalar square) on the FMA pipe, which the
-// exponentials leave half idle. Tiles with larger scores, rare in models that cap them,
+// pair of scores (packed; 5 % faster than with a scalar square) on the FMA pipe. Neither that
+// pipe nor the MUFU is full: a step waits for the magnitude of all its columns and the vote
+// before P. Tiles with larger scores, rare in models that cap them,
 // take the MUFU form.
 //
 // Measured, 32 query and 8 kv heads of 128, bf16, two prompts' chunks of up to 4096 tokens
-// on up to 12288 cached keys: causal 985 us, 1080 TFLOP/s; capped 1.26 ms (2.3 ms with every
-// tile in the MUFU form); capped and with a distance bias 1.8 ms (3.8 ms). A pair's step
+// on up to 12288 cached keys: causal 985 us, 1080 TFLOP/s; capped 1.24 to 1.33 ms on different
+// boxes (2.3 ms with every tile in the MUFU form); capped and with a distance bias 1.8 ms (3.8 ms). A pair's step
 // of 128 keys takes 2.0 us (the softmax chain, then the wait for its S), a solo step
 // 1.05 us per 128 keys, and a CTA about 10 us besides: the scan 2, the first S 2.5, a
 // masked tile 1.3, the epilogue 3 to 4. Slower, and not kept: P beside S in TMEM, which at

@@ -22,7 +22,7 @@
 // store is fp32.
 //
 // 16381 tokens of 32 query and 8 kv heads of 128, bf16, three axes: 79 to 83 us, 5.1 TB/s, 0.78
-// of a plain copy (units of two rows 85 us, of eight 80 with three CTAs per SM; four CTAs
+// of a plain copy (units of two rows 86 to 88 us, of eight 80 with three CTAs per SM; four CTAs
 // are 64 registers a thread, three hide less latency and take 87, five and six spill; the
 // next unit's rows fetched ahead 94). 16 tokens: 4.6 us, a launch and three dependent loads.
 #pragma once

@@ -10,7 +10,7 @@
 // the vocabulary, so nothing is normalised, and each score is one IEEE subtraction and one
 // IEEE division of the inputs, so the token does not depend on how the row is split. Ties
 // go to the lowest index. A row without a positive score gives the first largest
-// probability.
+// probability. Entries with NaN take no part in either.
 //
 // Bound by HBM for many requests (one row of p, q and e each) and by latency for few:
 // the vocabulary is split over `nsplit` CTAs per request. Each walks the request's drafts
@@ -21,9 +21,9 @@
 // division that is slow for the many zero weights.
 //
 // Measured: 4 requests of a 32000-entry vocabulary 5.7 us; 64 requests of 131071 f32
-// entries (100 MB; odd rows start 4 bytes off, so one array is read by words) 22 us, 0.69 of
-// a plain copy's rate; the greedy form, 64 requests with up to 7 drafts of 131072 bf16
-// logits (91 MB), 20 us, 0.70. Five CTAs per SM of the race and eight of the comparison
+// entries (100 MB; rows start at any word, and a request whose three rows are not all aligned
+// reads each by words) 22 us, 0.70 of a plain copy's rate; the greedy form, 64 requests with
+// up to 7 drafts of 131072 bf16 logits (91 MB), 20 us, 0.70. Five CTAs per SM of the race and eight of the comparison
 // measured best.
 #pragma once
 
@@ -324,7 +324,7 @@ __global__ void __launch_bounds__(kVerifyThreads) gqa_verify_kernel(const Verify
     best = block_best(best);
   }
   if (!(best.score > 0.f)) {
-    // No weight is left (p and q agree where p is not zero, or the row holds NaN): the row's first largest.
+    // No weight is left (p exceeds q nowhere, or only by NaN): the row's first largest.
     best = scan_largest<PT>(prow, 0, p.vocab, false);
     best = block_best(best);
     if (best.index >= p.vocab) best.index = 0;

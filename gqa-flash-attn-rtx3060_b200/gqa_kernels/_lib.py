@@ -74,7 +74,7 @@ SIGNATURES = {
                                   _P]),
 }
 
-# The ragged serving step's entry points take a struct (packed by _serving.py) and a stream.
+# The ragged serving step's entry points take a struct (filled by csrc/serving_ext.cpp) and a stream.
 SIGNATURES.update({
     "gqa_step_plan": (_I, [_P, _P]),
     "gqa_qk_norm_rope": (_I, [_P, _P]),

@@ -313,7 +313,7 @@ class PagedAttention:
             query_len = md.query_len if lens is None else lens[0]
             out = self._attend(q, key_cache, value_cache, md.block_tables, md.seq_lens, md.max_seq_len, query_len)
             return out.view(shape)
-        # Mixed batch: the kernels take one chunk length per call, so the sequences are
+        # Mixed batch: paged_decode and paged_prefill take one chunk length per call, so the sequences are
         # grouped by their new-token count, each group attends in one call, and the rows
         # are gathered from and scattered back to their places in the token order.
         out = torch.empty((num_tokens, self.num_heads, self.head_size), dtype=query.dtype, device=query.device)

@@ -27,8 +27,9 @@ def paged_ragged_attention(query, key_cache, value_cache, block_tables, cu_query
             after the other; head_dim 64 or 128, d stride 1.
         key_cache, value_cache: (num_blocks, block_size, num_kv_heads, head_dim), d stride 1,
             block_size a power of two >= 16; query's dtype, or float8_e4m3fn (head_dim 128)
-            with key = stored key * k_scale and value = stored value * v_scale. num_heads
-            is any multiple (up to 64) of num_kv_heads.
+            with key = stored key * k_scale and value = stored value * v_scale (the products
+            then run in f16: |query| must stay within its range, 65504). num_heads is any
+            multiple (up to 64) of num_kv_heads.
         block_tables: int32 (num_seqs, max_blocks); request b's key k is in block
             block_tables[b, k // block_size] at position k % block_size.
         cu_query_lens: int32 (num_seqs + 1,); request b's tokens are rows
@@ -57,7 +58,9 @@ def paged_ragged_attention(query, key_cache, value_cache, block_tables, cu_query
         (num_tokens, num_heads, head_dim) in query's dtype, and with return_lse float32
         (num_tokens, num_heads). A token that sees no key gives zeros and -inf (where
         gqa_flash_attn and paged_prefill give NaN, the reference's rule: here masks that
-        leave a row empty are ordinary). Asynchronous on the current stream.
+        leave a row empty are ordinary). Cache slots that no token sees may hold anything; a
+        NaN or infinite value that some token of a request sees may reach the request's
+        other tokens as well. Asynchronous on the current stream.
     """
     return (_serving._ext or _serving.load()).ragged(
         query, key_cache, value_cache, block_tables, cu_query_lens, seq_lens, max_query_len, max_seq_len, scale, causal, softcap,

@@ -30,7 +30,8 @@ def verify_drafts(draft_tokens, target_probs, draft_probs, uniforms, exponential
         from what is left of the target's distribution (from its next one when all were
         accepted), then -1; and num_tokens int32 (num_seqs,), how many there are (0 for a
         request without rows). Draft i is accepted while uniforms * draft_prob <
-        target_prob; the drawn token is the first argmax of weight / exponentials.
+        target_prob; the drawn token is the first argmax of weight / exponentials (entries
+        with NaN never are).
         Asynchronous on the current stream.
     """
     return (_serving._ext or _serving.load()).verify(draft_tokens, target_probs, draft_probs, uniforms, exponentials, cu_query_lens,

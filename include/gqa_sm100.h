@@ -329,8 +329,8 @@ int gqa_paged_kv_append(const void* key, const void* value, const int64_t* k_str
  * request, positions, slot_mapping and token_seqs (max_tokens; -1 past the step's
  * tokens). New table entries are written into block_tables. The inputs blocks_held,
  * free_count and context_lens must not be the outputs of the same name. More tokens than
- * max_tokens are dropped and reported (GQA_ERR_INVALID_ARG, site 211). block_size: a
- * power of two.
+ * max_tokens are dropped and reported (GQA_ERR_INVALID_ARG, site 211); cu_query_lens
+ * counts them, and stays at 2^31 - 1 if they are more. block_size: a power of two.
  */
 typedef struct {
   const int* query_lens;
@@ -405,7 +405,7 @@ int gqa_qk_norm_rope(const gqa_qk_norm_rope_args* args, void* stream);
  * - alibi_slopes[head] * |p - key| if given. A token that sees no key gives 0 (unlike
  * gqa_fwd's NaN, which is the reference's rule) and lse -inf. lse (num_tokens,
  * num_heads), float32, natural log, may be NULL. Groups of up to 64 heads, any number.
- * e4m3 caches (cache_fp8, scales as gqa_paged_fwd_kv8) need head_dim 128. max_query_len
+ * e4m3 caches (cache_fp8, scales and range of q as gqa_paged_fwd_kv8) need head_dim 128. max_query_len
  * and max_seq_len bound the lengths and must hold: a request with more tokens may have
  * rows unwritten (reported: GQA_ERR_INVALID_ARG, site 214), keys past max_seq_len are not
  * seen (reported, site 215).
@@ -448,8 +448,8 @@ int gqa_ragged_fwd(const gqa_ragged_args* args, void* stream);
  * NULL: 1 * uniforms); the token after the accepted ones is the argmax over j of
  * max(target[i][j] - draft_probs[b][i][j], 0) / exponentials[b][j] (of target[i][j] /
  * exponentials[b][j] after the last draft; without draft_probs the refused token's
- * weight is 0), ties to the lowest index, or, if no weight is positive, the row's first
- * largest probability. tokens (num_seqs, max_drafts + 1): accepted drafts, then that
+ * weight is 0), ties to the lowest index, NaN left out, or, if no weight is positive, the
+ * row's first largest probability. tokens (num_seqs, max_drafts + 1): accepted drafts, then that
  * token, then -1; num_tokens (num_seqs): how many. A request without rows gives 0
  * tokens. Probabilities share dtype (GQA_DTYPE_F32, _BF16 or _F16); uniforms and
  * exponentials are float32. Strides in elements, the vocabulary's is 1. A draft outside
